@@ -322,6 +322,90 @@ size_t tiermm_qgemm_grouped_ws_bytes(const int* qtype_e, const int* expert_offse
 int tiermm_moe_combine(const float* Y_sorted, const int* token_pairs, const float* pair_weight,
                        float* out, int T, int topk, int N, tiermm_stream_t stream);
 
+/* ------------------------------------- routed tokens, to the experts and back */
+/* No reference functions (the reference refuses MoE models, arch.py:158-159).  T
+ * tokens choose topk experts each: pair i = t * topk + j is token t's j-th choice.
+ * A pair whose expert id lies outside [0, n_experts) is dropped (padding tokens,
+ * full experts): it reaches no expert, and nothing of it enters a sum, its weight
+ * and its rows included, whatever they hold.  Rows are of type TIERMM_F32,
+ * TIERMM_F16 or TIERMM_BF16, strides count elements, and rows may start at any
+ * element (16-byte aligned rows are the fastest).  Sums run in fp32 in a fixed
+ * order and are rounded once, to nearest even; no result depends on the order in
+ * which workgroups run.  At most TIERMM_MOE_MAX_EXPERTS experts and
+ * TIERMM_MOE_MAX_PAIRS pairs (TIERMM_UNSUPPORTED above).  Outputs must not overlap
+ * inputs. */
+#define TIERMM_MOE_MAX_EXPERTS 1024
+#define TIERMM_MOE_MAX_PAIRS (1 << 23)
+/* The order of the pairs by expert, and within an expert by pair:
+ *   expert_offsets[n_experts + 1]  first place of each expert; the last entry is the
+ *                                  number of pairs that are not dropped
+ *   token_pairs[T][topk]           place of each pair, -1 for a dropped one
+ *   sorted_pairs[T * topk]         pair at each place, -1 from expert_offsets[n_experts] up
+ * (the tables that tiermm_qgemm_grouped, from a host copy of the offsets, and
+ * tiermm_moe_combine take).  All are device int32 arrays.  Workspace only where the size query
+ * says so (more than 65536 pairs). */
+int tiermm_moe_plan(const int32_t* expert_ids, int T, int topk, int n_experts, int32_t* expert_offsets,
+                    int32_t* token_pairs, int32_t* sorted_pairs, void* ws, size_t ws_bytes, tiermm_stream_t stream);
+size_t tiermm_moe_plan_ws_bytes(int T, int topk, int n_experts);
+/* X_sorted[p] = X[sorted_pairs[p] / topk], bit for bit, and zeros where no pair is:
+ * every one of the T * topk rows is written. */
+int tiermm_moe_sort(const void* X, int xtype, size_t ldx, const int32_t* token_pairs, const int32_t* sorted_pairs,
+                    void* X_sorted, size_t lds, int T, int topk, int K, tiermm_stream_t stream);
+/* Its gradient: dX[t] = sum_j dX_sorted[token_pairs[t][j]] (zeros where all are dropped). */
+int tiermm_moe_sort_grad(const void* dX_sorted, int xtype, size_t lds, const int32_t* token_pairs, void* dX, size_t ldx,
+                         int T, int topk, int K, tiermm_stream_t stream);
+/* The way back: out[t] = sum_j weights[t][j] * Y_sorted[token_pairs[t][j]], weights fp32
+ * in the router's own order (tiermm_moe_combine takes fp32 rows and weights in the
+ * sorted order). */
+int tiermm_moe_unsort(const void* Y_sorted, int ytype, size_t lds, const int32_t* token_pairs, const float* weights,
+                      void* out, size_t ldo, int T, int topk, int N, tiermm_stream_t stream);
+/* Its gradients: dY_sorted[p] = weights[i] * dout[i / topk], i = sorted_pairs[p], zeros
+ * where no pair is (every row is written); dweights[t][j] = <dout[t],
+ * Y_sorted[token_pairs[t][j]]>, 0 for a dropped pair. */
+int tiermm_moe_unsort_grad(const void* dout, int ytype, size_t ldo, const void* Y_sorted, size_t lds,
+                           const int32_t* token_pairs, const int32_t* sorted_pairs, const float* weights,
+                           void* dY_sorted, size_t ldd, float* dweights, int T, int topk, int N,
+                           tiermm_stream_t stream);
+
+/* ------------------------------ int8 products with a scale for each token and channel */
+/* No reference function.  Both sides are rows of int8 codes with one fp32 scale a row:
+ * Y[m][n] = sx[m] * sw[n] * sum_k Xq[m][k] * Wq[n][k] (+ bias[n]).  The sum is exact
+ * (int32 MFMA; K <= 133120, TIERMM_UNSUPPORTED above), then fp32(sum) * (sx * sw) and
+ * the bias in fp32, and one rounding to the output's type: results do not depend on the
+ * shape of the call.  An int8 row holds tiermm_i8_row_bytes(K) bytes: K codes, then
+ * zeros to a whole number of 128 bytes (rows of x: zeros; what a weight's padding holds
+ * does not matter, but it has to be there).  Row strides rb may be longer, in whole
+ * 16-byte units, from a 16-byte aligned start.
+ * A frozen linear's input gradient is the same product on W transposed and quantized by
+ * its own rows: dX = dY * W with Wt[K][N], tiermm_i8_linear(dY, Wt). */
+size_t tiermm_i8_row_bytes(int K); /* 0 where K is not supported */
+/* Codes and scales of M rows of x (TIERMM_F32, TIERMM_F16 or TIERMM_BF16, ldx elements
+ * apart): scale = max|x| / 127, code = x * (127 / max|x|) rounded to nearest even, each step
+ * in fp32; a zero row has scale 0.  A row that holds a NaN or an infinity gets the scale
+ * NaN and codes 0, so every product of it is NaN.  Weights are laid out by the same call
+ * (rows = output channels). */
+int tiermm_i8_quant(const void* x, int xtype, size_t ldx, int8_t* q, size_t rb, float* scale, int M, int K,
+                    tiermm_stream_t stream);
+/* The product; bias fp32 [N] or NULL; ytype TIERMM_F32, TIERMM_F16 or TIERMM_BF16. */
+int tiermm_i8_gemm(const int8_t* Xq, size_t rbx, const float* sx, const int8_t* W, size_t rbw, const float* sw,
+                   const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K, tiermm_stream_t stream);
+/* tiermm_i8_quant and tiermm_i8_gemm in one call, the same result bit for bit.  ws 16-byte
+ * aligned. */
+int tiermm_i8_linear(const void* x, int xtype, size_t ldx, const int8_t* W, size_t rbw, const float* sw,
+                     const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K, void* ws, size_t ws_bytes,
+                     tiermm_stream_t stream);
+size_t tiermm_i8_linear_ws_bytes(int M, int N, int K);
+/* The experts' products of a routed batch: row p of Y[P][N], expert_offsets[e] <= p <
+ * expert_offsets[e + 1], is row rows[p] / topk of Xq (n_rows of them) times expert e's
+ * weight W + e * N * rbw with the scales sw[e][N].  rows = tiermm_moe_plan's
+ * sorted_pairs: the tokens are quantized once and gathered here, without a sorted copy;
+ * NULL: row p of Xq.  expert_offsets and rows are DEVICE arrays, read by the kernel: no
+ * host copy, and a captured graph follows new routings.  Rows of no expert, and rows
+ * whose index points nowhere, become zeros. */
+int tiermm_i8_gemm_grouped(const int8_t* Xq, size_t rbx, const float* sx, const int32_t* rows, int n_rows, int topk,
+                           const int32_t* expert_offsets, int n_experts, const int8_t* W, size_t rbw, const float* sw,
+                           void* Y, int ytype, size_t ldy, int P, int N, int K, tiermm_stream_t stream);
+
 /* ------------------------------------------------------ host quantizer */
 /* q_row (quant.h:201-204) over `rows` rows of `cols` host floats, writing
  * rows*rb bytes of blocks to host memory `out`: Q8_0 (quant.h:134-136),

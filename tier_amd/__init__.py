@@ -67,6 +67,9 @@ EXPORTS = (
     "tiermm_qgemm_x3parts_ws_bytes",
     "tiermm_split3_f16_ktiled",
     "tiermm_qgemv_batch",
+    "tiermm_moe_plan", "tiermm_moe_plan_ws_bytes", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
+    "tiermm_moe_unsort_grad", "tiermm_i8_row_bytes", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
+    "tiermm_i8_linear_ws_bytes", "tiermm_i8_gemm_grouped",
 )
 
 
@@ -157,6 +160,18 @@ _sig("tiermm_chat_lora_scale", [_vp, _f, _f, _i])
 _sig("tiermm_host_alloc", [_sz, ctypes.POINTER(_vp)])
 _sig("tiermm_host_free", [_vp])
 _sig("tiermm_x3_rows_noalloc", [_vp, _vp, _vp, _i, _i, _i, _i, _vp])
+_sig("tiermm_moe_plan", [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp])
+_sig("tiermm_moe_plan_ws_bytes", [_i, _i, _i], _sz)
+_sig("tiermm_moe_sort", [_vp, _i, _sz, _vp, _vp, _vp, _sz, _i, _i, _i, _vp])
+_sig("tiermm_moe_sort_grad", [_vp, _i, _sz, _vp, _vp, _sz, _i, _i, _i, _vp])
+_sig("tiermm_moe_unsort", [_vp, _i, _sz, _vp, _vp, _vp, _sz, _i, _i, _i, _vp])
+_sig("tiermm_moe_unsort_grad", [_vp, _i, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _vp])
+_sig("tiermm_i8_row_bytes", [_i], _sz)
+_sig("tiermm_i8_quant", [_vp, _i, _sz, _vp, _sz, _vp, _i, _i, _vp])
+_sig("tiermm_i8_gemm", [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _i, _sz, _i, _i, _i, _vp])
+_sig("tiermm_i8_linear", [_vp, _i, _sz, _vp, _sz, _vp, _vp, _vp, _i, _sz, _i, _i, _i, _vp, _sz, _vp])
+_sig("tiermm_i8_linear_ws_bytes", [_i, _i, _i], _sz)
+_sig("tiermm_i8_gemm_grouped", [_vp, _sz, _vp, _vp, _i, _i, _vp, _i, _vp, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _vp])
 NOALLOC_SCRATCH_BYTES = 32 << 20  # TIERMM_NOALLOC_SCRATCH_BYTES
 
 
@@ -433,6 +448,85 @@ def dequant_host(blocks: np.ndarray, qtype: int, cols: int) -> np.ndarray:
 def moe_combine(Y_sorted: int, token_pairs: int, pair_weight: int, out: int, T: int, topk: int, N: int,
                 stream=None) -> None:
     _check(_L.tiermm_moe_combine(Y_sorted, token_pairs, pair_weight, out, T, topk, N, _s(stream)))
+
+
+# ------------------------------------- routed tokens, to the experts and back
+MOE_MAX_EXPERTS, MOE_MAX_PAIRS = 1024, 1 << 23  # TIERMM_MOE_MAX_EXPERTS, TIERMM_MOE_MAX_PAIRS
+
+
+def moe_plan(expert_ids: int, T: int, topk: int, n_experts: int, expert_offsets: int, token_pairs: int,
+             sorted_pairs: int, ws: int | None = None, ws_bytes: int = 0, stream=None) -> None:
+    """The order of T * topk (token, expert) pairs by expert: device int32 tables
+    expert_offsets[n_experts + 1], token_pairs[T][topk] (places), sorted_pairs[T * topk].
+    Ids outside [0, n_experts) are dropped pairs."""
+    _check(_L.tiermm_moe_plan(expert_ids, T, topk, n_experts, expert_offsets, token_pairs, sorted_pairs, ws, ws_bytes,
+                              _s(stream)))
+
+
+def moe_plan_ws_bytes(T: int, topk: int, n_experts: int) -> int:
+    return _L.tiermm_moe_plan_ws_bytes(T, topk, n_experts)
+
+
+def moe_sort(X: int, xtype: int, ldx: int, token_pairs: int, sorted_pairs: int, X_sorted: int, lds: int, T: int,
+             topk: int, K: int, stream=None) -> None:
+    """X_sorted[p] = X[sorted_pairs[p] / topk] (zeros where no pair is); xtype F32, F16 or BF16."""
+    _check(_L.tiermm_moe_sort(X, xtype, ldx, token_pairs, sorted_pairs, X_sorted, lds, T, topk, K, _s(stream)))
+
+
+def moe_sort_grad(dX_sorted: int, xtype: int, lds: int, token_pairs: int, dX: int, ldx: int, T: int, topk: int, K: int,
+                  stream=None) -> None:
+    """dX[t] = sum_j dX_sorted[token_pairs[t][j]]."""
+    _check(_L.tiermm_moe_sort_grad(dX_sorted, xtype, lds, token_pairs, dX, ldx, T, topk, K, _s(stream)))
+
+
+def moe_unsort(Y_sorted: int, ytype: int, lds: int, token_pairs: int, weights: int, out: int, ldo: int, T: int,
+               topk: int, N: int, stream=None) -> None:
+    """out[t] = sum_j weights[t][j] * Y_sorted[token_pairs[t][j]], weights fp32 [T][topk]."""
+    _check(_L.tiermm_moe_unsort(Y_sorted, ytype, lds, token_pairs, weights, out, ldo, T, topk, N, _s(stream)))
+
+
+def moe_unsort_grad(dout: int, ytype: int, ldo: int, Y_sorted: int, lds: int, token_pairs: int, sorted_pairs: int,
+                    weights: int, dY_sorted: int, ldd: int, dweights: int, T: int, topk: int, N: int,
+                    stream=None) -> None:
+    """dY_sorted[p] = w_p * dout[its token] and dweights[t][j] = <dout[t], Y_sorted[token_pairs[t][j]]>."""
+    _check(_L.tiermm_moe_unsort_grad(dout, ytype, ldo, Y_sorted, lds, token_pairs, sorted_pairs, weights, dY_sorted,
+                                     ldd, dweights, T, topk, N, _s(stream)))
+
+
+# ------------------------------------------------------------- int8 products
+def i8_row_bytes(K: int) -> int:
+    """Bytes of an int8 row of K codes: zero-padded to whole 128 bytes."""
+    return _L.tiermm_i8_row_bytes(K)
+
+
+def i8_quant(x: int, xtype: int, ldx: int, q: int, rb: int, scale: int, M: int, K: int, stream=None) -> None:
+    """int8 codes and one fp32 scale for each of M rows of x (F32, F16 or BF16)."""
+    _check(_L.tiermm_i8_quant(x, xtype, ldx, q, rb, scale, M, K, _s(stream)))
+
+
+def i8_gemm(Xq: int, rbx: int, sx: int, W: int, rbw: int, sw: int, bias: int | None, Y: int, ytype: int, ldy: int,
+            M: int, N: int, K: int, stream=None) -> None:
+    """Y[m][n] = sx[m] * sw[n] * <Xq[m], W[n]> (+ bias[n])."""
+    _check(_L.tiermm_i8_gemm(Xq, rbx, sx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, _s(stream)))
+
+
+def i8_linear(x: int, xtype: int, ldx: int, W: int, rbw: int, sw: int, bias: int | None, Y: int, ytype: int, ldy: int,
+              M: int, N: int, K: int, ws: int | None = None, ws_bytes: int = 0, stream=None) -> None:
+    """i8_quant of x and i8_gemm in one call."""
+    _check(_L.tiermm_i8_linear(x, xtype, ldx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, ws, ws_bytes, _s(stream)))
+
+
+def i8_linear_ws_bytes(M: int, N: int, K: int) -> int:
+    return _L.tiermm_i8_linear_ws_bytes(M, N, K)
+
+
+def i8_gemm_grouped(Xq: int, rbx: int, sx: int, rows: int | None, n_rows: int, topk: int, expert_offsets: int,
+                    n_experts: int, W: int, rbw: int, sw: int, Y: int, ytype: int, ldy: int, P: int, N: int, K: int,
+                    stream=None) -> None:
+    """The experts' int8 products of a routed batch, by moe_plan's device tables: row p of Y
+    is row rows[p] / topk of Xq times its expert's weight."""
+    _check(_L.tiermm_i8_gemm_grouped(Xq, rbx, sx, rows, n_rows, topk, expert_offsets, n_experts, W, rbw, sw, Y, ytype,
+                                     ldy, P, N, K, _s(stream)))
 
 
 def qlinear(W: int, qtype: int, rb: int, x: int, y: int, M: int, N: int, K: int, ws: int | None = None,

@@ -21,7 +21,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = ["dequant.hip", "qgemv.hip", "qgemv_dot.hip", "qgemv_q4k.hip", "qgemv_q4k_ws.hip", "qgemv_q6k.hip", "qgemm_fused.hip", "qgemm_skinny.hip", "x3.hip",
-               "noalloc.hip", "host_dequant.hip", "chat_ops.hip"]
+               "noalloc.hip", "host_dequant.hip", "chat_ops.hip", "moe.hip", "i8.hip"]
 CXX_SOURCES = ["api.cpp", "quantize.cpp", "tq.cpp", "chat.cpp"]
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 are generated (hipcc's host pass

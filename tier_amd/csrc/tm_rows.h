@@ -1,0 +1,103 @@
+// tm_rows.h -- rows of fp32, fp16 or bf16 elements, read and written in units of 16
+// bytes as fp32 values.  Rows start wherever their elements may (a stride of any
+// number of elements): the unit types promise no more than the element's alignment,
+// and global memory takes dwordx4 accesses at any address.
+#pragma once
+
+#include "tm_device.h"
+
+namespace tiermm {
+
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
+// Rows of type XT (QT_F32, QT_F16, QT_BF16): ES bytes an element, EPU elements a unit.
+template <int XT>
+struct Rows {
+  static_assert(XT == QT_F32 || XT == QT_F16 || XT == QT_BF16, "row types");
+  static constexpr int ES = XT == QT_F32 ? 4 : 2, EPU = 16 / ES;
+
+  static __device__ __forceinline__ void widen(u32x4 u, float (&v)[EPU]) {
+    if constexpr (XT == QT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = one((uint16_t)(u[i] & 0xffffu));
+        v[2 * i + 1] = one((uint16_t)(u[i] >> 16));
+      }
+    }
+  }
+  // Rounds to nearest even.
+  static __device__ __forceinline__ u32x4 narrow(const float (&v)[EPU]) {
+    u32x4 u;
+    if constexpr (XT == QT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = bits(v[2 * i]) | ((uint32_t)bits(v[2 * i + 1]) << 16);
+    }
+    return u;
+  }
+  static __device__ __forceinline__ u32x4 raw(const uint8_t* p) { return *(const u32x4_a2*)p; }
+  static __device__ __forceinline__ void put(uint8_t* p, u32x4 u) { *(u32x4_a2*)p = u; }
+  // The first n elements at p as a unit (0 behind them), and the first n of a unit to p: bits as they are.
+  static __device__ __forceinline__ u32x4 raw_part(const uint8_t* p, int n) {
+    u32x4 u = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < EPU; ++i) {
+      if (i >= n) break;
+      if constexpr (XT == QT_F32) u[i] = *(const uint32_t*)(p + 4 * i);
+      else u[i >> 1] |= (uint32_t)*(const uint16_t*)(p + 2 * i) << (16 * (i & 1));
+    }
+    return u;
+  }
+  static __device__ __forceinline__ void put_part(uint8_t* p, u32x4 u, int n) {
+#pragma unroll
+    for (int i = 0; i < EPU; ++i) {
+      if (i >= n) break;
+      if constexpr (XT == QT_F32) *(uint32_t*)(p + 4 * i) = u[i];
+      else *(uint16_t*)(p + 2 * i) = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+  // Unit starting at element c of a row of `cols` elements (c < cols).
+  static __device__ __forceinline__ u32x4 get(const uint8_t* row, int c, int cols) {
+    const uint8_t* p = row + (size_t)c * ES;
+    return c + EPU <= cols ? raw(p) : raw_part(p, cols - c);
+  }
+  static __device__ __forceinline__ void set(uint8_t* row, int c, int cols, u32x4 u) {
+    uint8_t* p = row + (size_t)c * ES;
+    if (c + EPU <= cols) put(p, u);
+    else put_part(p, u, cols - c);
+  }
+  static __device__ __forceinline__ void store_one(uint8_t* p, float f) {
+    if constexpr (XT == QT_F32) *(float*)p = f;
+    else *(uint16_t*)p = (uint16_t)bits(f);
+  }
+
+ private:
+  static __device__ __forceinline__ float one(uint16_t h) {
+    if constexpr (XT == QT_F16) return h2f(h);
+    else return __uint_as_float((uint32_t)h << 16);
+  }
+  static __device__ __forceinline__ uint32_t bits(float f) {
+    if constexpr (XT == QT_F16) return f2h(f);
+    else return f2bf(f);
+  }
+};
+
+// Bytes of one element of row type `xtype`, 0 for a type that is none.
+inline int row_elem_bytes(int xtype) {
+  return xtype == QT_F32 ? 4 : xtype == QT_F16 || xtype == QT_BF16 ? 2 : 0;
+}
+
+// f(std::integral_constant<int, XT>) for a row type already checked.
+template <class F>
+inline void with_rows(int xtype, F f) {
+  if (xtype == QT_F32) f(std::integral_constant<int, QT_F32>());
+  else if (xtype == QT_F16) f(std::integral_constant<int, QT_F16>());
+  else f(std::integral_constant<int, QT_BF16>());
+}
+
+}  // namespace tiermm
