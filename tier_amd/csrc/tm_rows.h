@@ -8,7 +8,11 @@
 
 namespace tiermm {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
 
 // Rows of type XT (QT_F32, QT_F16, QT_BF16): ES bytes an element, EPU elements a unit.
 template <int XT>
@@ -36,7 +40,7 @@ struct Rows {
       for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = bits(v[2 * i]) | ((uint32_t)bits(v[2 * i + 1]) << 16);
+      for (int i = 0; i < 4; ++i) u[i] = pair(v[2 * i], v[2 * i + 1]);
     }
     return u;
   }
@@ -71,9 +75,25 @@ struct Rows {
     if (c + EPU <= cols) put(p, u);
     else put_part(p, u, cols - c);
   }
-  static __device__ __forceinline__ void store_one(uint8_t* p, float f) {
-    if constexpr (XT == QT_F32) *(float*)p = f;
-    else *(uint16_t*)p = (uint16_t)bits(f);
+  // Four elements at p (aligned to them).
+  static __device__ __forceinline__ void set4(uint8_t* p, const f32x4& v) {
+    if constexpr (XT == QT_F32) *(f32x4*)p = v;
+    else *(u32x2*)p = u32x2{pair(v[0], v[1]), pair(v[2], v[3])};
+  }
+  // The first n of four elements to p, which is aligned to one.
+  static __device__ __forceinline__ void put4(uint8_t* p, const float (&v)[4], int n) {
+    if (n == 4) {
+      if constexpr (XT == QT_F32) *(u32x4_a2*)p = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                        __float_as_uint(v[2]), __float_as_uint(v[3])};
+      else *(u32x2_a2*)p = u32x2{pair(v[0], v[1]), pair(v[2], v[3])};
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= n) break;
+      if constexpr (XT == QT_F32) *(float*)(p + 4 * i) = v[i];
+      else *(uint16_t*)(p + 2 * i) = (uint16_t)pair(v[i], 0.f);
+    }
   }
 
  private:
@@ -81,9 +101,10 @@ struct Rows {
     if constexpr (XT == QT_F16) return h2f(h);
     else return __uint_as_float((uint32_t)h << 16);
   }
-  static __device__ __forceinline__ uint32_t bits(float f) {
-    if constexpr (XT == QT_F16) return f2h(f);
-    else return f2bf(f);
+  // v_cvt_pk_bf16_f32 rounds to nearest even, two at a time, and keeps NaN.
+  static __device__ __forceinline__ uint32_t pair(float a, float b) {
+    if constexpr (XT == QT_F16) return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
   }
 };
 
