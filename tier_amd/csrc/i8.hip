@@ -12,8 +12,10 @@
 #include "tm_rows.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace tiermm {
+int device_cus(int* cus);
 namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -109,10 +111,11 @@ struct I8Args {
   int E, topk, xrows;
 };
 
-// The rows of Y that a workgroup's tile covers.
+// What a workgroup computes: rows [m0, m1) of Y, column tile tn.
 struct Tile {
-  int m0, m1, tn;   // rows [m0, m1), column tile
-  int e;            // expert; E: rows that no expert has, which become zeros
+  int m0, m1, tn;
+  int e;      // expert; E: rows that no expert has, which become zeros
+  bool once;  // no other tile reads these rows of W
 };
 
 // Tile `t` of the workgroups' sequence in which XCD x (blockIdx % 8) walks the x-th
@@ -161,6 +164,7 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
       tl.tn = in / ntm;
       tl.m0 = r0 + (in % ntm) * BM;
       tl.m1 = min(tl.m0 + BM, r0 + nr);
+      tl.once = ntm == 1;
       return true;
     }
     run += __shfl(s, 63, 64);
@@ -168,12 +172,49 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
   return false;
 }
 
+// The tile of this workgroup; false past the last.  Dense tiles go in groups of 4 tile rows,
+// column by column.
+template <int BM, int BN, bool GROUPED>
+__device__ __forceinline__ bool find_tile(const I8Args& a, Tile& tl) {
+  const int ntn = (a.N + BN - 1) / BN;
+  if constexpr (GROUPED) return grouped_tile<BM>(a, ntn, blockIdx.x, tl);
+  const int ntm = (a.M + BM - 1) / BM, t = xcd_share(blockIdx.x, ntm * ntn);
+  if (t < 0) return false;
+  constexpr int GM = 4;
+  const int grp = t / (GM * ntn), first = grp * GM, gm = min(GM, ntm - first), in = t - grp * GM * ntn;
+  tl.m0 = (first + in % gm) * BM;
+  tl.m1 = min(tl.m0 + BM, a.M);
+  tl.tn = in / gm;
+  tl.e = 0;
+  tl.once = ntm == 1;
+  return true;
+}
+
 // Row of X behind row p of Y, or -1.
+template <bool GROUPED>
 __device__ __forceinline__ int source_row(const I8Args& a, int p) {
+  if constexpr (!GROUPED) return p;
   if (!a.rows) return p < a.xrows ? p : -1;
   const int i = a.rows[p];
   const int r = i < 0 ? -1 : i / a.topk;
   return r < a.xrows ? r : -1;
+}
+
+// Start of row r of a stage of BM rows of X and BN of W (rows past the tile: its last one).
+template <int BM, bool GROUPED>
+__device__ __forceinline__ const uint8_t* stage_row(const I8Args& a, const Tile& tl, int n0, int r) {
+  if (r < BM) return a.X + (size_t)max(source_row<GROUPED>(a, min(tl.m0 + r, tl.m1 - 1)), 0) * a.rbx;
+  const uint8_t* W = a.W + (GROUPED ? (size_t)tl.e * a.N * a.rbw : 0);
+  return W + (size_t)min(n0 + r - BM, a.N - 1) * a.rbw;
+}
+
+// Columns n0 .. n0 + BN - 1 of the tile's rows become zeros.
+template <class Y, int BN, int THREADS>
+__device__ __forceinline__ void zero_tile(const I8Args& a, const Tile& tl, int n0) {
+  const int cols = min(BN, a.N - n0);
+  for (int m = tl.m0; m < tl.m1; ++m)
+    for (int c = threadIdx.x * Y::EPU; c < cols; c += THREADS * Y::EPU)
+      Y::set(a.Y + (size_t)m * a.ldy + (size_t)n0 * Y::ES, c, cols, u32x4{0u, 0u, 0u, 0u});
 }
 
 // One element of Y: the sum rounded to fp32, times sx * sw, plus the bias (0: none).
@@ -204,7 +245,7 @@ __device__ __forceinline__ void wave_lds_wait() {
 // way from the step after the barrier that frees their place on.
 //
 // W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y.
-template <int YT, int BM, int BN, int WVM, int WVN, bool GROUPED>
+template <int YT, int BM, int BN, int WVM, int WVN, int S, bool GROUPED>
 __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, NM = WM * WN, NF = WM + WN;
   constexpr int STAGE = (BM + BN) * kStep, INST = STAGE / 1024 / NW;
@@ -212,59 +253,36 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   // loads of a stage by the step that issues them: 3 (of the stage before last), 0 and 1
   constexpr int D0 = (INST + 2) / 3, D1 = (INST - D0 + 1) / 2, D2 = INST - D0 - D1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  float* col_scale = (float*)(lds + 2 * STAGE);
+  float* col_scale = (float*)(lds + S * STAGE);
   float* col_bias = col_scale + BN;
   float* row_scale = col_bias + BN;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ntn = (a.N + BN - 1) / BN;
-
   Tile tl;
-  if constexpr (GROUPED) {
-    if (!grouped_tile<BM>(a, ntn, blockIdx.x, tl)) return;
-  } else {
-    const int ntm = (a.M + BM - 1) / BM, t = xcd_share(blockIdx.x, ntm * ntn);
-    if (t < 0) return;
-    constexpr int GM = 4;  // groups of 4 tile rows, column by column
-    const int grp = t / (GM * ntn), first = grp * GM, gm = min(GM, ntm - first), in = t - grp * GM * ntn;
-    tl.m0 = (first + in % gm) * BM;
-    tl.m1 = min(tl.m0 + BM, a.M);
-    tl.tn = in / gm;
-    tl.e = 0;
-  }
+  if (!find_tile<BM, BN, GROUPED>(a, tl)) return;
   const int n0 = tl.tn * BN;
   using Y = Rows<YT>;
-
-  if (GROUPED && tl.e == a.E) {  // rows of no expert
-    const int cols = min(BN, a.N - n0);
-    for (int m = tl.m0; m < tl.m1; ++m)
-      for (int c = tid * Y::EPU; c < cols; c += 64 * NW * Y::EPU)
-        Y::set(a.Y + (size_t)m * a.ldy + (size_t)n0 * Y::ES, c, cols, u32x4{0u, 0u, 0u, 0u});
-    return;
-  }
-  const uint8_t* W = a.W + (GROUPED ? (size_t)tl.e * a.N * a.rbw : 0);
+  if (GROUPED && tl.e == a.E) return zero_tile<Y, BN, 64 * NW>(a, tl, n0);
   const float* sw = a.sw + (GROUPED ? (size_t)tl.e * a.N : 0);
 
   // load u of this wave: rows 8 * (wave + NW * u) .. + 7 of the stage (X's, then W's)
   const uint8_t* src[INST];
-  const int slot = lane & 7, lr = lane >> 3;
 #pragma unroll
   for (int u = 0; u < INST; ++u) {
-    const int r = 8 * (wave + NW * u) + lr, c = slot ^ ((r >> 1) & 7);
-    if (r < BM) {
-      const int m = min(tl.m0 + r, tl.m1 - 1);
-      const int xr = GROUPED ? max(source_row(a, m), 0) : m;
-      src[u] = a.X + (size_t)xr * a.rbx + c * 16;
-    } else {
-      src[u] = W + (size_t)min(n0 + r - BM, a.N - 1) * a.rbw + c * 16;
-    }
+    const int r = 8 * (wave + NW * u) + (lane >> 3);
+    src[u] = stage_row<BM, GROUPED>(a, tl, n0, r) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
   }
   const uint32_t lds0 = lds_addr(lds);
+  auto ring = [](int kt) { return S == 2 ? kt & 1 : S == 4 ? kt & 3 : kt % S; };
   auto issue = [&](int kt, int u) __attribute__((always_inline)) {
-    dma16(src[u] + (size_t)kt * kStep, lds0 + (kt & 1) * STAGE + (wave + NW * u) * 1024);
+    dma16(src[u] + (size_t)kt * kStep, lds0 + ring(kt) * STAGE + (wave + NW * u) * 1024);
   };
 #pragma unroll
-  for (int u = 0; u < INST; ++u) issue(0, u);
+  for (int t = 0; t < S - 1; ++t)
+    if (t < a.nk) {
+#pragma unroll
+      for (int u = 0; u < INST; ++u) issue(t, u);
+    }
 
   // the scales of the tile's rows and columns, for the end; NaN-free zeros where a row has no source
   for (int i = tid; i < BN; i += 64 * NW) {
@@ -273,7 +291,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     col_bias[i] = a.bias ? a.bias[n] : 0.f;
   }
   for (int i = tid; i < BM; i += 64 * NW) {
-    const int m = min(tl.m0 + i, tl.m1 - 1), xr = GROUPED ? source_row(a, m) : m;
+    const int xr = source_row<GROUPED>(a, min(tl.m0 + i, tl.m1 - 1));
     row_scale[i] = xr < 0 ? 0.f : a.sx[xr];
   }
 
@@ -290,7 +308,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   i32x4 xf[2][WM], wf[2][WN];
   // fragment v of step kk of stage kt into set f: W's first, X's, W's others, as the products need them
   auto fragment = [&](int kt, int kk, int f, int v) __attribute__((always_inline)) {
-    const uint8_t* s = lds + (kt & 1) * STAGE + ((2 * kk + fh) ^ turn) * 16;
+    const uint8_t* s = lds + ring(kt) * STAGE + ((2 * kk + fh) ^ turn) * 16;
     if (v >= 1 && v <= WM) xf[f][v - 1] = *(const i32x4*)(s + xrow + (v - 1) * 32 * kStep);
     else wf[f][v == 0 ? 0 : v - WM] = *(const i32x4*)(s + wrow + (v == 0 ? 0 : v - WM) * 32 * kStep);
   };
@@ -302,38 +320,45 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     for (int q = 0; q < NM; ++q) {
 #pragma unroll
       for (int v = 0; v < NF; ++v)
-        if (v * (NM - 2) / NF == q) fragment(kt, kk, f ^ 1, v);
+        if (std::max(v * (NM - 2) / NF, 0) == q) fragment(kt, kk, f ^ 1, v);
 #pragma unroll
       for (int d = 0; d < n; ++d)
-        if (1 + d * (NM - 1) / n == q && dt < a.nk) issue(dt, u0 + d);
+        if (std::min(1 + d * (NM - 1) / n, NM - 1) == q && dt < a.nk) issue(dt, u0 + d);
       const int j = q / WM, i = q % WM;
       acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[f][j], xf[f][i], acc[j][i], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  vm_wait<0>();
+  // waits until stage kt has landed, those up to kt + S - 2 being on their way too
+  auto landed = [&](int kt) __attribute__((always_inline)) {
+    const int behind = a.nk - 1 - kt;
+    if (behind >= S - 2) vm_wait<(S - 2) * INST>();
+    else if (S > 3 && behind == 1) vm_wait<INST>();
+    else vm_wait<0>();
+  };
+  landed(0);
   __syncthreads();
-  if (a.nk > 1) {
+  if (S - 1 < a.nk) {
 #pragma unroll
-    for (int u = 0; u < D0; ++u) issue(1, u);
+    for (int u = 0; u < D0; ++u) issue(S - 1, u);
   }
 #pragma unroll
   for (int v = 0; v < NF; ++v) fragment(0, 0, 0, v);
   for (int kt = 0; kt < a.nk; ++kt) {
-    step(0, kt, 1, kt + 1, D0, D1);
-    step(1, kt, 2, kt + 1, D0 + D1, D2);
-    step(0, kt, 3, kt + 1, 0, 0);
-    vm_wait<0>();
+    step(0, kt, 1, kt + S - 1, D0, D1);
+    step(1, kt, 2, kt + S - 1, D0 + D1, D2);
+    step(0, kt, 3, 0, 0, 0);
+    landed(kt + 1);
     __syncthreads();  // stage kt + 1 has landed for every wave, and stage kt is read
     // (past the end: the fragments of what the place holds, which nothing uses)
-    step(1, kt + 1, 0, kt + 2, 0, D0);
+    step(1, kt + 1, 0, kt + S, 0, D0);
   }
 
   // Element r of a block is column 8 * (r / 4) + 4 * fh + r % 4 of row fr: a lane's own
   // stores would be 4 columns wide.  Each wave passes 32 rows of one or two blocks at a
   // time through its part of LDS and stores whole 16-byte units, 8 of them a row.
   constexpr int JB = Y::ES == 2 ? 2 : 1, PART = 4096;
-  static_assert(NW * PART <= 2 * STAGE, "rows of the epilogue in LDS");
+  static_assert(NW * PART <= S * STAGE, "rows of the epilogue in LDS");
   uint8_t* part = lds + wave * PART;
   auto store = [&](auto jn, int j0) __attribute__((always_inline)) {
     constexpr int J = decltype(jn)::value, CH = J * 32 * Y::ES / 16;
@@ -370,225 +395,346 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   if constexpr (WN % JB) store(std::integral_constant<int, WN % JB>(), WN - WN % JB);
 }
 
-template <int YT, int BM, int BN, int WVM, int WVN, bool GROUPED>
-int launch_gemm(const I8Args& a, hipStream_t s, const char* who) {
-  constexpr int LDS = 2 * (BM + BN) * kStep + (BM + 2 * BN) * 4;
-  static_assert(LDS <= 160 * 1024, "LDS of a CU");
-  static std::atomic<uint64_t> done{0};
-  auto* fn = i8_gemm_kernel<YT, BM, BN, WVM, WVN, GROUPED>;
-  const int st = lds_attr_once(done, (const void*)fn, LDS, who);
+// Launches fn over the tiles; grouped, every expert may end in a partly filled one.
+template <class Fn>
+int launch(Fn* fn, std::atomic<uint64_t>& done, const I8Args& a, bool grouped, int bm, int bn, int threads, int lds,
+           hipStream_t s, const char* who) {
+  const int st = lds_attr_once(done, (const void*)fn, lds, who);
   if (st != TIERMM_OK) return st;
-  const long long ntn = (a.N + BN - 1) / BN;
-  // grouped: every group may end in a partly filled tile
-  const long long ntm = GROUPED ? a.M / BM + std::min(a.E, a.M) + 1 : (a.M + BM - 1) / BM;
+  const long long ntn = (a.N + bn - 1) / bn;
+  const long long ntm = grouped ? a.M / bm + std::min(a.E, a.M) + 1 : (a.M + bm - 1) / bm;
   const long long grid = (ntm * ntn + 7) / 8 * 8;
   if (grid > (1ll << 22)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, ntm * ntn);
-  fn<<<(unsigned)grid, 64 * WVM * WVN, LDS, s>>>(a);
+  fn<<<(unsigned)grid, threads, lds, s>>>(a);
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
 }
 
-// Few rows: the product is bound by the bytes of W, each read once.  A workgroup takes 16 * NF
-// rows of W and up to 16 * MT rows of X; its NW waves share K, wave w taking the 128-byte chunks
-// w, w + NW, .. of every row.  Both operands go straight to registers (an MFMA 16x16x64 operand
-// is 16 rows of 64 bytes), so nothing is staged and no wave waits for another until the end,
-// where the waves' sums meet in LDS.
-//
-// XT >= 0: x comes as M <= 16 * MT rows of that type and the workgroup quantizes them into
-// LDS itself, the weight's first chunks already on their way.
-template <int YT, int XT, int MT, int NF, int NW, bool GROUPED>
-__global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const I8Args a) {
-  constexpr bool FUSED = XT >= 0;
-  constexpr int BN = 16 * NF, BM = 16 * MT;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ntn = (a.N + BN - 1) / BN;
-  Tile tl;
-  if constexpr (GROUPED) {
-    if (!grouped_tile<BM>(a, ntn, blockIdx.x, tl)) return;
-  } else {
-    tl = {0, a.M, (int)blockIdx.x, 0};
-  }
-  const int n0 = tl.tn * BN;
-  using Y = Rows<YT>;
-  if (GROUPED && tl.e == a.E) {  // rows of no expert
-    const int cols = min(BN, a.N - n0);
-    for (int m = tl.m0; m < tl.m1; ++m)
-      for (int c = tid * Y::EPU; c < cols; c += 64 * NW * Y::EPU)
-        Y::set(a.Y + (size_t)m * a.ldy + (size_t)n0 * Y::ES, c, cols, u32x4{0u, 0u, 0u, 0u});
-    return;
-  }
-  const uint8_t* W = a.W + (GROUPED ? (size_t)tl.e * a.N * a.rbw : 0);
-  const float* sw = a.sw + (GROUPED ? (size_t)tl.e * a.N : 0);
+template <int YT, int BM, int BN, int WVM, int WVN, int S, bool GROUPED>
+int launch_gemm(const I8Args& a, hipStream_t s, const char* who) {
+  constexpr int LDS = S * (BM + BN) * kStep + (BM + 2 * BN) * 4;
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static std::atomic<uint64_t> done{0};
+  return launch(i8_gemm_kernel<YT, BM, BN, WVM, WVN, S, GROUPED>, done, a, GROUPED, BM, BN, 64 * WVM * WVN, LDS, s, who);
+}
 
-  const uint8_t* wp[NF];
-  const uint8_t* xp[MT];
+// ----------------------------------------------------------------- single tokens
+// Sum of two wave-wide vectors' halves (32) or rows of 16 lanes (16): the lanes of one half
+// then hold a's sums, the others' b's.
+__device__ __forceinline__ int merge32(int a, int b) {
+  const auto t = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return (int)t[0] + (int)t[1];
+}
+__device__ __forceinline__ int merge16(int a, int b) {
+  const auto t = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  return (int)t[0] + (int)t[1];
+}
+template <int CTRL>
+__device__ __forceinline__ int add_ror(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+// Wave-wide sums of v[0 .. R): lanes 16 g .. + 15 hold that of v[g * R / 4].
+template <int R>
+__device__ __forceinline__ int wave_sums(const int (&v)[R]) {
+  int s;
+  if constexpr (R == 2) { const int h = merge32(v[0], v[1]); s = merge16(h, h); }
+  else { const int h = merge32(v[0], v[0]); s = merge16(h, h); }
+  return add_ror<0x121>(add_ror<0x122>(add_ror<0x124>(add_ror<0x128>(s))));  // row_ror 8, 4, 2, 1
+}
+
+// Up to MX rows of x, quantized by each workgroup into LDS while its first weights are on the
+// way.  A wave takes R rows of W in 1 KiB pieces, 16 bytes a lane, so each load is eight whole
+// lines of one row; v_dot4 on 16 bytes a lane costs a tenth of what the bytes take to come.
+template <int YT, int XT, int MX, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t codes[];  // [MX][whole KiB]
+  __shared__ float row_scale[MX];
+  __shared__ uint32_t red[MX][NW];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Kp = a.nk * kStep, nc = (Kp + 1023) >> 10, ldc = nc << 10;
+  const int n0 = (blockIdx.x * NW + wave) * R;
+  const uint8_t* wp[R];
 #pragma unroll
-  for (int f = 0; f < NF; ++f) wp[f] = W + (size_t)min(n0 + 16 * f + r, a.N - 1) * a.rbw + 16 * g;
-  if constexpr (!FUSED) {
+  for (int r = 0; r < R; ++r) wp[r] = a.W + (size_t)min(n0 + r, a.N - 1) * a.rbw + 16 * lane;
+  constexpr int U = 4;  // pieces in flight
+  i32x4 q[U][R];
+  auto load = [&](int u, int c) __attribute__((always_inline)) {
+    const bool in = (c << 10) + 16 * lane < Kp;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int m = min(tl.m0 + 16 * t + r, tl.m1 - 1);
-      xp[t] = a.X + (size_t)(GROUPED ? max(source_row(a, m), 0) : m) * a.rbx + 16 * g;
-    }
-  }
-  // operands of one chunk: two steps of 64 bytes
-  struct Chunk {
-    i32x4 w[2][NF], x[2][FUSED ? 1 : MT];
+    for (int r = 0; r < R; ++r)
+      q[u][r] = in ? __builtin_nontemporal_load((const i32x4*)(wp[r] + ((size_t)c << 10))) : i32x4{0, 0, 0, 0};
   };
-  auto load = [&](Chunk& q, int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int f = 0; f < NF; ++f) q.w[h][f] = *(const i32x4*)(wp[f] + (size_t)c * kStep + 64 * h);
-      if constexpr (!FUSED) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) q.x[h][t] = *(const i32x4*)(xp[t] + (size_t)c * kStep + 64 * h);
-      }
-    }
-  };
-  i32x4 acc[NF][MT] = {};
-  uint8_t* codes = lds + NW * NF * MT * 1024;  // FUSED: [M][nk * 128]
-  auto mul = [&](const Chunk& q, int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        i32x4 x;
-        if constexpr (FUSED)
-          x = *(const i32x4*)(codes + (size_t)min(16 * t + r, a.M - 1) * a.nk * kStep + c * kStep + 64 * h + 16 * g);
-        else
-          x = q.x[h][t];
-#pragma unroll
-        for (int f = 0; f < NF; ++f) acc[f][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.w[h][f], x, acc[f][t], 0, 0, 0);
-      }
-  };
-  constexpr int U = MT + NF <= 2 ? 3 : MT + NF <= 3 ? 2 : 1;  // chunks in flight
-  Chunk q[U];
-  int c = wave;
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (c + u * NW < a.nk) load(q[u], c + u * NW);
+    if (u < nc) load(u, u);
 
-  __shared__ float row_scale[BM];
-  if constexpr (FUSED) {
-    using X = Rows<XT < 0 ? QT_F32 : XT>;
-    __shared__ uint32_t red[NW];
-    const int K = a.K, Kp = a.nk * kStep;
-    for (int m = 0; m < a.M; ++m) {
-      const uint8_t* row = a.X + (size_t)m * a.rbx;
-      uint32_t top = 0;
-      for (int k = tid * X::EPU; k < K; k += 64 * NW * X::EPU) {
-        float v[X::EPU];
-        X::widen(X::get(row, k, K), v);
-        top = top_bits(v, top);
-      }
+  using X = Rows<XT>;
+  uint32_t top[MX] = {};
+  for (int k = tid * X::EPU; k < a.K; k += 64 * NW * X::EPU)
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-      if (lane == 0) red[wave] = top;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < NW; ++w) top = max(top, red[w]);
-      const RowScale s = row_scale_of(top);
-      for (int k = tid * X::EPU; k < Kp; k += 64 * NW * X::EPU) {
-        float v[X::EPU] = {};
-        if (k < K) X::widen(X::get(row, k, K), v);
-#pragma unroll
-        for (int i = 0; i < X::EPU; i += 4) *(uint32_t*)(codes + (size_t)m * Kp + k + i) = codes4(v + i, s);
-      }
-      if (tid == 0) row_scale[m] = s.sc;
-      __syncthreads();
+    for (int m = 0; m < MX; ++m) {
+      float v[X::EPU];
+      X::widen(X::get(a.X + (size_t)min(m, a.M - 1) * a.rbx, k, a.K), v);
+      top[m] = top_bits(v, top[m]);
     }
-  } else {
-    if (tid < BM) {
-      const int m = min(tl.m0 + tid, tl.m1 - 1), xr = GROUPED ? source_row(a, m) : m;
-      row_scale[tid] = xr < 0 ? 0.f : a.sx[xr];
+#pragma unroll
+  for (int m = 0; m < MX; ++m) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top[m] = max(top[m], (uint32_t)__shfl_xor((int)top[m], o, 64));
+    if (lane == 0) red[m][wave] = top[m];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < MX; ++m) {
+    #pragma unroll
+    for (int w = 0; w < NW; ++w) top[m] = max(top[m], red[m][w]);
+    const RowScale s = row_scale_of(top[m]);
+    if (tid == 0) row_scale[m] = s.sc;
+    for (int k = tid * X::EPU; k < Kp; k += 64 * NW * X::EPU) {
+      float v[X::EPU] = {};
+      if (k < a.K) X::widen(X::get(a.X + (size_t)min(m, a.M - 1) * a.rbx, k, a.K), v);
+#pragma unroll
+      for (int i = 0; i < X::EPU; i += 4) *(uint32_t*)(codes + m * ldc + k + i) = codes4(v + i, s);
     }
   }
+  __syncthreads();
 
-  while (c < a.nk) {
+  int acc[MX][R] = {};
+  for (int c0 = 0; c0 < nc; c0 += U)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (c >= a.nk) break;
-      mul(q[u], c);
-      if (c + U * NW < a.nk) load(q[u], c + U * NW);
-      c += NW;
+      const int c = c0 + u;
+      if (c >= nc) break;
+#pragma unroll
+      for (int m = 0; m < MX; ++m) {
+        // past the padded row both sides may be anything but the weight, which is 0
+        const i32x4 x = *(const i32x4*)(codes + m * ldc + (c << 10) + 16 * lane);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][r] = __builtin_amdgcn_sdot4(q[u][r][i], x[i], acc[m][r], false);
+      }
+      if (c + U < nc) load(u, c + U);
+    }
+  using Y = Rows<YT>;
+  const int n = n0 + (lane >> 4) * R / 4;
+#pragma unroll
+  for (int m = 0; m < MX; ++m) {
+    const int sum = wave_sums<R>(acc[m]);
+    if (m < a.M && (lane & 15) == 0 && lane % (64 / R) == 0 && n < a.N) {
+      const float v[4] = {scaled(sum, row_scale[m], a.sw[n], a.bias ? a.bias[n] : 0.f), 0.f, 0.f, 0.f};
+      Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, v, 1);
     }
   }
+}
 
-  // element i of a sum is column 4 * g + i of row r
-  i32x4* sums = (i32x4*)lds;
+template <int YT, int XT, int MX, int R, int NW>
+int launch_gemv(const I8Args& a, hipStream_t s, const char* who) {
+  const int ldc = (a.nk * kStep + 1023) / 1024 * 1024;
+  i8_gemv_kernel<YT, XT, MX, R, NW><<<(a.N + NW * R - 1) / (NW * R), 64 * NW, MX * ldc, s>>>(a);
+  TM_LAUNCH_CHECK(who);
+  return TIERMM_OK;
+}
+
+// Few rows: the product is bound by the bytes of W.  A workgroup takes a BM x BN tile; its
+// WVN x WVK waves share the columns and the 64-byte steps of a stage, which holds KS * 128 bytes
+// of every row.  A ring of S stages keeps S - 1 on their way by global_load_lds, whole lines of
+// eight rows a load; one barrier a stage.
+template <int YT, int BM, int BN, int WVN, int WVK, int KS, int S, bool GROUPED>
+__global__ __launch_bounds__(64 * WVN * WVK) void i8_tile_kernel(const I8Args a) {
+  constexpr int NW = WVN * WVK, MB = BM / 16, NB = BN / WVN / 16, KK = 2 * KS / WVK;
+  constexpr int SUB = (BM + BN) * kStep, STAGE = KS * SUB, INST = STAGE / 1024 / NW;
+  static_assert(INST * NW * 1024 == STAGE && KK * WVK == 2 * KS && NB * WVN * 16 == BN, "whole loads, steps and blocks a wave");
+  constexpr int LDO = BN + 4;  // dwords of a row of sums
+  static_assert(WVK * BM * LDO * 4 <= S * STAGE, "sums in LDS");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Tile tl;
+  if (!find_tile<BM, BN, GROUPED>(a, tl)) return;
+  const int n0 = tl.tn * BN;
+  using Y = Rows<YT>;
+  if (GROUPED && tl.e == a.E) return zero_tile<Y, BN, 64 * NW>(a, tl, n0);
+  const float* sw = a.sw + (GROUPED ? (size_t)tl.e * a.N : 0);
+
+  // load u of this wave: eight rows of a sub-stage (X's, then W's)
+  const uint8_t* src[INST];
 #pragma unroll
-  for (int f = 0; f < NF; ++f)
+  for (int u = 0; u < INST; ++u) {
+    const int r = (8 * (wave + NW * u) + (lane >> 3)) % (BM + BN);
+    src[u] = stage_row<BM, GROUPED>(a, tl, n0, r) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+  }
+  const uint32_t lds0 = lds_addr(lds);
+  const int ns = (a.nk + KS - 1) / KS;
+  int put = 0;
+  auto issue = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) sums[(wave * NF * MT + f * MT + t) * 64 + lane] = acc[f][t];
+    for (int u = 0; u < INST; ++u) {
+      const int i = 8 * (wave + NW * u), r = i % (BM + BN);
+      // steps past the end load the last one again, and are not multiplied
+      const size_t k = (size_t)(KS == 1 ? st : min(st * KS + i / (BM + BN), a.nk - 1)) * kStep;
+      const uint32_t to = lds0 + put * STAGE + (wave + NW * u) * 1024;
+      if (tl.once && r >= BM) dma16_nt(src[u] + k, to);
+      else dma16(src[u] + k, to);
+    }
+    put = put + 1 == S ? 0 : put + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i)
+    if (i < ns) issue(i);
+
+  i32x4 acc[NB][MB] = {};
+  const int wn = wave % WVN, wk = wave / WVN, fr = lane & 15, fg = lane >> 4, turn = (fr >> 1) & 7;
+  int get = 0;
+  for (int st = 0; st < ns; ++st) {
+    const int after = ns - 1 - st;  // stages on their way behind this one
+    if (after >= S - 2) vm_wait<(S - 2) * INST>();
+    else if (S > 6 && after == 4) vm_wait<4 * INST>();
+    else if (S > 5 && after == 3) vm_wait<3 * INST>();
+    else if (S > 4 && after == 2) vm_wait<2 * INST>();
+    else if (S > 3 && after == 1) vm_wait<INST>();
+    else vm_wait<0>();
+    __syncthreads();  // stage st has landed for every wave, and the one before it is read
+    if (st + S - 1 < ns) issue(st + S - 1);
+    const uint8_t* s = lds + get * STAGE;
+    get = get + 1 == S ? 0 : get + 1;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      const int step = wk * KK + k, sub = step >> 1;
+      if (KS > 1 && st * KS + sub >= a.nk) break;
+      const uint8_t* p = s + sub * SUB + fr * kStep + ((4 * (step & 1) + fg) ^ turn) * 16;
+      i32x4 xf[MB], wf[NB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) xf[i] = *(const i32x4*)(p + i * 16 * kStep);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(p + (BM + (wn * NB + j) * 16) * kStep);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+    }
+  }
   __syncthreads();
-  for (int i = tid; i < NF * MT * 64; i += 64 * NW) {
-    const int f = i / (MT * 64), t = i / 64 % MT, m = tl.m0 + 16 * t + r, n = n0 + 16 * f + 4 * g;
-    if (m >= tl.m1 || n >= a.N) continue;
-    i32x4 v = sums[i];
+  // a lane's sum is columns 4 * fg .. + 3 of row fr of each block
+  int32_t* sums = (int32_t*)lds;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += sums[w * NF * MT * 64 + i];
-    const float s = row_scale[16 * t + r];
-    uint8_t* y = a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES;
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      *(i32x4*)(sums + (wk * BM + i * 16 + fr) * LDO + (wn * NB + j) * 16 + 4 * fg) = acc[j][i];
+  __syncthreads();
+  for (int q = tid; q < BM * BN / 4; q += 64 * NW) {
+    const int r = q / (BN / 4), c = q % (BN / 4) * 4, m = tl.m0 + r, n = n0 + c;
+    if (m >= tl.m1 || n >= a.N) continue;
+    i32x4 v = *(const i32x4*)(sums + r * LDO + c);
+#pragma unroll
+    for (int w = 1; w < WVK; ++w) v += *(const i32x4*)(sums + (w * BM + r) * LDO + c);
+    const int xr = source_row<GROUPED>(a, m);
+    const float sc = xr < 0 ? 0.f : a.sx[xr];
     float o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int nn = min(n + k, a.N - 1);
-      o[k] = scaled(v[k], s, sw[nn], a.bias ? a.bias[nn] : 0.f);
+      o[k] = scaled(v[k], sc, sw[nn], a.bias ? a.bias[nn] : 0.f);
     }
-    Y::put4(y, o, min(4, a.N - n));
+    Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, min(4, a.N - n));
   }
 }
 
-template <int YT, int XT, int MT, int NF, int NW, bool GROUPED>
-int launch_rows(const I8Args& a, hipStream_t s, const char* who) {
-  const int LDS = NW * NF * MT * 1024 + (XT >= 0 ? a.M * a.nk * kStep : 0);
+template <int YT, int BM, int BN, int WVN, int WVK, int KS, int S, bool GROUPED>
+int launch_tile(const I8Args& a, hipStream_t s, const char* who) {
+  constexpr int LDS = S * KS * (BM + BN) * kStep;
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> done{0};
-  auto* fn = i8_rows_kernel<YT, XT, MT, NF, NW, GROUPED>;
-  const int st = lds_attr_once(done, (const void*)fn, 160 * 1024 - 1024, who);
-  if (st != TIERMM_OK) return st;
-  const long long ntn = (a.N + 16 * NF - 1) / (16 * NF);
-  const long long ntm = GROUPED ? a.M / (16 * MT) + std::min(a.E, a.M) + 1 : 1;
-  const long long grid = GROUPED ? (ntm * ntn + 7) / 8 * 8 : ntn;
-  if (grid > (1ll << 22)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, ntm * ntn);
-  fn<<<(unsigned)grid, 64 * NW, LDS, s>>>(a);
-  TM_LAUNCH_CHECK(who);
-  return TIERMM_OK;
+  return launch(i8_tile_kernel<YT, BM, BN, WVN, WVK, KS, S, GROUPED>, done, a, GROUPED, BM, BN, 64 * WVN * WVK, LDS, s,
+                who);
 }
 
-// Up to kRows rows the few-row kernel, above it 256 x 320 tiles.
-constexpr int kRows = 64, kFused = 4, kFusedLds = 64 * 1024;
+// The tiles, and what one costs: a call takes about t0 + K / 1024 * max(one, each * n) us, n the
+// tiles that the fullest CU runs.  `one` is a tile alone on its CU (its loads' latency),
+// `each` what another adds (the CU's share of the stream, or its MFMAs).  Fitted to measured
+// times of 104 sizes (8 to 4096 rows, 500 to 28672 columns, K of 1000 to 14336) on weights that
+// the last-level cache holds; the tile with the least such time is within 2 % of the best one
+// in the mean, 25 % at worst.  Example, 5120 x 5120: 8 rows 16 x 16 tiles 6.7 us, 64 x 64
+// 12.0, 128 x 128 17.9; 512 rows 110, 28.2 and 19.8; 4096 rows 256 x 320 90, 128 x 128 120.
+struct TileCost {
+  int bm, bn;
+  float t0, one, each;
+};
+constexpr TileCost kTiles[] = {
+    {16, 16, 3.4f, 0.39f, 0.50f},   {16, 64, 3.1f, 1.54f, 1.33f},    {32, 32, 3.0f, 0.24f, 1.16f},
+    {64, 32, 3.0f, 0.44f, 1.66f},   {64, 64, 3.2f, 1.86f, 1.75f},    {128, 64, 2.8f, 2.55f, 2.80f},
+    {128, 128, 2.9f, 3.30f, 3.75f}, {256, 128, 3.5f, 5.83f, 6.75f},  {256, 192, 2.2f, 6.62f, 9.86f},
+    {256, 256, 4.6f, 0.18f, 11.6f}, {256, 320, 4.3f, 11.1f, 14.1f},
+};
+
+// Tiles of bm rows that hold the rows of Y; grouped, of experts as independent choices fill
+// them (the offsets are on the device): those with rows, each with half a tile to spare.
+double row_tiles(const I8Args& a, bool grouped, int bm) {
+  if (!grouped) return (a.M + bm - 1) / bm;
+  const double used = a.E * (1.0 - std::exp(-(double)a.M / a.E));
+  return used * std::max(1.0, a.M / used / bm + 0.5);
+}
+
+int pick_tile(const I8Args& a, bool grouped, int cus) {
+  int best = 0;
+  double least = 1e30;
+  for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
+    const TileCost& c = kTiles[i];
+    const double n = std::ceil(row_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) / cus);
+    const double t = c.t0 + a.nk * kStep / 1024.0 * std::max((double)c.one, c.each * n);
+    if (t < least) least = t, best = i;
+  }
+  return best;
+}
+
+template <int YT, bool GROUPED>
+int launch_picked(int tile, const I8Args& a, hipStream_t s, const char* who) {
+  switch (tile) {
+    case 0: return launch_tile<YT, 16, 16, 1, 8, 4, 4, GROUPED>(a, s, who);
+    case 1: return launch_tile<YT, 16, 64, 2, 2, 2, 4, GROUPED>(a, s, who);
+    case 2: return launch_tile<YT, 32, 32, 2, 8, 4, 4, GROUPED>(a, s, who);
+    case 3: return launch_tile<YT, 64, 32, 2, 4, 2, 4, GROUPED>(a, s, who);
+    case 4: return launch_gemm<YT, 64, 64, 2, 2, 4, GROUPED>(a, s, who);
+    case 5: return launch_gemm<YT, 128, 64, 4, 2, 4, GROUPED>(a, s, who);
+    case 6: return launch_gemm<YT, 128, 128, 2, 4, 4, GROUPED>(a, s, who);
+    case 7: return launch_gemm<YT, 256, 128, 4, 2, 3, GROUPED>(a, s, who);
+    case 8: return launch_gemm<YT, 256, 192, 4, 2, 2, GROUPED>(a, s, who);
+    case 9: return launch_gemm<YT, 256, 256, 4, 2, 2, GROUPED>(a, s, who);
+    default: return launch_gemm<YT, 256, 320, 4, 2, 2, GROUPED>(a, s, who);
+  }
+}
 
 int gemm(const I8Args& a, int ytype, bool grouped, hipStream_t s, const char* who) {
-  int st = TIERMM_OK;
+  int cus = 0, st = device_cus(&cus);
+  if (st != TIERMM_OK) return st;
+  const int tile = pick_tile(a, grouped, cus);
   with_rows(ytype, [&](auto yt) {
     constexpr int YT = decltype(yt)::value;
-    if (grouped) {
-      const int avg = a.M / a.E;
-      if (avg <= 8) st = launch_rows<YT, -1, 1, 2, 4, true>(a, s, who);
-      else if (avg <= 32) st = launch_rows<YT, -1, 2, 2, 4, true>(a, s, who);
-      else st = launch_gemm<YT, 128, 128, 2, 2, true>(a, s, who);
-    } else if (a.M <= kRows) {
-      if (a.M <= 16) st = launch_rows<YT, -1, 1, 2, 8, false>(a, s, who);
-      else if (a.M <= 32) st = launch_rows<YT, -1, 2, 2, 8, false>(a, s, who);
-      else if (a.M <= 48) st = launch_rows<YT, -1, 3, 2, 8, false>(a, s, who);
-      else st = launch_rows<YT, -1, 4, 2, 8, false>(a, s, who);
-    } else {
-      st = launch_gemm<YT, 256, 320, 4, 2, false>(a, s, who);
-    }
+    st = grouped ? launch_picked<YT, true>(tile, a, s, who) : launch_picked<YT, false>(tile, a, s, who);
   });
   return st;
 }
 
-// x of a few rows is quantized by the product's own workgroups.
-bool fuses(int M, int K) { return M <= kFused && M * padded(K) <= kFusedLds; }
+// One or two rows of x are quantized by the product's own workgroups (the GEMV): a launch less,
+// and each byte of W in whole lines.
+constexpr int kGemvLds = 60 * 1024;
+bool fuses(int M, int K) { return M <= 2 && M * (padded(K) + 1024) <= kGemvLds; }
+
 int fused(const I8Args& a, int xtype, int ytype, hipStream_t s, const char* who) {
   int st = TIERMM_OK;
   with_rows(ytype, [&](auto yt) {
     with_rows(xtype, [&](auto xt) {
-      st = launch_rows<decltype(yt)::value, decltype(xt)::value, 1, 2, 8, false>(a, s, who);
+      constexpr int YT = decltype(yt)::value, XT = decltype(xt)::value;
+      auto rows = [&](auto mx) {
+        constexpr int MX = decltype(mx)::value;
+        if (a.N < 5120) st = launch_gemv<YT, XT, MX, 1, 8>(a, s, who);
+        else st = launch_gemv<YT, XT, MX, 2, 16>(a, s, who);
+      };
+      if (a.M == 1) rows(std::integral_constant<int, 1>());
+      else rows(std::integral_constant<int, 2>());
     });
   });
   return st;
