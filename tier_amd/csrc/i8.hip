@@ -49,14 +49,13 @@ __device__ __forceinline__ RowScale row_scale_of(uint32_t top) {
 
 // Codes of 4 elements, packed: rint(x * inv), nearest even.
 __device__ __forceinline__ uint32_t codes4(const float* v, const RowScale& r) {
-  uint32_t w = 0;
+  // a scale of 0 or NaN has inv = 0: codes 0, whatever the element
+  uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // a scale of 0 or NaN has inv = 0: codes 0, whatever the element
-    const float f = r.inv == 0.f ? 0.f : __builtin_rintf((v[i] * r.pre) * r.inv);
-    w |= ((uint32_t)(int)f & 0xffu) << (8 * i);
-  }
-  return w;
+  for (int i = 0; i < 4; ++i) c[i] = (uint32_t)(int)(r.inv == 0.f ? 0.f : __builtin_rintf((v[i] * r.pre) * r.inv));
+  // byte 0 of each
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+  return lo | hi;
 }
 
 template <int N>
@@ -66,31 +65,54 @@ __device__ __forceinline__ uint32_t top_bits(const float (&v)[N], uint32_t top) 
   return top;
 }
 
-// One row a workgroup, read twice.
-template <int XT>
-__global__ __launch_bounds__(256) void i8_quant_kernel(const uint8_t* __restrict__ x, size_t ldx,
-                                                       int8_t* __restrict__ q, size_t rb, float* __restrict__ scale,
-                                                       int K, int Kp) {
-  using R = Rows<XT>;
-  __shared__ uint32_t red[4];
+// One row a workgroup of NT threads.  R > 0: the row has at most R * NT units of 16 bytes and
+// stays in registers, all its loads on their way at once; R = 0: any row, read twice.
+template <int XT, int NT, int R>
+__global__ __launch_bounds__(NT) void i8_quant_kernel(const uint8_t* __restrict__ x, size_t ldx,
+                                                      int8_t* __restrict__ q, size_t rb, float* __restrict__ scale,
+                                                      int K, int Kp) {
+  using X = Rows<XT>;
+  __shared__ uint32_t red[NT / 64];
   const uint8_t* row = x + (size_t)blockIdx.x * ldx;
+  const int k0 = threadIdx.x * X::EPU, step = NT * X::EPU;
+  u32x4 u[R > 0 ? R : 1];
   uint32_t top = 0;
-  for (int c = threadIdx.x * R::EPU; c < K; c += 256 * R::EPU) {
-    float v[R::EPU];
-    R::widen(R::get(row, c, K), v);
-    top = top_bits(v, top);
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) u[i] = k0 + i * step < K ? X::get(row, k0 + i * step, K) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float v[X::EPU];
+      X::widen(u[i], v);
+      top = top_bits(v, top);
+    }
+  } else {
+    for (int k = k0; k < K; k += step) {
+      float v[X::EPU];
+      X::widen(X::get(row, k, K), v);
+      top = top_bits(v, top);
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
-  const RowScale r = row_scale_of(max(max(red[0], red[1]), max(red[2], red[3])));
-  int8_t* out = q + (size_t)blockIdx.x * rb;
-  for (int c = threadIdx.x * R::EPU; c < Kp; c += 256 * R::EPU) {
-    float v[R::EPU] = {};
-    if (c < K) R::widen(R::get(row, c, K), v);
 #pragma unroll
-    for (int i = 0; i < R::EPU; i += 4) *(uint32_t*)(out + c + i) = codes4(v + i, r);
+  for (int w = 0; w < NT / 64; ++w) top = max(top, red[w]);
+  const RowScale r = row_scale_of(top);
+  int8_t* out = q + (size_t)blockIdx.x * rb;
+  auto put = [&](int k, const u32x4& c) __attribute__((always_inline)) {
+    float v[X::EPU];
+    X::widen(c, v);
+    if constexpr (X::EPU == 8) *(u32x2*)(out + k) = u32x2{codes4(v, r), codes4(v + 4, r)};
+    else *(uint32_t*)(out + k) = codes4(v, r);
+  };
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (k0 + i * step < Kp) put(k0 + i * step, u[i]);
+  } else {
+    for (int k = k0; k < Kp; k += step) put(k, k < K ? X::get(row, k, K) : u32x4{0u, 0u, 0u, 0u});
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = r.sc;
 }
@@ -109,6 +131,7 @@ struct I8Args {
   const int32_t* off;
   const int32_t* rows;  // row p of Y reads row rows[p] / topk of X (null: row p)
   int E, topk, xrows;
+  int share;  // tiles that an XCD takes at a time
 };
 
 // What a workgroup computes: rows [m0, m1) of Y, column tile tn.
@@ -125,30 +148,19 @@ __device__ __forceinline__ int xcd_share(int bid, int total) {
   return i < each + (x < more) ? x * each + min(x, more) + i : -1;
 }
 
+// Tile `bid` over the experts' rows, expert by expert, and in each column by column; false past
+// the last.  XCD x (bid % 8) takes `share` tiles at a time: their rows of W and X meet in its L2.
+// Each wave finds it from the offsets, 64 experts a step.
 template <int BM>
 __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, Tile& tl) {
-  const int lane = threadIdx.x & 63, P = a.M;
-  auto begin = [&](int e) { return min(max(a.off[e], 0), P); };
-  // rows of group e0 + lane (group E: from off[E] to P)
-  auto rows_of = [&](int e, int& b) {
-    b = e <= a.E ? begin(e) : P;
-    const int n = e < a.E ? begin(e + 1) - b : e == a.E ? P - b : 0;
-    return max(n, 0);
-  };
-  int total = 0;
-  for (int e0 = 0; e0 <= a.E; e0 += 64) {
-    int b;
-    int n = (rows_of(e0 + lane, b) + BM - 1) / BM;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    total += n;
-  }
-  const int t = xcd_share(bid, total * ntn);
-  if (t < 0) return false;
+  const int lane = threadIdx.x & 63, P = a.M, i = bid >> 3;
+  const int t = ((i / a.share) * 8 + (bid & 7)) * a.share + i % a.share;
   int run = 0;
   for (int e0 = 0; e0 <= a.E; e0 += 64) {
-    int b;
-    const int rows = rows_of(e0 + lane, b), n = (rows + BM - 1) / BM * ntn;
+    // rows of expert e (E: those from off[E] to P), whatever the offsets hold within [0, P]
+    const int e = e0 + lane, b = e <= a.E ? min(max(a.off[e], 0), P) : P;
+    const int end = e < a.E ? min(max(a.off[e + 1], 0), P) : P;
+    const int rows = max(end - b, 0), n = (rows + BM - 1) / BM * ntn;
     int s = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -312,9 +324,17 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     if (v >= 1 && v <= WM) xf[f][v - 1] = *(const i32x4*)(s + xrow + (v - 1) * 32 * kStep);
     else wf[f][v == 0 ? 0 : v - WM] = *(const i32x4*)(s + wrow + (v == 0 ? 0 : v - WM) * 32 * kStep);
   };
+  // Grouped: a wave whose rows all lie past the expert's last one only brings its loads.
+  const bool live = !GROUPED || tl.m0 + wm * WM * 32 < tl.m1;
   // The products of fragments f, with the fragments (kt, kk) into the other set and loads
   // u0 .. u0 + n - 1 of stage `dt` between them.
   auto step = [&](int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
+    if (!live) {
+#pragma unroll
+      for (int d = 0; d < n; ++d)
+        if (dt < a.nk) issue(dt, u0 + d);
+      return;
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
@@ -397,13 +417,14 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
 
 // Launches fn over the tiles; grouped, every expert may end in a partly filled one.
 template <class Fn>
-int launch(Fn* fn, std::atomic<uint64_t>& done, const I8Args& a, bool grouped, int bm, int bn, int threads, int lds,
+int launch(Fn* fn, std::atomic<uint64_t>& done, I8Args a, bool grouped, int bm, int bn, int threads, int lds,
            hipStream_t s, const char* who) {
   const int st = lds_attr_once(done, (const void*)fn, lds, who);
   if (st != TIERMM_OK) return st;
   const long long ntn = (a.N + bn - 1) / bn;
   const long long ntm = grouped ? a.M / bm + std::min(a.E, a.M) + 1 : (a.M + bm - 1) / bm;
-  const long long grid = (ntm * ntn + 7) / 8 * 8;
+  a.share = (int)std::min(32ll, (ntm * ntn + 7) / 8);
+  const long long step = grouped ? 8ll * a.share : 8, grid = (ntm * ntn + step - 1) / step * step;
   if (grid > (1ll << 22)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, ntm * ntn);
   fn<<<(unsigned)grid, threads, lds, s>>>(a);
   TM_LAUNCH_CHECK(who);
@@ -740,12 +761,33 @@ int fused(const I8Args& a, int xtype, int ytype, hipStream_t s, const char* who)
   return st;
 }
 
+// Rows up to which a row gets 1024 threads: few rows wait for their latency.  4096 rows of
+// 5120 bf16: 11.5 us (5.5 TB/s) with 256 threads a row, 16.3 with 1024; of 14336 fp32, whose
+// registers 256 threads do not hold: 20.8 (2000 rows, 6.9 TB/s) against 27.7 read twice.
+constexpr int kQuantWide = 512;
+
 int quant(const void* x, int xtype, size_t ldx, int8_t* q, size_t rb, float* scale, int M, int K, hipStream_t s,
           const char* who) {
-  const size_t es = row_elem_bytes(xtype);
+  const size_t ld = ldx * row_elem_bytes(xtype);
+  const uint8_t* p = (const uint8_t*)x;
+  const int Kp = padded(K);
   with_rows(xtype, [&](auto xt) {
-    i8_quant_kernel<decltype(xt)::value>
-        <<<M, 256, 0, s>>>((const uint8_t*)x, ldx * es, q, rb, scale, K, padded(K));
+    constexpr int XT = decltype(xt)::value;
+    const int units = Kp / Rows<XT>::EPU;
+#define QUANT(NT, R) i8_quant_kernel<XT, NT, R><<<M, NT, 0, s>>>(p, ld, q, rb, scale, K, Kp)
+    if (M <= kQuantWide) {
+      if (units <= 1024) QUANT(1024, 1);
+      else if (units <= 2048) QUANT(1024, 2);
+      else if (units <= 4096) QUANT(1024, 4);
+      else QUANT(1024, 0);
+    } else {
+      if (units <= 512) QUANT(256, 2);
+      else if (units <= 1024) QUANT(256, 4);
+      else if (units <= 2048) QUANT(256, 8);
+      else if (units <= 4096) QUANT(1024, 4);
+      else QUANT(1024, 0);
+    }
+#undef QUANT
   });
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
@@ -811,7 +853,7 @@ int tiermm_i8_gemm(const int8_t* Xq, size_t rbx, const float* sx, const int8_t* 
   if (!sx || !sw || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4))
     return set_error(TIERMM_EINVAL, "%s: null or misaligned scales", who);
   const I8Args a = {(const uint8_t*)Xq, sx, (const uint8_t*)W, sw, bias, (uint8_t*)Y, rbx, rbw,
-                    ldy * row_elem_bytes(ytype), M, N, K, padded(K) / kStep, nullptr, nullptr, 0, 1, M};
+                    ldy * row_elem_bytes(ytype), M, N, K, padded(K) / kStep, nullptr, nullptr, 0, 1, M, 1};
   return gemm(a, ytype, false, (hipStream_t)stream, who);
 }
 
@@ -836,7 +878,7 @@ int tiermm_i8_linear(const void* x, int xtype, size_t ldx, const int8_t* W, size
   if (!sw || misaligned(sw, 4) || misaligned(bias, 4))
     return set_error(TIERMM_EINVAL, "%s: null or misaligned scales", who);
   I8Args a = {(const uint8_t*)x, nullptr, (const uint8_t*)W, sw, bias, (uint8_t*)Y, ldx * es, rbw,
-              ldy * row_elem_bytes(ytype), M, N, K, padded(K) / kStep, nullptr, nullptr, 0, 1, M};
+              ldy * row_elem_bytes(ytype), M, N, K, padded(K) / kStep, nullptr, nullptr, 0, 1, M, 1};
   if (fuses(M, K)) return fused(a, xtype, ytype, (hipStream_t)stream, who);
   void* w = nullptr;
   if (misaligned(ws, 16)) return set_error(TIERMM_EINVAL, "%s: workspace not 16-byte aligned", who);
@@ -868,7 +910,7 @@ int tiermm_i8_gemm_grouped(const int8_t* Xq, size_t rbx, const float* sx, const 
       misaligned(rows, 4))
     return set_error(TIERMM_EINVAL, "%s: null or misaligned table", who);
   const I8Args a = {(const uint8_t*)Xq, sx, (const uint8_t*)W, sw, nullptr, (uint8_t*)Y, rbx, rbw,
-                    ldy * row_elem_bytes(ytype), P, N, K, padded(K) / kStep, expert_offsets, rows, n_experts, topk, n_rows};
+                    ldy * row_elem_bytes(ytype), P, N, K, padded(K) / kStep, expert_offsets, rows, n_experts, topk, n_rows, 1};
   return gemm(a, ytype, true, (hipStream_t)stream, who);
 }
 
