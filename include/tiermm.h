@@ -343,7 +343,7 @@ int tiermm_moe_combine(const float* Y_sorted, const int* token_pairs, const floa
  *   sorted_pairs[T * topk]         pair at each place, -1 from expert_offsets[n_experts] up
  * (the tables that tiermm_qgemm_grouped, from a host copy of the offsets, and
  * tiermm_moe_combine take).  All are device int32 arrays.  Workspace only where the size query
- * says so (more than 65536 pairs). */
+ * says so (more than 32768 pairs). */
 int tiermm_moe_plan(const int32_t* expert_ids, int T, int topk, int n_experts, int32_t* expert_offsets,
                     int32_t* token_pairs, int32_t* sorted_pairs, void* ws, size_t ws_bytes, tiermm_stream_t stream);
 size_t tiermm_moe_plan_ws_bytes(int T, int topk, int n_experts);

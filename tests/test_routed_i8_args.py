@@ -27,8 +27,8 @@ def test_plan_refuses(kw, code):
 
 
 def test_plan_workspace():
-    assert tier_amd.moe_plan_ws_bytes(8192, 8, 64) == 0
-    assert tier_amd.moe_plan_ws_bytes(8193, 8, 64) > 0
+    assert tier_amd.moe_plan_ws_bytes(4096, 8, 64) == 0
+    assert tier_amd.moe_plan_ws_bytes(4097, 8, 64) > 0
     assert tier_amd.moe_plan_ws_bytes(-1, 8, 64) == 0
 
 

@@ -4,8 +4,12 @@
 // models, arch.py:158-159).
 //
 // All are bound by memory: a row is read or written once, in 16-byte units, with the
-// few indices of a token in scalar registers.  No atomics: every sum has one owner and
-// one order, so results do not change between runs.
+// few indices of a token in scalar registers.  No atomics on results: every sum has one
+// owner and one order, so results do not change between runs.  Measured on 4096 tokens,
+// top 8 of 64, rows of 2048 (a large copy moves 5.1 TB/s): sort 51-54 us fp32 (5.6-5.9
+// TB/s), 24 us bf16; its gradient 46 and 23.5 (6.4-6.6); the weighted sum 47 and 23.6; its
+// gradient 115 and 60 (4.9-5.0, the same bytes read as written).  Rows of 2047 bf16, which start at
+// any 2 bytes: 26, 26 and 68 us.
 #include "tm_rows.h"
 
 namespace tiermm {
@@ -18,12 +22,14 @@ namespace {
 // One workgroup per expert (and one for the dropped pairs, as expert E) reads all ids:
 // it counts those below and the earlier ones of its own, and writes its own places.
 // That is E + 1 reads of P ids through L2, but one launch and no exchange between
-// workgroups.  A tile is 4 ids a thread; NT tiles stay in registers.
-constexpr int kPlanThreads = 1024, kPlanTile = 4 * kPlanThreads;
+// workgroups: 32768 pairs, 64 experts 7.6 us, where the two launches below take 8.3.  A tile
+// is 4 ids a thread; NT tiles stay in registers (16 of them spilled: the limit of 8).
+constexpr int kPlanThreads = 1024, kPlanTile = 4 * kPlanThreads, kPlanMost = 8 * kPlanTile;
+typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int NT>
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int P, int E,
-                                                                int vec, int32_t* __restrict__ offsets,
+                                                                int32_t* __restrict__ offsets,
                                                                 int32_t* __restrict__ places,
                                                                 int32_t* __restrict__ sorted) {
   constexpr int NW = kPlanThreads / 64;
@@ -31,30 +37,30 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint64_t below = (1ull << lane) - 1;
   int first[NT];      // pairs of this expert before this thread's, within its wave and tile
-  uint32_t mine = 0;  // bit 4t + i: id i of tile t's four is of this expert (NT <= 8 a word)
-  uint32_t mine2 = 0;
+  uint32_t mine = 0;  // bit 4t + i: id i of tile t's four is of this expert
   int lt = 0;
+  i32x4_a4 id[NT];  // every load on its way before the first is used
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int i0 = t * kPlanTile + 4 * tid;
-    int4 v = {-1, -1, -1, -1};
-    if (i0 + 3 < P && vec) v = *(const int4*)(ids + i0);
-    else {
-      if (i0 < P) v.x = ids[i0];
-      if (i0 + 1 < P) v.y = ids[i0 + 1];
-      if (i0 + 2 < P) v.z = ids[i0 + 2];
-      if (i0 + 3 < P) v.w = ids[i0 + 3];
+    if ((t + 1) * kPlanTile <= P) {
+      id[t] = *(const i32x4_a4*)(ids + i0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) id[t][i] = i0 + i < P ? ids[i0 + i] : -1;
     }
-    const int id[4] = {v.x, v.y, v.z, v.w};
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int i0 = t * kPlanTile + 4 * tid;
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int key = (uint32_t)id[i] < (uint32_t)E ? id[i] : E;
+      const int v = id[t][i], key = (uint32_t)v < (uint32_t)E ? v : E;
       lt += key < e;
       m |= (uint32_t)(key == e && i0 + i < P) << i;
     }
-    if (t < 8) mine |= m << (4 * (t & 7));
-    else mine2 |= m << (4 * (t & 7));
+    mine |= m << (4 * t);
     // prefix over the wave of counts 0..4, from the ballots of their three bits
     const int c = __popc(m);
     const uint64_t b0 = __ballot(c & 1), b1 = __ballot(c & 2), b2 = __ballot(c & 4);
@@ -86,7 +92,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const uint32_t m = (t < 8 ? mine : mine2) >> (4 * (t & 7));
+    const uint32_t m = mine >> (4 * t);
     int at = own[t * NW + wave] + first[t];
     const int i0 = t * kPlanTile + 4 * tid;
 #pragma unroll
@@ -99,17 +105,19 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   }
 }
 
-// Longer batches: a histogram of each chunk of kChunk pairs, then one workgroup per
-// chunk that adds the histograms before its own and places its pairs.
-constexpr int kChunk = 4096, kChunkWaves = 4, kPerWave = kChunk / kChunkWaves;
+// Longer batches: a histogram of each chunk of pairs, then one workgroup per chunk that adds
+// the histograms before its own and places its pairs (524288 pairs, 256 experts: 26 us).
+// Each workgroup reads every chunk's histogram, so long batches take longer chunks.
+constexpr int kChunkWaves = 4;
+constexpr int plan_chunk(long long P) { return P <= 256 * 1024 ? 1024 : 4096; }
 
 __global__ __launch_bounds__(64 * kChunkWaves) void moe_hist_kernel(const int32_t* __restrict__ ids, int P, int E,
-                                                                    int32_t* __restrict__ hist) {
+                                                                    int chunk, int32_t* __restrict__ hist) {
   extern __shared__ int cnt[];
   for (int e = threadIdx.x; e <= E; e += 64 * kChunkWaves) cnt[e] = 0;
   __syncthreads();
-  const int end = min(P, (int)(blockIdx.x + 1) * kChunk);
-  for (int i = blockIdx.x * kChunk + threadIdx.x; i < end; i += 64 * kChunkWaves) {
+  const int end = min(P, (int)(blockIdx.x + 1) * chunk);
+  for (int i = blockIdx.x * chunk + threadIdx.x; i < end; i += 64 * kChunkWaves) {
     const int id = ids[i];
     atomicAdd(&cnt[(uint32_t)id < (uint32_t)E ? id : E], 1);  // whole numbers: any order
   }
@@ -119,16 +127,18 @@ __global__ __launch_bounds__(64 * kChunkWaves) void moe_hist_kernel(const int32_
 
 // LDS: next[kChunkWaves][E + 1], the place of each wave's next pair of each expert, and total[E + 1].
 __global__ __launch_bounds__(64 * kChunkWaves) void moe_place_kernel(const int32_t* __restrict__ ids, int P, int E,
+                                                                     int chunk, int nb,
                                                                      const int32_t* __restrict__ hist,
                                                                      int32_t* __restrict__ offsets,
                                                                      int32_t* __restrict__ places,
                                                                      int32_t* __restrict__ sorted) {
   extern __shared__ int lds[];
-  const int K = E + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nb = gridDim.x, b = blockIdx.x;
+  const int K = E + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   int* next = lds;
   int* total = lds + kChunkWaves * K;
   for (int e = tid; e < K; e += 64 * kChunkWaves) {
     int all = 0, before = 0;
+#pragma unroll 16
     for (int c = 0; c < nb; ++c) {
       const int n = hist[(size_t)c * K + e];
       all += n;
@@ -141,7 +151,7 @@ __global__ __launch_bounds__(64 * kChunkWaves) void moe_place_kernel(const int32
   }
   __syncthreads();
   // counts of waves 0 .. kChunkWaves-2 into the next wave's start
-  const int w0 = b * kChunk + wave * kPerWave, w1 = min(P, w0 + kPerWave);
+  const int per = chunk / kChunkWaves, w0 = b * chunk + wave * per, w1 = min(P, w0 + per);
   if (wave + 1 < kChunkWaves)
     for (int i = w0 + lane; i < w1; i += 64) {
       const int id = ids[i];
@@ -269,7 +279,9 @@ struct UnsortGradArgs {
 };
 
 // dYs[p] = w dout[t] and dw[t][j] = <dout[t], Ys[p]> of pair (t, j) at place p, by one
-// workgroup: dout comes from L2 for all but a token's first pair.
+// workgroup: dout comes from L2 for all but a token's first pair.  (A workgroup a token, dout
+// read once: 138 against 119 us in fp32 at 4096 tokens, 10.3 against 4.2 at 128.)  The rows
+// of dYs are stored past the caches: 118 -> 115 us, and 89 -> 68 on rows of 2047 bf16.
 template <int XT>
 __global__ __launch_bounds__(256) void moe_unsort_grad_kernel(const UnsortGradArgs a) {
   using R = Rows<XT>;
@@ -288,7 +300,7 @@ __global__ __launch_bounds__(256) void moe_unsort_grad_kernel(const UnsortGradAr
         s = fmaf(d[k], y[k], s);
         d[k] *= w;
       }
-      R::set(a.dys + (size_t)p * a.ldd, c, a.cols, R::narrow(d));
+      R::set_nt(a.dys + (size_t)p * a.ldd, c, a.cols, R::narrow(d));
     }
   if (a.sorted[i] < 0)
     for (int c = tid * R::EPU; c < a.cols; c += 256 * R::EPU)
@@ -321,8 +333,8 @@ extern "C" {
 size_t tiermm_moe_plan_ws_bytes(int T, int topk, int n_experts) {
   if (T < 0 || topk < 0 || n_experts < 1) return 0;
   const long long P = (long long)T * topk;
-  if (P <= 16 * kPlanTile) return 0;
-  return (size_t)((P + kChunk - 1) / kChunk) * (n_experts + 1) * sizeof(int32_t);
+  if (P <= kPlanMost) return 0;
+  return (size_t)((P + plan_chunk(P) - 1) / plan_chunk(P)) * (n_experts + 1) * sizeof(int32_t);
 }
 
 int tiermm_moe_plan(const int32_t* expert_ids, int T, int topk, int n_experts, int32_t* expert_offsets,
@@ -345,19 +357,19 @@ int tiermm_moe_plan(const int32_t* expert_ids, int T, int topk, int n_experts, i
     void* hist = nullptr;
     const int st = get_workspace(ws, ws_bytes, need, &hist, who);
     if (st != TIERMM_OK) return st;
-    const unsigned nb = (unsigned)((pairs + kChunk - 1) / kChunk);
-    moe_hist_kernel<<<nb, 64 * kChunkWaves, (E + 1) * sizeof(int), s>>>(expert_ids, P, E, (int32_t*)hist);
+    const int chunk = plan_chunk(P), nb = (P + chunk - 1) / chunk;
+    moe_hist_kernel<<<nb, 64 * kChunkWaves, (E + 1) * sizeof(int), s>>>(expert_ids, P, E, chunk, (int32_t*)hist);
     TM_LAUNCH_CHECK("tiermm_moe_plan: histogram");
     moe_place_kernel<<<nb, 64 * kChunkWaves, (kChunkWaves + 1) * (E + 1) * sizeof(int), s>>>(
-        expert_ids, P, E, (const int32_t*)hist, expert_offsets, token_pairs, sorted_pairs);
+        expert_ids, P, E, chunk, nb, (const int32_t*)hist, expert_offsets, token_pairs, sorted_pairs);
     TM_LAUNCH_CHECK("tiermm_moe_plan: places");
     return TIERMM_OK;
   }
-#define PLAN(NT) moe_plan_kernel<NT><<<E + 1, kPlanThreads, 0, s>>>(expert_ids, P, E, vec, expert_offsets, token_pairs, sorted_pairs)
-  const int vec = !misaligned(expert_ids, 16);
+#define PLAN(NT) moe_plan_kernel<NT><<<E + 1, kPlanThreads, 0, s>>>(expert_ids, P, E, expert_offsets, token_pairs, sorted_pairs)
   if (P <= kPlanTile) PLAN(1);
+  else if (P <= 2 * kPlanTile) PLAN(2);
   else if (P <= 4 * kPlanTile) PLAN(4);
-  else PLAN(16);
+  else PLAN(8);
 #undef PLAN
   TM_LAUNCH_CHECK("tiermm_moe_plan: launch");
   return TIERMM_OK;

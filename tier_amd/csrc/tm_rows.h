@@ -46,6 +46,12 @@ struct Rows {
   }
   static __device__ __forceinline__ u32x4 raw(const uint8_t* p) { return *(const u32x4_a2*)p; }
   static __device__ __forceinline__ void put(uint8_t* p, u32x4 u) { *(u32x4_a2*)p = u; }
+  // The same, not to be read again soon.
+  static __device__ __forceinline__ void set_nt(uint8_t* row, int c, int cols, u32x4 u) {
+    uint8_t* p = row + (size_t)c * ES;
+    if (c + EPU <= cols) __builtin_nontemporal_store(u, (u32x4_a2*)p);
+    else put_part(p, u, cols - c);
+  }
   // The first n elements at p as a unit (0 behind them), and the first n of a unit to p: bits as they are.
   static __device__ __forceinline__ u32x4 raw_part(const uint8_t* p, int n) {
     u32x4 u = {0u, 0u, 0u, 0u};
