@@ -877,11 +877,11 @@ int tiermm_i8_linear(const void* x, int xtype, size_t ldx, const int8_t* W, size
   if ((st = check_i8_rows(who, "weight", W, rbw, K)) != TIERMM_OK) return st;
   if (!sw || misaligned(sw, 4) || misaligned(bias, 4))
     return set_error(TIERMM_EINVAL, "%s: null or misaligned scales", who);
+  if (misaligned(ws, 16)) return set_error(TIERMM_EINVAL, "%s: workspace not 16-byte aligned", who);
   I8Args a = {(const uint8_t*)x, nullptr, (const uint8_t*)W, sw, bias, (uint8_t*)Y, ldx * es, rbw,
               ldy * row_elem_bytes(ytype), M, N, K, padded(K) / kStep, nullptr, nullptr, 0, 1, M, 1};
   if (fuses(M, K)) return fused(a, xtype, ytype, (hipStream_t)stream, who);
   void* w = nullptr;
-  if (misaligned(ws, 16)) return set_error(TIERMM_EINVAL, "%s: workspace not 16-byte aligned", who);
   if ((st = get_workspace(ws, ws_bytes, tiermm_i8_linear_ws_bytes(M, N, K), &w, who)) != TIERMM_OK) return st;
   int8_t* q = (int8_t*)w;
   float* sx = (float*)(q + (size_t)M * padded(K));
