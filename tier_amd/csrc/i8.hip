@@ -234,6 +234,17 @@ __device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias)
   return fmaf((float)sum, sx * sw, bias);
 }
 
+// Waits until no more than n (at most N) stages of INST loads are on their way.
+template <int N, int INST>
+__device__ __forceinline__ void wait_stages(int n) {
+  if constexpr (N > 0) {
+    if (n >= N) vm_wait<N * INST>();
+    else wait_stages<N - 1, INST>(n);
+  } else {
+    vm_wait<0>();
+  }
+}
+
 // LDS place of byte `o` of row r of CH 16-byte chunks: neighbouring rows' chunks are
 // spread over the 16 chunks that the banks span.
 template <int CH>
@@ -353,8 +364,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   auto landed = [&](int kt) __attribute__((always_inline)) {
     const int behind = a.nk - 1 - kt;
     if (behind >= S - 2) vm_wait<(S - 2) * INST>();
-    else if (S > 3 && behind == 1) vm_wait<INST>();
-    else vm_wait<0>();
+    else wait_stages<S - 3, INST>(behind);
   };
   landed(0);
   __syncthreads();
@@ -611,11 +621,7 @@ __global__ __launch_bounds__(64 * WVN * WVK) void i8_tile_kernel(const I8Args a)
   for (int st = 0; st < ns; ++st) {
     const int after = ns - 1 - st;  // stages on their way behind this one
     if (after >= S - 2) vm_wait<(S - 2) * INST>();
-    else if (S > 6 && after == 4) vm_wait<4 * INST>();
-    else if (S > 5 && after == 3) vm_wait<3 * INST>();
-    else if (S > 4 && after == 2) vm_wait<2 * INST>();
-    else if (S > 3 && after == 1) vm_wait<INST>();
-    else vm_wait<0>();
+    else wait_stages<S - 3, INST>(after);
     __syncthreads();  // stage st has landed for every wave, and the one before it is read
     if (st + S - 1 < ns) issue(st + S - 1);
     const uint8_t* s = lds + get * STAGE;
@@ -677,18 +683,19 @@ int launch_tile(const I8Args& a, hipStream_t s, const char* who) {
 // tiles that the fullest CU runs.  `one` is a tile alone on its CU (its loads' latency),
 // `each` what another adds (the CU's share of the stream, or its MFMAs).  Fitted to measured
 // times of 104 sizes (8 to 4096 rows, 500 to 28672 columns, K of 1000 to 14336) on weights that
-// the last-level cache holds; the tile with the least such time is within 2 % of the best one
-// in the mean, 25 % at worst.  Example, 5120 x 5120: 8 rows 16 x 16 tiles 6.7 us, 64 x 64
-// 12.0, 128 x 128 17.9; 512 rows 110, 28.2 and 19.8; 4096 rows 256 x 320 90, 128 x 128 120.
+// the last-level cache holds; the tile with the least such time is within 2 % of the best of
+// twenty in the mean, 19 % at worst.  Example, 5120 x 5120, us: 8 rows 16 x 32 tiles 6.1, 64 x 64
+// 11.4, 128 x 128 17.9; 64 rows 32 x 64 9.1, 64 x 64 11.8, 16 x 16 13.6; 512 rows 128 x 128 19.8,
+// 64 x 64 28.2, 256 x 256 55.9; 4096 rows 256 x 320 89.7, 128 x 128 120, 256 x 256 124.
 struct TileCost {
   int bm, bn;
   float t0, one, each;
 };
 constexpr TileCost kTiles[] = {
-    {16, 16, 3.4f, 0.39f, 0.50f},   {16, 64, 3.1f, 1.54f, 1.33f},    {32, 32, 3.0f, 0.24f, 1.16f},
-    {64, 32, 3.0f, 0.44f, 1.66f},   {64, 64, 3.2f, 1.86f, 1.75f},    {128, 64, 2.8f, 2.55f, 2.80f},
-    {128, 128, 2.9f, 3.30f, 3.75f}, {256, 128, 3.5f, 5.83f, 6.75f},  {256, 192, 2.2f, 6.62f, 9.86f},
-    {256, 256, 4.6f, 0.18f, 11.6f}, {256, 320, 4.3f, 11.1f, 14.1f},
+    {16, 16, 3.4f, 0.39f, 0.50f},  {16, 32, 3.2f, 0.77f, 0.92f},   {16, 64, 3.1f, 1.54f, 1.33f},
+    {32, 32, 3.3f, 0.74f, 0.93f},  {32, 64, 3.8f, 1.19f, 1.43f},   {64, 64, 3.2f, 1.86f, 1.75f},
+    {128, 64, 2.8f, 2.55f, 2.80f}, {128, 128, 2.9f, 3.30f, 3.75f}, {256, 128, 3.5f, 5.83f, 6.75f},
+    {256, 192, 2.2f, 6.62f, 9.86f}, {256, 256, 4.6f, 0.18f, 11.6f}, {256, 320, 4.3f, 11.1f, 14.1f},
 };
 
 // Tiles of bm rows that hold the rows of Y; grouped, of experts as independent choices fill
@@ -715,15 +722,16 @@ template <int YT, bool GROUPED>
 int launch_picked(int tile, const I8Args& a, hipStream_t s, const char* who) {
   switch (tile) {
     case 0: return launch_tile<YT, 16, 16, 1, 8, 4, 4, GROUPED>(a, s, who);
-    case 1: return launch_tile<YT, 16, 64, 2, 2, 2, 4, GROUPED>(a, s, who);
-    case 2: return launch_tile<YT, 32, 32, 2, 8, 4, 4, GROUPED>(a, s, who);
-    case 3: return launch_tile<YT, 64, 32, 2, 4, 2, 4, GROUPED>(a, s, who);
-    case 4: return launch_gemm<YT, 64, 64, 2, 2, 4, GROUPED>(a, s, who);
-    case 5: return launch_gemm<YT, 128, 64, 4, 2, 4, GROUPED>(a, s, who);
-    case 6: return launch_gemm<YT, 128, 128, 2, 4, 4, GROUPED>(a, s, who);
-    case 7: return launch_gemm<YT, 256, 128, 4, 2, 3, GROUPED>(a, s, who);
-    case 8: return launch_gemm<YT, 256, 192, 4, 2, 2, GROUPED>(a, s, who);
-    case 9: return launch_gemm<YT, 256, 256, 4, 2, 2, GROUPED>(a, s, who);
+    case 1: return launch_tile<YT, 16, 32, 1, 8, 4, 4, GROUPED>(a, s, who);
+    case 2: return launch_tile<YT, 16, 64, 2, 2, 2, 4, GROUPED>(a, s, who);
+    case 3: return launch_tile<YT, 32, 32, 1, 8, 4, 4, GROUPED>(a, s, who);
+    case 4: return launch_tile<YT, 32, 64, 1, 8, 4, 3, GROUPED>(a, s, who);
+    case 5: return launch_gemm<YT, 64, 64, 2, 2, 4, GROUPED>(a, s, who);
+    case 6: return launch_gemm<YT, 128, 64, 4, 2, 4, GROUPED>(a, s, who);
+    case 7: return launch_gemm<YT, 128, 128, 2, 4, 4, GROUPED>(a, s, who);
+    case 8: return launch_gemm<YT, 256, 128, 4, 2, 3, GROUPED>(a, s, who);
+    case 9: return launch_gemm<YT, 256, 192, 4, 2, 2, GROUPED>(a, s, who);
+    case 10: return launch_gemm<YT, 256, 256, 4, 2, 2, GROUPED>(a, s, who);
     default: return launch_gemm<YT, 256, 320, 4, 2, 2, GROUPED>(a, s, who);
   }
 }
