@@ -346,3 +346,63 @@ def test_in_a_graph(gpu, M):
         assert np.array_equal(Y.bits(), replayed)
     g.destroy()
     s.destroy()
+
+
+@pytest.mark.parametrize("M", [1, 2, 10, 140])
+def test_offsets_past_32_bits(gpu, M):
+    """Rows of W, x and Y 32 MiB apart: the last ones start past 4 GiB."""
+    t, N, K, far = tier_amd.F32, 140, 100, 1 << 25
+    rng = np.random.default_rng(M)
+    w, sw, _, _ = weight(N, K, 1)
+    W = hip.DeviceBuffer((N - 1) * far + 128)
+    for n in range(N):
+        W.upload(np.pad(w[n], (0, 28)).astype(np.int8), n * far)
+    x = _x(M, K, 8)
+    X, Y = hip.DeviceBuffer((M - 1) * far + 4 * K), hip.DeviceBuffer((M - 1) * far + 4 * N)
+    for m in range(M):
+        X.upload(x[m], m * far)
+    tier_amd.i8_linear(X.ptr, t, far // 4, W.ptr, far, f32(sw).ptr, None, Y.ptr, t, far // 4, M, N, K)
+    hip.synchronize()
+    q, sx = quantize(x)
+    check(np.stack([Y.download(np.float32, N, m * far) for m in range(M)]).astype(np.float64), t, q, sx, w, sw)
+
+
+def test_experts_past_32_bits(gpu):
+    """Experts' weights 2.3 GB apart, gathered by rows in any order (one of them pointing nowhere)."""
+    t, E, N, K, far = tier_amd.BF16, 3, 70, 128, 1 << 25
+    w, sw, _, _ = weight(E * N, K, 2)
+    W = hip.DeviceBuffer((E * N - 1) * far + 128)
+    for n in range(E * N):
+        W.upload(w[n].astype(np.int8), n * far)
+    q = np.random.default_rng(3).integers(-127, 128, (6, K))
+    X, rb = i8_rows(q)
+    sx, rows = np.ones(6, np.float32), np.array([5, 0, 3, 99, 1, 2, 4, 0, 5], np.int32)
+    off, Y = np.array([0, 2, 4, 9], np.int32), Rows(t, 9, N)
+    tier_amd.i8_gemm_grouped(X.ptr, rb, f32(sx).ptr, i32(rows).ptr, 6, 1, i32(off).ptr, E, W.ptr, far, f32(sw).ptr, Y.ptr, t,
+                             N, 9, N, K)
+    hip.synchronize()
+    y = Y.values()
+    assert not y[3].any()
+    for e in range(E):
+        for p in range(off[e], off[e + 1]):
+            if p != 3:
+                check(y[p:p + 1], t, q[rows[p]][None], sx[:1], w[e * N:(e + 1) * N], sw[e * N:(e + 1) * N])
+
+
+def test_every_tile(gpu):
+    """Sizes at which each tile of the cost table is the least dear, with ragged rows and columns."""
+    t = tier_amd.BF16
+    for M, N, K in ((6, 1003, 640), (6, 1003, 260), (6, 10001, 260), (50, 2501, 260), (50, 5101, 2600), (50, 5101, 640),
+                    (50, 5101, 260), (30, 20001, 260), (130, 20001, 1300), (401, 20001, 260), (401, 28001, 640),
+                    (2051, 8001, 260)):
+        rng = np.random.default_rng(M)
+        q = rng.integers(-127, 128, (M, K))
+        sx = (0.5 + rng.random(M)).astype(np.float32)
+        w, sw, W, rbw = weight(N, K, N, pad_fill=-3)
+        X, rbx = i8_rows(q)
+        Y = Rows(t, M, N, None, pad=1)
+        tier_amd.i8_gemm(X.ptr, rbx, f32(sx).ptr, W.ptr, rbw, f32(sw).ptr, None, Y.ptr, t, Y.ld, M, N, K)
+        hip.synchronize()
+        rows = np.unique(np.concatenate([rng.choice(M, min(M, 60), replace=False), [0, M - 1]]))
+        check(Y.values()[rows], t, q[rows], sx[rows], w, sw)
+        assert Y.outside_kept(), (M, N, K)

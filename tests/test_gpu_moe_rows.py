@@ -252,3 +252,47 @@ def test_on_a_stream_and_in_a_graph(gpu):
         assert np.array_equal(O.bits(), replayed)
     g.destroy()
     s.destroy()
+
+
+def test_rows_past_the_caches(gpu):
+    """Gathered rows of more bytes than the caches keep (80 MiB) take the streaming form of the sums."""
+    t, T, k, N = tier_amd.F32, 2500, 8, 1050
+    rng = np.random.default_rng(1)
+    _, places, srt, TP, SP = _case(T, k, E=16)
+    y = rng.standard_normal((T * k, N)).astype(np.float32)
+    w = rng.random((T, k)).astype(np.float32)
+    Y, O, G, W = Rows(t, T * k, N, y, pad=2), Rows(t, T, N), Rows(t, T, N), f32(w)
+    tier_amd.moe_unsort(Y.ptr, t, Y.ld, TP.ptr, W.ptr, O.ptr, N, T, k, N)
+    tier_amd.moe_sort_grad(Y.ptr, t, Y.ld, TP.ptr, G.ptr, N, T, k, N)
+    hip.synchronize()
+    live = places >= 0
+    rows = np.where(live[..., None], y[np.maximum(places, 0)], np.float32(0)).astype(np.float64)
+    for got, terms in ((O, rows * np.where(live, w, 0).astype(np.float64)[..., None]), (G, rows)):
+        want, mag = terms.sum(1), np.abs(terms).sum(1)
+        assert np.all(np.abs(got.values() - want) <= (k + 2) * U * mag)
+
+
+def test_row_offsets_past_32_bits(gpu):
+    """Rows 32 MiB apart: the last ones start past 4 GiB."""
+    t, T, k, N, ld = tier_amd.F16, 2, 70, 24, 1 << 24
+    P, rng = T * k, np.random.default_rng(2)
+    _, places, srt, TP, SP = _case(T, k, how="drop", E=5)
+    x, w, d = (rng.standard_normal(s).astype(np.float32) for s in ((T, N), (T, k), (T, N)))
+    X, D, O, W, DW = Rows(t, T, N, x), Rows(t, T, N, d), Rows(t, T, N), f32(w), f32(np.zeros(P))
+    far, far2 = hip.DeviceBuffer((P - 1) * ld * 2 + 64), hip.DeviceBuffer((P - 1) * ld * 2 + 64)
+    rows = lambda b: np.stack([b.download(np.float16, N, p * ld * 2) for p in range(P)]).astype(np.float64)  # noqa: E731
+    tier_amd.moe_sort(X.ptr, t, N, TP.ptr, SP.ptr, far.ptr, ld, T, k, N)
+    tier_amd.moe_unsort(far.ptr, t, ld, TP.ptr, W.ptr, O.ptr, N, T, k, N)
+    tier_amd.moe_unsort_grad(D.ptr, t, N, far.ptr, ld, TP.ptr, SP.ptr, W.ptr, far2.ptr, ld, DW.ptr, T, k, N)
+    hip.synchronize()
+    xs, i = X.values(), np.maximum(srt, 0)
+    assert np.array_equal(rows(far), np.where(srt[:, None] >= 0, xs[i // k], 0))
+    live = places >= 0
+    terms = np.where(live, w, 0).astype(np.float64)[..., None] * xs[:, None]
+    err = (k + 1) * U * np.abs(terms).sum(1)
+    assert np.all(np.abs(O.values() - terms.sum(1)) <= err + UNIT[t] * (np.abs(terms.sum(1)) + err) + TINY[t])
+    want = np.where(srt[:, None] >= 0, w.ravel()[i].astype(np.float64)[:, None] * D.values()[i // k], 0)
+    assert np.all(np.abs(rows(far2) - want) <= (U + UNIT[t] * (1 + U)) * np.abs(want) + TINY[t])
+    dots = D.values() * xs
+    dw = DW.download(np.float32).reshape(T, k)
+    assert np.all(np.abs(dw - np.where(live, dots.sum(1)[:, None], 0)) <= 17 * U * np.abs(dots).sum(1)[:, None])

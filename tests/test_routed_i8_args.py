@@ -104,6 +104,7 @@ def test_quant_refuses(kw, code):
 @pytest.mark.parametrize("kw,code", [
     ({"M": -1}, EINVAL), ({"N": -1}, EINVAL), ({"K": -3}, EINVAL), ({"K": 140000}, UNSUPPORTED), ({"t": Q8}, UNSUPPORTED),
     ({"ldy": 19}, EINVAL), ({"y": None}, EINVAL), ({"y": A + 1, "t": F16}, EINVAL), ({"rbw": 256}, EINVAL),
+    ({"N": (1 << 26) + 1, "ldy": 1 << 27}, UNSUPPORTED), ({"M": (1 << 23) + 1}, UNSUPPORTED),
     ({"rbw": 390}, EINVAL), ({"w": A + 4}, EINVAL), ({"w": None}, EINVAL), ({"sw": None}, EINVAL),
     ({"sw": A + 1}, EINVAL), ({"x": None}, EINVAL)])
 def test_products_refuse(call, kw, code):

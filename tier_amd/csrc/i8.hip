@@ -698,21 +698,17 @@ constexpr TileCost kTiles[] = {
     {256, 192, 2.2f, 6.62f, 9.86f}, {256, 256, 4.6f, 0.18f, 11.6f}, {256, 320, 4.3f, 11.1f, 14.1f},
 };
 
-// Tiles of bm rows that hold the rows of Y; grouped, of experts as independent choices fill
-// them (the offsets are on the device): those with rows, each with half a tile to spare.
-double row_tiles(const I8Args& a, bool grouped, int bm) {
-  if (!grouped) return (a.M + bm - 1) / bm;
-  const double used = a.E * (1.0 - std::exp(-(double)a.M / a.E));
-  return used * std::max(1.0, a.M / used / bm + 0.5);
-}
-
+// The tile for a call.  Grouped, the offsets are on the device: the rows are taken as independent
+// choices of the experts, those with rows each having half a tile to spare.
 int pick_tile(const I8Args& a, bool grouped, int cus) {
+  const float used = grouped ? a.E * (1.f - std::exp(-(float)a.M / a.E)) : 1.f, each = a.M / used;
   int best = 0;
-  double least = 1e30;
+  float least = 1e30f;
   for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
     const TileCost& c = kTiles[i];
-    const double n = std::ceil(row_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) / cus);
-    const double t = c.t0 + a.nk * kStep / 1024.0 * std::max((double)c.one, c.each * n);
+    const float rows = grouped ? used * std::max(1.f, each / c.bm + 0.5f) : std::ceil(each / c.bm);
+    const float n = std::ceil(rows * ((a.N + c.bn - 1) / c.bn) / cus);
+    const float t = c.t0 + a.nk * (kStep / 1024.f) * std::max(c.one, c.each * n);
     if (t < least) least = t, best = i;
   }
   return best;
@@ -808,6 +804,7 @@ int check_size(const char* who, int M, int N, int K) {
   if (M < 0 || N < 0 || K < 1) return set_error(TIERMM_EINVAL, "%s: bad size %d x %d x %d", who, M, N, K);
   if (K > kMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: K = %d, at most %d", who, K, kMaxK);
   if (M > (1 << 23)) return set_error(TIERMM_UNSUPPORTED, "%s: %d rows, at most %d", who, M, 1 << 23);
+  if (N > (1 << 26)) return set_error(TIERMM_UNSUPPORTED, "%s: %d columns, at most %d", who, N, 1 << 26);
   return TIERMM_OK;
 }
 int check_i8_rows(const char* who, const char* what, const void* p, size_t rb, int K) {

@@ -6,10 +6,10 @@
 // All are bound by memory: a row is read or written once, in 16-byte units, with the
 // few indices of a token in scalar registers.  No atomics on results: every sum has one
 // owner and one order, so results do not change between runs.  Measured on 4096 tokens,
-// top 8 of 64, rows of 2048 (a large copy moves 5.1 TB/s): sort 51-54 us fp32 (5.6-5.9
-// TB/s), 24 us bf16; its gradient 46 and 23.5 (6.4-6.6); the weighted sum 47 and 23.6; its
-// gradient 115 and 60 (4.9-5.0, the same bytes read as written).  Rows of 2047 bf16, which start at
-// any 2 bytes: 26, 26 and 68 us.
+// top 8 of 64, rows of 2048, between buffers that the caches do not hold (a large copy moves
+// 5.1 TB/s): sort 53 us fp32 (5.7 TB/s), 27 us bf16; its gradient 54 and 27; the weighted sum's
+// 27.5 in bf16 (5.5); that one's gradient 115 and 62 (4.7-4.9, the same bytes read as written).
+// Eight tokens: 4 us each from Python, whose call takes as long.
 #include "tm_rows.h"
 
 namespace tiermm {
@@ -224,7 +224,11 @@ struct RowArgs {
 // Xs[places[t][j]] = X[t]: a token's row is read once and written topk times, by the
 // workgroups of blockIdx.x = t, 256 units each.  Those of token t also clear the rows
 // t * topk .. + topk - 1 of Xs that hold no pair.
-template <int XT>
+//
+// NT: the copies go past the caches, where rows are whole 16-byte units: 59 -> 53 us in fp32 at
+// 4096 tokens, top 8, 2048 columns, 30 -> 27 in bf16, between buffers that the caches do not
+// hold; on rows of 2047 bf16, whose units straddle lines, 36 -> 39.
+template <int XT, bool NT>
 __global__ __launch_bounds__(256) void moe_sort_kernel(const RowArgs a) {
   using R = Rows<XT>;
   const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * R::EPU;
@@ -232,14 +236,22 @@ __global__ __launch_bounds__(256) void moe_sort_kernel(const RowArgs a) {
   const u32x4 u = R::get(a.x + (size_t)t * a.ldx, c, a.cols);
   for (int j = 0; j < a.topk; ++j) {
     const int i = t * a.topk + j, p = a.places[i];
-    if ((uint32_t)p < (uint32_t)a.P) R::set(a.y + (size_t)p * a.ldy, c, a.cols, u);
+    if ((uint32_t)p < (uint32_t)a.P) {
+      if constexpr (NT) R::set_nt(a.y + (size_t)p * a.ldy, c, a.cols, u);
+      else R::set(a.y + (size_t)p * a.ldy, c, a.cols, u);
+    }
     if (a.sorted[i] < 0) R::set(a.y + (size_t)i * a.ldy, c, a.cols, u32x4{0u, 0u, 0u, 0u});
   }
 }
 
 // out[t] = sum_j w[t][j] Ys[places[t][j]], in j order in fp32 (WEIGHTED false: w = 1).
 // Eight rows are in flight at a time.
-template <int XT, bool WEIGHTED>
+//
+// NT: rows of more bytes in all than the last-level cache keeps from one call to the next are
+// read past it: 68 -> 54 us in fp32 at 4096 tokens, top 8, 2048 columns (256 MiB), 26.5 -> 24.6
+// at 80 MiB, but 7.5 -> 7.7 at 32 and 12.2 -> 13.7 at 64; on rows of 1023 bf16 16 -> 20.
+constexpr size_t kStreamBytes = 72 << 20;
+template <int XT, bool WEIGHTED, bool NT>
 __global__ __launch_bounds__(256) void moe_gather_sum_kernel(const RowArgs a) {
   using R = Rows<XT>;
   const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * R::EPU;
@@ -253,7 +265,8 @@ __global__ __launch_bounds__(256) void moe_gather_sum_kernel(const RowArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       p[j] = j0 + j < a.topk ? a.places[(size_t)t * a.topk + j0 + j] : -1;
-      if ((uint32_t)p[j] < (uint32_t)a.P) u[j] = R::get(a.x + (size_t)p[j] * a.ldx, c, a.cols);
+      if ((uint32_t)p[j] < (uint32_t)a.P) u[j] = NT ? R::get_nt(a.x + (size_t)p[j] * a.ldx, c, a.cols)
+                                                 : R::get(a.x + (size_t)p[j] * a.ldx, c, a.cols);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -322,6 +335,9 @@ int check_rows(const char* who, int xtype, int T, int topk, int cols, int* es) {
   return TIERMM_OK;
 }
 bool misaligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
+bool stream_rows(const void* rows, const RowArgs& a) {
+  return !misaligned(rows, 16) && a.ldx % 16 == 0 && (size_t)a.P * a.ldx >= kStreamBytes;
+}
 
 }  // namespace
 }  // namespace tiermm
@@ -389,7 +405,12 @@ int tiermm_moe_sort(const void* X, int xtype, size_t ldx, const int32_t* token_p
   const RowArgs a = {(const uint8_t*)X, (uint8_t*)X_sorted, token_pairs, sorted_pairs, nullptr,
                      ldx * es, lds * es, T * topk, topk, K};
   const dim3 grid(T, (K * (size_t)es + 4095) / 4096);
-  with_rows(xtype, [&](auto xt) { moe_sort_kernel<decltype(xt)::value><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+  const bool whole = !misaligned(X_sorted, 16) && lds * es % 16 == 0;
+  with_rows(xtype, [&](auto xt) {
+    constexpr int XT = decltype(xt)::value;
+    if (whole) moe_sort_kernel<XT, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else moe_sort_kernel<XT, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+  });
   TM_LAUNCH_CHECK("tiermm_moe_sort: launch");
   return TIERMM_OK;
 }
@@ -409,7 +430,9 @@ int tiermm_moe_sort_grad(const void* dX_sorted, int xtype, size_t lds, const int
                      lds * es, ldx * es, T * topk, topk, K};
   const dim3 grid(T, (K * (size_t)es + 4095) / 4096);
   with_rows(xtype, [&](auto xt) {
-    moe_gather_sum_kernel<decltype(xt)::value, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    constexpr int XT = decltype(xt)::value;
+    if (stream_rows(dX_sorted, a)) moe_gather_sum_kernel<XT, false, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else moe_gather_sum_kernel<XT, false, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   });
   TM_LAUNCH_CHECK("tiermm_moe_sort_grad: launch");
   return TIERMM_OK;
@@ -431,7 +454,9 @@ int tiermm_moe_unsort(const void* Y_sorted, int ytype, size_t lds, const int32_t
                      lds * es, ldo * es, T * topk, topk, N};
   const dim3 grid(T, (N * (size_t)es + 4095) / 4096);
   with_rows(ytype, [&](auto xt) {
-    moe_gather_sum_kernel<decltype(xt)::value, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    constexpr int XT = decltype(xt)::value;
+    if (stream_rows(Y_sorted, a)) moe_gather_sum_kernel<XT, true, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else moe_gather_sum_kernel<XT, true, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   });
   TM_LAUNCH_CHECK("tiermm_moe_unsort: launch");
   return TIERMM_OK;

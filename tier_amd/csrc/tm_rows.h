@@ -46,7 +46,7 @@ struct Rows {
   }
   static __device__ __forceinline__ u32x4 raw(const uint8_t* p) { return *(const u32x4_a2*)p; }
   static __device__ __forceinline__ void put(uint8_t* p, u32x4 u) { *(u32x4_a2*)p = u; }
-  // The same, not to be read again soon.
+  // A store past the caches, of what is not read again soon.
   static __device__ __forceinline__ void set_nt(uint8_t* row, int c, int cols, u32x4 u) {
     uint8_t* p = row + (size_t)c * ES;
     if (c + EPU <= cols) __builtin_nontemporal_store(u, (u32x4_a2*)p);
@@ -75,6 +75,11 @@ struct Rows {
   static __device__ __forceinline__ u32x4 get(const uint8_t* row, int c, int cols) {
     const uint8_t* p = row + (size_t)c * ES;
     return c + EPU <= cols ? raw(p) : raw_part(p, cols - c);
+  }
+  // The same for rows that are read once.
+  static __device__ __forceinline__ u32x4 get_nt(const uint8_t* row, int c, int cols) {
+    const uint8_t* p = row + (size_t)c * ES;
+    return c + EPU <= cols ? __builtin_nontemporal_load((const u32x4_a2*)p) : raw_part(p, cols - c);
   }
   static __device__ __forceinline__ void set(uint8_t* row, int c, int cols, u32x4 u) {
     uint8_t* p = row + (size_t)c * ES;
