@@ -389,8 +389,8 @@ int tiermm_i8_quant(const void* x, int xtype, size_t ldx, int8_t* q, size_t rb, 
 /* The product; bias fp32 [N] or NULL; ytype TIERMM_F32, TIERMM_F16 or TIERMM_BF16. */
 int tiermm_i8_gemm(const int8_t* Xq, size_t rbx, const float* sx, const int8_t* W, size_t rbw, const float* sw,
                    const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K, tiermm_stream_t stream);
-/* tiermm_i8_quant and tiermm_i8_gemm in one call, the same result bit for bit.  ws 16-byte
- * aligned. */
+/* tiermm_i8_quant and tiermm_i8_gemm in one call, the same result bit for bit; one or two
+ * rows of x are quantized by the product's own kernel.  ws 16-byte aligned. */
 int tiermm_i8_linear(const void* x, int xtype, size_t ldx, const int8_t* W, size_t rbw, const float* sw,
                      const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K, void* ws, size_t ws_bytes,
                      tiermm_stream_t stream);

@@ -260,14 +260,24 @@ __device__ __forceinline__ void wave_lds_wait() {
 
 // BM rows of X times BN rows of W by WVM x WVN waves of WM x WN blocks of 32 x 32.
 //
-// A stage is 128 bytes of every row, brought to LDS by global_load_lds; two stages take
+// A stage is 128 bytes of every row, brought to LDS by global_load_lds; S stages take
 // turns.  A row's 16-byte chunk c lies at slot c ^ ((row >> 1) & 7): the 16 rows that one
-// cycle of a fragment read touches then cover all the banks.  A stage is four MFMA
-// steps of K = 32.  While the products of one step run, the fragments of the next come in,
-// one read between two MFMAs, and the loads of the stage after next go out, spread the same
-// way from the step after the barrier that frees their place on.
+// cycle of a fragment read touches then cover all the banks (c ^ (row & 7) spent half of the
+// LDS cycles on conflicts).  A stage is four MFMA steps of K = 32.  While the products of one
+// step run, the fragments of the next come in, one read between two MFMAs, and the loads of
+// stage kt + S go out, spread the same way from the step after the barrier that frees their
+// place on (256 x 256, a stage: 2993 -> 2760 cycles; the MFMAs alone take 2048).
 //
-// W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y.
+// W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y;
+// rows leave through LDS in 16-byte units (stored from the lanes, element by element, the
+// epilogue took 12 us a tile; so it takes 4).
+//
+// Measured: 4096 x 14336 x 5120, bf16 out, 256 x 320 tiles: 244-252 us, 2.4-2.5 PFLOP/s (a
+// library's int8 product of this size without scales: 2.12).  The card's power limit bounds
+// it: the clock falls to 1.6-1.7 GHz and the MFMAs alone, on operands that stay put, take 175
+// of the K loop's 240 us; on zeros the clock stays at 2.36 GHz and the call takes 224 us.
+// Larger tiles cost less power for loads and LDS reads a product: 256 x 256 266, 128 x 128 315.
+// No faster: 64-byte stages in rings of 4 and 5 (312, 326), four waves of 128 x 128 (337).
 template <int YT, int BM, int BN, int WVM, int WVN, int S, bool GROUPED>
 __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, NM = WM * WN, NF = WM + WN;
@@ -476,6 +486,12 @@ __device__ __forceinline__ int wave_sums(const int (&v)[R]) {
 // Up to MX rows of x, quantized by each workgroup into LDS while its first weights are on the
 // way.  A wave takes R rows of W in 1 KiB pieces, 16 bytes a lane, so each load is eight whole
 // lines of one row; v_dot4 on 16 bytes a lane costs a tenth of what the bytes take to come.
+//
+// Bound by the stream of W, and by x's preparation in front of it (some 2 us): 1 x 28672 x 14336
+// bf16 59-61 us (6.7-7.0 TB/s), 1 x 14336 x 5120 13.0-13.5 (5.4-5.6), 1 x 1024 x 5120 fp32
+// 4.3-5.1.  Two rows a wave and 16 waves: each CU prepares x once or twice; 4 waves 15.6 us, four
+// rows and 4 waves 14.6, at 14336 rows; one row a wave and 8 waves at 1024: 5.1 against 7.0.  On
+// MFMA 16x16x64 with W straight from memory, 16 rows of 64 bytes a load: 16.7.
 template <int YT, int XT, int MX, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t codes[];  // [MX][whole KiB]
@@ -572,6 +588,13 @@ int launch_gemv(const I8Args& a, hipStream_t s, const char* who) {
 // WVN x WVK waves share the columns and the 64-byte steps of a stage, which holds KS * 128 bytes
 // of every row.  A ring of S stages keeps S - 1 on their way by global_load_lds, whole lines of
 // eight rows a load; one barrier a stage.
+//
+// A lone workgroup streams 60-80 GB/s into its CU (a plain loop of such loads out of L2: 131; 16
+// rows of 64 bytes straight to registers: 38), so few columns take small tiles, and long stages,
+// whose steps the waves share: 8 x 1024 x 5120 5.0 us on 16 x 16, 10.6 on 16 x 64, 14.1 on 128 x 64.
+// With columns enough W's bytes bound it: 8 x 14336 x 5120 12.2 us (6.0 TB/s), routed experts of
+// 8 tokens (16 x 64) 5.5 TB/s.  Waves that share only K read each operand once: 32 x 32 1 x 8
+// waves 6.4 us against 7.1 of 2 x 8 at 8 x 1024 x 5120.  Rings of 6 and 8 stages were no faster.
 template <int YT, int BM, int BN, int WVN, int WVK, int KS, int S, bool GROUPED>
 __global__ __launch_bounds__(64 * WVN * WVK) void i8_tile_kernel(const I8Args a) {
   constexpr int NW = WVN * WVK, MB = BM / 16, NB = BN / WVN / 16, KK = 2 * KS / WVK;
