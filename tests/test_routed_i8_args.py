@@ -132,3 +132,22 @@ def test_row_bytes():
         128, 128, 128, 256, 5120, 1408, 133120, 0, 0, 0]
     assert tier_amd.i8_linear_ws_bytes(3, 5, 300) >= 3 * 384 + 12
     assert tier_amd.i8_linear_ws_bytes(0, 5, 300) == 0
+
+
+def test_call_arguments():
+    """tier_amd._call: integers of either sign, None as a null pointer, and nothing else."""
+    from tier_amd import _call
+    import ctypes
+    f = _call.Call(ctypes.cast(L().tiermm_moe_plan, ctypes.c_void_p).value, 10)
+    assert f(A, -1, 2, 8, A, A, A, None, 0, None) == EINVAL
+    assert f(None, 4, 2, 8, A, A, A, None, 0, None) == EINVAL
+    for bad in ((A,) * 9, (A,) * 11, ("x",) + (1,) * 9, (1.5,) + (1,) * 9):
+        with pytest.raises(TypeError):
+            f(*bad)
+    with pytest.raises(TypeError):
+        f(*(A,) * 9, stream=None)
+    for address, n in ((0, 3), (16, -1), (16, 21)):
+        with pytest.raises(ValueError):
+            _call.Call(address, n)
+    with pytest.raises(tier_amd.TiermmError):
+        tier_amd.moe_plan(A, -1, 2, 8, A, A, A)

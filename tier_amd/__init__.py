@@ -86,6 +86,11 @@ class TiermmUnsupported(TiermmError):
 if not os.path.isfile(LIB_PATH):
     raise ImportError(f"{LIB_PATH} is not built: run `python -m tier_amd.build` (no CPU fallback exists)")
 
+try:
+    from . import _call
+except ImportError as e:
+    raise ImportError(f"{os.path.join(HERE, '_call.so')} is not built: run `python -m tier_amd.build`") from e
+
 _L = ctypes.CDLL(LIB_PATH)
 _vp, _sz, _i, _f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
 
@@ -182,6 +187,18 @@ def chat_fp3_noalloc(W: int, x: int, y: int, M: int, K: int, N: int, ldo: int, s
         return False
     _check(code)
     return True
+
+
+# Entry points whose small calls a ctypes call (1.3 to 2 us) would take longer than: name -> function
+# of the same arguments (integers, addresses, None), the status back.
+_fast = {n: _call.Call(ctypes.cast(getattr(_L, n), _vp).value, len(getattr(_L, n).argtypes))
+         for n in ("tiermm_moe_plan", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
+                   "tiermm_moe_unsort_grad", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
+                   "tiermm_i8_gemm_grouped")}
+_moe_plan, _moe_sort, _moe_sort_grad = (_fast["tiermm_moe_" + n] for n in ("plan", "sort", "sort_grad"))
+_moe_unsort, _moe_unsort_grad = _fast["tiermm_moe_unsort"], _fast["tiermm_moe_unsort_grad"]
+_i8_quant, _i8_gemm, _i8_linear, _i8_gemm_grouped = (
+    _fast["tiermm_i8_" + n] for n in ("quant", "gemm", "linear", "gemm_grouped"))
 
 
 def lib():
@@ -459,8 +476,8 @@ def moe_plan(expert_ids: int, T: int, topk: int, n_experts: int, expert_offsets:
     """The order of T * topk (token, expert) pairs by expert: device int32 tables
     expert_offsets[n_experts + 1], token_pairs[T][topk] (places), sorted_pairs[T * topk].
     Ids outside [0, n_experts) are dropped pairs."""
-    _check(_L.tiermm_moe_plan(expert_ids, T, topk, n_experts, expert_offsets, token_pairs, sorted_pairs, ws, ws_bytes,
-                              _s(stream)))
+    _check(_moe_plan(expert_ids, T, topk, n_experts, expert_offsets, token_pairs, sorted_pairs, ws, ws_bytes,
+                     _s(stream)))
 
 
 def moe_plan_ws_bytes(T: int, topk: int, n_experts: int) -> int:
@@ -470,27 +487,27 @@ def moe_plan_ws_bytes(T: int, topk: int, n_experts: int) -> int:
 def moe_sort(X: int, xtype: int, ldx: int, token_pairs: int, sorted_pairs: int, X_sorted: int, lds: int, T: int,
              topk: int, K: int, stream=None) -> None:
     """X_sorted[p] = X[sorted_pairs[p] / topk] (zeros where no pair is); xtype F32, F16 or BF16."""
-    _check(_L.tiermm_moe_sort(X, xtype, ldx, token_pairs, sorted_pairs, X_sorted, lds, T, topk, K, _s(stream)))
+    _check(_moe_sort(X, xtype, ldx, token_pairs, sorted_pairs, X_sorted, lds, T, topk, K, _s(stream)))
 
 
 def moe_sort_grad(dX_sorted: int, xtype: int, lds: int, token_pairs: int, dX: int, ldx: int, T: int, topk: int, K: int,
                   stream=None) -> None:
     """dX[t] = sum_j dX_sorted[token_pairs[t][j]]."""
-    _check(_L.tiermm_moe_sort_grad(dX_sorted, xtype, lds, token_pairs, dX, ldx, T, topk, K, _s(stream)))
+    _check(_moe_sort_grad(dX_sorted, xtype, lds, token_pairs, dX, ldx, T, topk, K, _s(stream)))
 
 
 def moe_unsort(Y_sorted: int, ytype: int, lds: int, token_pairs: int, weights: int, out: int, ldo: int, T: int,
                topk: int, N: int, stream=None) -> None:
     """out[t] = sum_j weights[t][j] * Y_sorted[token_pairs[t][j]], weights fp32 [T][topk]."""
-    _check(_L.tiermm_moe_unsort(Y_sorted, ytype, lds, token_pairs, weights, out, ldo, T, topk, N, _s(stream)))
+    _check(_moe_unsort(Y_sorted, ytype, lds, token_pairs, weights, out, ldo, T, topk, N, _s(stream)))
 
 
 def moe_unsort_grad(dout: int, ytype: int, ldo: int, Y_sorted: int, lds: int, token_pairs: int, sorted_pairs: int,
                     weights: int, dY_sorted: int, ldd: int, dweights: int, T: int, topk: int, N: int,
                     stream=None) -> None:
     """dY_sorted[p] = w_p * dout[its token] and dweights[t][j] = <dout[t], Y_sorted[token_pairs[t][j]]>."""
-    _check(_L.tiermm_moe_unsort_grad(dout, ytype, ldo, Y_sorted, lds, token_pairs, sorted_pairs, weights, dY_sorted,
-                                     ldd, dweights, T, topk, N, _s(stream)))
+    _check(_moe_unsort_grad(dout, ytype, ldo, Y_sorted, lds, token_pairs, sorted_pairs, weights, dY_sorted, ldd,
+                            dweights, T, topk, N, _s(stream)))
 
 
 # ------------------------------------------------------------- int8 products
@@ -501,19 +518,19 @@ def i8_row_bytes(K: int) -> int:
 
 def i8_quant(x: int, xtype: int, ldx: int, q: int, rb: int, scale: int, M: int, K: int, stream=None) -> None:
     """int8 codes and one fp32 scale for each of M rows of x (F32, F16 or BF16)."""
-    _check(_L.tiermm_i8_quant(x, xtype, ldx, q, rb, scale, M, K, _s(stream)))
+    _check(_i8_quant(x, xtype, ldx, q, rb, scale, M, K, _s(stream)))
 
 
 def i8_gemm(Xq: int, rbx: int, sx: int, W: int, rbw: int, sw: int, bias: int | None, Y: int, ytype: int, ldy: int,
             M: int, N: int, K: int, stream=None) -> None:
     """Y[m][n] = sx[m] * sw[n] * <Xq[m], W[n]> (+ bias[n])."""
-    _check(_L.tiermm_i8_gemm(Xq, rbx, sx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, _s(stream)))
+    _check(_i8_gemm(Xq, rbx, sx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, _s(stream)))
 
 
 def i8_linear(x: int, xtype: int, ldx: int, W: int, rbw: int, sw: int, bias: int | None, Y: int, ytype: int, ldy: int,
               M: int, N: int, K: int, ws: int | None = None, ws_bytes: int = 0, stream=None) -> None:
     """i8_quant of x and i8_gemm in one call."""
-    _check(_L.tiermm_i8_linear(x, xtype, ldx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, ws, ws_bytes, _s(stream)))
+    _check(_i8_linear(x, xtype, ldx, W, rbw, sw, bias, Y, ytype, ldy, M, N, K, ws, ws_bytes, _s(stream)))
 
 
 def i8_linear_ws_bytes(M: int, N: int, K: int) -> int:
@@ -525,8 +542,8 @@ def i8_gemm_grouped(Xq: int, rbx: int, sx: int, rows: int | None, n_rows: int, t
                     stream=None) -> None:
     """The experts' int8 products of a routed batch, by moe_plan's device tables: row p of Y
     is row rows[p] / topk of Xq times its expert's weight."""
-    _check(_L.tiermm_i8_gemm_grouped(Xq, rbx, sx, rows, n_rows, topk, expert_offsets, n_experts, W, rbw, sw, Y, ytype,
-                                     ldy, P, N, K, _s(stream)))
+    _check(_i8_gemm_grouped(Xq, rbx, sx, rows, n_rows, topk, expert_offsets, n_experts, W, rbw, sw, Y, ytype, ldy, P,
+                            N, K, _s(stream)))
 
 
 def qlinear(W: int, qtype: int, rb: int, x: int, y: int, M: int, N: int, K: int, ws: int | None = None,

@@ -2,7 +2,8 @@
 
 Run ``python -m tier_amd.build`` or call ``build()``; ``__graft_entry__.build()``
 calls it.  Objects go to ``tier_amd/_build/``; the library to ``tier_amd/libtiermm.so``,
-and bench.py's measurement kernels (probe.hip) to ``tier_amd/libtiermm_probe.so``.
+bench.py's measurement kernels (probe.hip) to ``tier_amd/libtiermm_probe.so``, the
+Python calls of the routed-row and int8 entry points (call.c) to ``tier_amd/_call.so``.
 """
 from __future__ import annotations
 
@@ -10,6 +11,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -17,6 +19,8 @@ OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libtiermm.so")
 # measurement kernels for bench.py only (the plain-read floor and the fp16 MFMA ceiling)
 PROBE_LIB = os.path.join(HERE, "libtiermm_probe.so")
+# tier_amd._call: entry points of integer arguments called without ctypes
+CALL_LIB = os.path.join(HERE, "_call.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
@@ -68,6 +72,10 @@ def build(verbose: bool = False) -> str:
     tmp = PROBE_LIB + ".tmp"
     _run([HIPCC] + HIP_FLAGS + ["-shared", "-o", tmp, os.path.join(CSRC, "probe.hip")])
     os.replace(tmp, PROBE_LIB)
+    tmp = CALL_LIB + ".tmp"
+    _run(["gcc", "-O2", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", tmp,
+          os.path.join(CSRC, "call.c")])
+    os.replace(tmp, CALL_LIB)
     return LIB
 
 
