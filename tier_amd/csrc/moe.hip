@@ -24,15 +24,15 @@ namespace {
 // That is E + 1 reads of P ids through L2, but one launch and no exchange between
 // workgroups: 32768 pairs, 64 experts 7.6 us, where the two launches below take 8.3.  A tile
 // is 4 ids a thread; NT tiles stay in registers (16 of them spilled: the limit of 8).
-constexpr int kPlanThreads = 1024, kPlanTile = 4 * kPlanThreads, kPlanMost = 8 * kPlanTile;
+constexpr int kPlanMost = 8 * 4096;
 typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <int NT>
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int P, int E,
+template <int THREADS, int NT>
+__global__ __launch_bounds__(THREADS) void moe_plan_kernel(const int32_t* __restrict__ ids, int P, int E,
                                                                 int32_t* __restrict__ offsets,
                                                                 int32_t* __restrict__ places,
                                                                 int32_t* __restrict__ sorted) {
-  constexpr int NW = kPlanThreads / 64;
+  constexpr int NW = THREADS / 64, TILE = 4 * THREADS;
   __shared__ int own[NT * NW], less[NW];
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint64_t below = (1ull << lane) - 1;
@@ -42,8 +42,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   i32x4_a4 id[NT];  // every load on its way before the first is used
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int i0 = t * kPlanTile + 4 * tid;
-    if ((t + 1) * kPlanTile <= P) {
+    const int i0 = t * TILE + 4 * tid;
+    if ((t + 1) * TILE <= P) {
       id[t] = *(const i32x4_a4*)(ids + i0);
     } else {
 #pragma unroll
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int i0 = t * kPlanTile + 4 * tid;
+    const int i0 = t * TILE + 4 * tid;
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
   for (int t = 0; t < NT; ++t) {
     const uint32_t m = mine >> (4 * t);
     int at = own[t * NW + wave] + first[t];
-    const int i0 = t * kPlanTile + 4 * tid;
+    const int i0 = t * TILE + 4 * tid;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (m >> i & 1) {
@@ -234,13 +234,24 @@ __global__ __launch_bounds__(256) void moe_sort_kernel(const RowArgs a) {
   const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * R::EPU;
   if (c >= a.cols) return;
   const u32x4 u = R::get(a.x + (size_t)t * a.ldx, c, a.cols);
-  for (int j = 0; j < a.topk; ++j) {
-    const int i = t * a.topk + j, p = a.places[i];
-    if ((uint32_t)p < (uint32_t)a.P) {
-      if constexpr (NT) R::set_nt(a.y + (size_t)p * a.ldy, c, a.cols, u);
-      else R::set(a.y + (size_t)p * a.ldy, c, a.cols, u);
+  for (int j0 = 0; j0 < a.topk; j0 += 8) {
+    int p[8], pair[8];  // eight places' loads at a time, before the first store
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = t * a.topk + min(j0 + j, a.topk - 1);
+      p[j] = a.places[i];
+      pair[j] = a.sorted[i];
     }
-    if (a.sorted[i] < 0) R::set(a.y + (size_t)i * a.ldy, c, a.cols, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= a.topk) break;
+      if ((uint32_t)p[j] < (uint32_t)a.P) {
+        uint8_t* row = a.y + (size_t)p[j] * a.ldy;
+        if constexpr (NT) R::set_nt(row, c, a.cols, u);
+        else R::set(row, c, a.cols, u);
+      }
+      if (pair[j] < 0) R::set(a.y + (size_t)(t * a.topk + j0 + j) * a.ldy, c, a.cols, u32x4{0u, 0u, 0u, 0u});
+    }
   }
 }
 
@@ -262,9 +273,15 @@ __global__ __launch_bounds__(256) void moe_gather_sum_kernel(const RowArgs a) {
   for (int j0 = 0; j0 < a.topk; j0 += 8) {
     u32x4 u[8];
     int p[8];
+    float w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = j0 + j < a.topk ? a.places[(size_t)t * a.topk + j0 + j] : -1;
+      const int i = t * a.topk + min(j0 + j, a.topk - 1);
+      p[j] = j0 + j < a.topk ? a.places[i] : -1;
+      w[j] = WEIGHTED ? a.w[i] : 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
       if ((uint32_t)p[j] < (uint32_t)a.P) u[j] = NT ? R::get_nt(a.x + (size_t)p[j] * a.ldx, c, a.cols)
                                                  : R::get(a.x + (size_t)p[j] * a.ldx, c, a.cols);
     }
@@ -273,9 +290,8 @@ __global__ __launch_bounds__(256) void moe_gather_sum_kernel(const RowArgs a) {
       if ((uint32_t)p[j] >= (uint32_t)a.P) continue;
       float v[R::EPU];
       R::widen(u[j], v);
-      const float w = WEIGHTED ? a.w[(size_t)t * a.topk + j0 + j] : 1.f;
 #pragma unroll
-      for (int i = 0; i < R::EPU; ++i) acc[i] = WEIGHTED ? fmaf(w, v[i], acc[i]) : acc[i] + v[i];
+      for (int i = 0; i < R::EPU; ++i) acc[i] = WEIGHTED ? fmaf(w[j], v[i], acc[i]) : acc[i] + v[i];
     }
   }
   R::set(a.y + (size_t)t * a.ldy, c, a.cols, R::narrow(acc));
@@ -381,11 +397,12 @@ int tiermm_moe_plan(const int32_t* expert_ids, int T, int topk, int n_experts, i
     TM_LAUNCH_CHECK("tiermm_moe_plan: places");
     return TIERMM_OK;
   }
-#define PLAN(NT) moe_plan_kernel<NT><<<E + 1, kPlanThreads, 0, s>>>(expert_ids, P, E, expert_offsets, token_pairs, sorted_pairs)
-  if (P <= kPlanTile) PLAN(1);
-  else if (P <= 2 * kPlanTile) PLAN(2);
-  else if (P <= 4 * kPlanTile) PLAN(4);
-  else PLAN(8);
+#define PLAN(THREADS, NT) moe_plan_kernel<THREADS, NT><<<E + 1, THREADS, 0, s>>>(expert_ids, P, E, expert_offsets, token_pairs, sorted_pairs)
+  if (P <= 1024) PLAN(256, 1);
+  else if (P <= 4096) PLAN(1024, 1);
+  else if (P <= 2 * 4096) PLAN(1024, 2);
+  else if (P <= 4 * 4096) PLAN(1024, 4);
+  else PLAN(1024, 8);
 #undef PLAN
   TM_LAUNCH_CHECK("tiermm_moe_plan: launch");
   return TIERMM_OK;
