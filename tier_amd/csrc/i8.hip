@@ -489,8 +489,8 @@ __device__ __forceinline__ int wave_sums(const int (&v)[R]) {
 //
 // Bound by the stream of W, and by x's preparation in front of it (some 2 us): 1 x 28672 x 14336
 // bf16 59-61 us (6.7-7.0 TB/s), 1 x 14336 x 5120 13.0-13.5 (5.4-5.6), 1 x 1024 x 5120 fp32
-// 4.3-5.1.  Two rows a wave and 16 waves: each CU prepares x once or twice; 4 waves 15.6 us, four
-// rows and 4 waves 14.6, at 14336 rows; one row a wave and 8 waves at 1024: 5.1 against 7.0.  On
+// 4.1-4.6.  Two rows a wave and 16 waves: each CU prepares x once or twice; 4 waves 15.6 us, four
+// rows and 4 waves 14.6, at 14336 rows; one row a wave and 8 waves at 1024: 4.5 against 7.0.  On
 // MFMA 16x16x64 with W straight from memory, 16 rows of 64 bytes a load: 16.7.
 template <int YT, int XT, int MX, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
@@ -517,14 +517,38 @@ __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
     if (u < nc) load(u, u);
 
   using X = Rows<XT>;
+  // With one row of W a wave, x is held in registers (all its loads on their way at once) where
+  // they have room: 1 x 1024 x 5120 fp32 5.1 -> 4.5 us, two tokens 6.6 -> 5.5.  With two rows, whose
+  // 16 waves would then need more than the 64 registers of two workgroups a CU, it is read twice:
+  // 13.4 against 15.7 us at 1 x 14336 x 5120 bf16.
+  constexpr int XR = 4, STEP = 64 * NW * X::EPU;
+  const int k0 = tid * X::EPU;
+  const bool held = R == 1 && a.K <= XR * STEP;
+  auto row = [&](int m) { return a.X + (size_t)min(m, a.M - 1) * a.rbx; };
+  u32x4 xu[MX][XR];
   uint32_t top[MX] = {};
-  for (int k = tid * X::EPU; k < a.K; k += 64 * NW * X::EPU)
+  auto more = [&](int m, const u32x4& u) __attribute__((always_inline)) {
+    float v[X::EPU];
+    X::widen(u, v);
+    top[m] = top_bits(v, top[m]);
+  };
+  if (held) {
 #pragma unroll
-    for (int m = 0; m < MX; ++m) {
-      float v[X::EPU];
-      X::widen(X::get(a.X + (size_t)min(m, a.M - 1) * a.rbx, k, a.K), v);
-      top[m] = top_bits(v, top[m]);
-    }
+    for (int m = 0; m < MX; ++m)
+#pragma unroll
+      for (int i = 0; i < XR; ++i) {
+        const int k = k0 + i * STEP;
+        xu[m][i] = k < a.K ? X::get(row(m), k, a.K) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+    for (int m = 0; m < MX; ++m)
+#pragma unroll
+      for (int i = 0; i < XR; ++i) more(m, xu[m][i]);
+  } else {
+    for (int k = k0; k < a.K; k += STEP)
+#pragma unroll
+      for (int m = 0; m < MX; ++m) more(m, X::get(row(m), k, a.K));
+  }
 #pragma unroll
   for (int m = 0; m < MX; ++m) {
 #pragma unroll
@@ -534,15 +558,23 @@ __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
   __syncthreads();
 #pragma unroll
   for (int m = 0; m < MX; ++m) {
-    #pragma unroll
+#pragma unroll
     for (int w = 0; w < NW; ++w) top[m] = max(top[m], red[m][w]);
     const RowScale s = row_scale_of(top[m]);
     if (tid == 0) row_scale[m] = s.sc;
-    for (int k = tid * X::EPU; k < Kp; k += 64 * NW * X::EPU) {
-      float v[X::EPU] = {};
-      if (k < a.K) X::widen(X::get(a.X + (size_t)min(m, a.M - 1) * a.rbx, k, a.K), v);
+    auto put = [&](int k, const u32x4& u) __attribute__((always_inline)) {
+      float v[X::EPU];
+      X::widen(u, v);
+      uint8_t* to = codes + m * ldc + k;
+      if constexpr (X::EPU == 8) *(u32x2*)to = u32x2{codes4(v, s), codes4(v + 4, s)};
+      else *(uint32_t*)to = codes4(v, s);
+    };
+    if (held) {
 #pragma unroll
-      for (int i = 0; i < X::EPU; i += 4) *(uint32_t*)(codes + m * ldc + k + i) = codes4(v + i, s);
+      for (int i = 0; i < XR; ++i)
+        if (k0 + i * STEP < Kp) put(k0 + i * STEP, xu[m][i]);
+    } else {
+      for (int k = k0; k < Kp; k += STEP) put(k, k < a.K ? X::get(row(m), k, a.K) : u32x4{0u, 0u, 0u, 0u});
     }
   }
   __syncthreads();
