@@ -280,9 +280,9 @@ __device__ __forceinline__ void wave_lds_wait() {
 // No faster: 64-byte stages in rings of 4 and 5 (312, 326), four waves of 128 x 128 (337).
 template <int YT, int BM, int BN, int WVM, int WVN, int S, bool GROUPED>
 __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a) {
-  constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, NM = WM * WN, NF = WM + WN;
+  constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, NF = WM + WN;
   constexpr int STAGE = (BM + BN) * kStep, INST = STAGE / 1024 / NW;
-  static_assert(WM * WVM * 32 == BM && WN * WVN * 32 == BN && INST * NW * 1024 == STAGE, "whole blocks and loads a wave");
+  static_assert(WM <= 2 && WM * WVM * 32 == BM && WN * WVN * 32 == BN && INST * NW * 1024 == STAGE, "whole blocks and loads a wave");
   // loads of a stage by the step that issues them: 3 (of the stage before last), 0 and 1
   constexpr int D0 = (INST + 2) / 3, D1 = (INST - D0 + 1) / 2, D2 = INST - D0 - D1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -337,38 +337,44 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0;
 
   const int wm = wave % WVM, wn = wave / WVM, fr = lane & 31, fh = lane >> 5, turn = (fr >> 1) & 7;
-  const uint32_t xrow = (uint32_t)(wm * WM * 32 + fr) * kStep, wrow = (uint32_t)(BM + wn * WN * 32 + fr) * kStep;
+  const uint32_t xrow = (uint32_t)(wm * 32 + fr) * kStep, wrow = (uint32_t)(BM + wn * WN * 32 + fr) * kStep;
   i32x4 xf[2][WM], wf[2][WN];
-  // fragment v of step kk of stage kt into set f: W's first, X's, W's others, as the products need them
-  auto fragment = [&](int kt, int kk, int f, int v) __attribute__((always_inline)) {
+  // fragment v of step kk of stage kt into set f: W's first, the m of X, W's others, as the products need them
+  auto fragment = [&](int m, int kt, int kk, int f, int v) __attribute__((always_inline)) {
     const uint8_t* s = lds + ring(kt) * STAGE + ((2 * kk + fh) ^ turn) * 16;
-    if (v >= 1 && v <= WM) xf[f][v - 1] = *(const i32x4*)(s + xrow + (v - 1) * 32 * kStep);
-    else wf[f][v == 0 ? 0 : v - WM] = *(const i32x4*)(s + wrow + (v == 0 ? 0 : v - WM) * 32 * kStep);
+    if (v >= 1 && v <= m) xf[f][v - 1] = *(const i32x4*)(s + xrow + (v - 1) * WVM * 32 * kStep);
+    else wf[f][v == 0 ? 0 : v - m] = *(const i32x4*)(s + wrow + (v == 0 ? 0 : v - m) * 32 * kStep);
   };
-  // Grouped: a wave whose rows all lie past the expert's last one only brings its loads.
-  const bool live = !GROUPED || tl.m0 + wm * WM * 32 < tl.m1;
+  // Grouped: the blocks of this wave that hold rows of the expert.  A wave's blocks of 32 rows lie
+  // WVM blocks apart, so a tile of 256 rows that holds 128 or fewer keeps every SIMD half busy:
+  // 512 tokens x 8 over 64 experts, 2816 x 2048, 256 x 256 tiles 102 us; with neighbouring blocks,
+  // and waves that have all their work or none, 112.
+  const int live = GROUPED ? (tl.m1 - tl.m0 - wm * 32 + WVM * 32 - 1) / (WVM * 32) : WM;
   // The products of fragments f, with the fragments (kt, kk) into the other set and loads
-  // u0 .. u0 + n - 1 of stage `dt` between them.
-  auto step = [&](int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
-    if (!live) {
-#pragma unroll
-      for (int d = 0; d < n; ++d)
-        if (dt < a.nk) issue(dt, u0 + d);
-      return;
-    }
+  // u0 .. u0 + n - 1 of stage `dt` between them; of the first m blocks of rows.
+  auto products = [&](auto mc, int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
+    constexpr int m = decltype(mc)::value, nm = m * WN, nf = m + WN;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int q = 0; q < NM; ++q) {
+    for (int q = 0; q < nm; ++q) {
 #pragma unroll
-      for (int v = 0; v < NF; ++v)
-        if (std::max(v * (NM - 2) / NF, 0) == q) fragment(kt, kk, f ^ 1, v);
+      for (int v = 0; v < nf; ++v)
+        if (std::max(v * (nm - 2) / nf, 0) == q) fragment(m, kt, kk, f ^ 1, v);
 #pragma unroll
       for (int d = 0; d < n; ++d)
-        if (std::min(1 + d * (NM - 1) / n, NM - 1) == q && dt < a.nk) issue(dt, u0 + d);
-      const int j = q / WM, i = q % WM;
+        if (std::min(1 + d * (nm - 1) / n, nm - 1) == q && dt < a.nk) issue(dt, u0 + d);
+      const int j = q / m, i = q % m;
       acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[f][j], xf[f][i], acc[j][i], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto step = [&](int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
+    if (live >= WM) return products(std::integral_constant<int, WM>(), f, kt, kk, dt, u0, n);
+    if constexpr (WM == 2)
+      if (live == 1) return products(std::integral_constant<int, 1>(), f, kt, kk, dt, u0, n);
+#pragma unroll
+    for (int d = 0; d < n; ++d)
+      if (dt < a.nk) issue(dt, u0 + d);
   };
   // waits until stage kt has landed, those up to kt + S - 2 being on their way too
   auto landed = [&](int kt) __attribute__((always_inline)) {
@@ -383,7 +389,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     for (int u = 0; u < D0; ++u) issue(S - 1, u);
   }
 #pragma unroll
-  for (int v = 0; v < NF; ++v) fragment(0, 0, 0, v);
+  for (int v = 0; v < NF; ++v) fragment(WM, 0, 0, 0, v);
   for (int kt = 0; kt < a.nk; ++kt) {
     step(0, kt, 1, kt + S - 1, D0, D1);
     step(1, kt, 2, kt + S - 1, D0 + D1, D2);
@@ -405,7 +411,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     const int cw = (wn * WN + j0) * 32, nw = n0 + cw;
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
-      const int rw = (wm * WM + i) * 32, mb = tl.m0 + rw;
+      const int rw = (i * WVM + wm) * 32, mb = tl.m0 + rw;
       if (mb >= tl.m1) break;
       const float s = row_scale[rw + fr];
 #pragma unroll
