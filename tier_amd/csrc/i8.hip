@@ -759,32 +759,70 @@ constexpr TileCost kTiles[] = {
     {256, 192, 2.2f, 6.62f, 9.86f}, {256, 256, 4.6f, 0.18f, 11.6f}, {256, 320, 4.3f, 11.1f, 14.1f},
 };
 
-// The tile for a call.  Grouped, the offsets are on the device: the rows are taken as independent
-// choices of the experts, those with rows each having half a tile to spare.
-int pick_tile(const I8Args& a, bool grouped, int cus) {
-  const float used = grouped ? a.E * (1.f - std::exp(-(float)a.M / a.E)) : 1.f, each = a.M / used;
+int pick_tile(const I8Args& a, int cus) {
   int best = 0;
   float least = 1e30f;
   for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
     const TileCost& c = kTiles[i];
-    const float rows = grouped ? used * std::max(1.f, each / c.bm + 0.5f) : std::ceil(each / c.bm);
-    const float n = std::ceil(rows * ((a.N + c.bn - 1) / c.bn) / cus);
+    const float n = std::ceil(std::ceil((float)a.M / c.bm) * ((a.N + c.bn - 1) / c.bn) / cus);
     const float t = c.t0 + a.nk * (kStep / 1024.f) * std::max(c.one, c.each * n);
     if (t < least) least = t, best = i;
   }
   return best;
 }
 
+// Grouped, a call takes about t0 + max(K / 1024 * each * n, stream * MB of W) us: the experts'
+// weights come from memory, past the last-level cache, and a tile whose rows are few costs large
+// tiles less.  Fitted to 49 sizes (2 to 160 experts, 1 to 1024 rows each, W of 1 to 1300 MB) and to
+// uniform routing: the tile with the least such time is within 2.3 % of the best in the mean, 21 % at
+// worst; with the costs above, 7.6 and 58 %.  Tiles 16 x 32, 32 x 32, 32 x 64 and 128 x 64 were
+// never the best by more than that.  Example, 64 experts of 2816 x 2048, us: 4 rows each 16 x 64 tiles
+// 63, 64 x 64 72, 256 x 256 90; 32 rows 64 x 64 82, 128 x 128 93; 188 rows 256 x 256 130, 128 x 128 181,
+// 64 x 64 240.
+struct GroupedCost {
+  int tile;  // of kTiles
+  float t0, each, stream;
+};
+constexpr GroupedCost kGroupedTiles[] = {
+    {0, 3.7f, 0.62f, 0.24f}, {2, 3.9f, 1.70f, 0.17f}, {5, 4.1f, 2.31f, 0.19f},  {7, 2.5f, 5.97f, 0.23f},
+    {8, 0.1f, 8.71f, 0.23f}, {9, 0.f, 13.0f, 0.25f},  {10, 0.f, 14.9f, 0.26f}, {11, 0.f, 18.3f, 0.27f},
+};
+
+// Tiles of bm rows that an expert of `mean` rows is expected to need where every row chooses by
+// itself, its rows then spread by sqrt(mean) (the normal distribution's tail as a logistic one).
+float tiles_of(float mean, int bm) {
+  const float j = std::floor(mean / bm);
+  auto above = [&](float rows) { return 1.f / (1.f + std::exp(-1.7f * (mean - rows) / std::sqrt(mean))); };
+  return j + (j > 0.f ? above(j * bm) : 1.f) + above((j + 1) * bm);
+}
+
+// The offsets are on the device: the rows are taken as independent choices of the experts.
+int pick_grouped_tile(const I8Args& a, int cus) {
+  const float used = a.E * (1.f - std::exp(-(float)a.M / a.E)), mean = a.M / used;
+  const float mb = used * a.N * a.nk * (kStep * 1e-6f);
+  int best = 0;
+  float least = 1e30f;
+  for (const GroupedCost& c : kGroupedTiles) {
+    const TileCost& z = kTiles[c.tile];
+    const float n = std::ceil(used * tiles_of(mean, z.bm) * ((a.N + z.bn - 1) / z.bn) / cus);
+    const float t = c.t0 + std::max(a.nk * (kStep / 1024.f) * c.each * n, c.stream * mb);
+    if (t < least) least = t, best = c.tile;
+  }
+  return best;
+}
+
 template <int YT, bool GROUPED>
 int launch_picked(int tile, const I8Args& a, hipStream_t s, const char* who) {
+  if constexpr (!GROUPED) switch (tile) {
+      case 1: return launch_tile<YT, 16, 32, 1, 8, 4, 4, false>(a, s, who);
+      case 3: return launch_tile<YT, 32, 32, 1, 8, 4, 4, false>(a, s, who);
+      case 4: return launch_tile<YT, 32, 64, 1, 8, 4, 3, false>(a, s, who);
+      case 6: return launch_gemm<YT, 128, 64, 4, 2, 4, false>(a, s, who);
+    }
   switch (tile) {
     case 0: return launch_tile<YT, 16, 16, 1, 8, 4, 4, GROUPED>(a, s, who);
-    case 1: return launch_tile<YT, 16, 32, 1, 8, 4, 4, GROUPED>(a, s, who);
     case 2: return launch_tile<YT, 16, 64, 2, 2, 2, 4, GROUPED>(a, s, who);
-    case 3: return launch_tile<YT, 32, 32, 1, 8, 4, 4, GROUPED>(a, s, who);
-    case 4: return launch_tile<YT, 32, 64, 1, 8, 4, 3, GROUPED>(a, s, who);
     case 5: return launch_gemm<YT, 64, 64, 2, 2, 4, GROUPED>(a, s, who);
-    case 6: return launch_gemm<YT, 128, 64, 4, 2, 4, GROUPED>(a, s, who);
     case 7: return launch_gemm<YT, 128, 128, 2, 4, 4, GROUPED>(a, s, who);
     case 8: return launch_gemm<YT, 256, 128, 4, 2, 3, GROUPED>(a, s, who);
     case 9: return launch_gemm<YT, 256, 192, 4, 2, 2, GROUPED>(a, s, who);
@@ -796,7 +834,7 @@ int launch_picked(int tile, const I8Args& a, hipStream_t s, const char* who) {
 int gemm(const I8Args& a, int ytype, bool grouped, hipStream_t s, const char* who) {
   int cus = 0, st = device_cus(&cus);
   if (st != TIERMM_OK) return st;
-  const int tile = pick_tile(a, grouped, cus);
+  const int tile = grouped ? pick_grouped_tile(a, cus) : pick_tile(a, cus);
   with_rows(ytype, [&](auto yt) {
     constexpr int YT = decltype(yt)::value;
     st = grouped ? launch_picked<YT, true>(tile, a, s, who) : launch_picked<YT, false>(tile, a, s, who);
