@@ -321,6 +321,28 @@ def test_grouped_many_rows(gpu):
         check(y[off[e]:off[e + 1]], t, q[r], sx[r], w[e * N:(e + 1) * N], sw[e * N:(e + 1) * N])
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,k,E,N,K", [(200, 1, 9, 1010, 130), (500, 1, 9, 3500, 130), (3000, 3, 33, 300, 512),
+                                       (500, 1, 9, 5000, 130), (3000, 3, 33, 1010, 130), (2000, 1, 33, 2050, 130),
+                                       (1100, 2, 3, 1000, 260)])
+def test_grouped_tiles(gpu, t, T, k, E, N, K):
+    """The tiles of 64 to 256 rows, with 20 to 700 rows an expert: wholly, by half of a wave's blocks, by none of them."""
+    ids, P = _routed(T, k, E, T + N, drop=0.1), T * k
+    q = np.random.default_rng(N).integers(-127, 128, (T, K))
+    X, rb = i8_rows(q)
+    sx = np.random.default_rng(T).random(T).astype(np.float32)
+    w, sw, W, rbw = weight(E * N, K, 13)
+    OF, TP, SP, Y = i32(np.zeros(E + 1)), i32(np.zeros(P)), i32(np.zeros(P)), Rows(t, P, N)
+    tier_amd.moe_plan(i32(ids).ptr, T, k, E, OF.ptr, TP.ptr, SP.ptr)
+    tier_amd.i8_gemm_grouped(X.ptr, rb, f32(sx).ptr, SP.ptr, T, k, OF.ptr, E, W.ptr, rbw, f32(sw).ptr, Y.ptr, t, N, P, N, K)
+    hip.synchronize()
+    off, srt, y = OF.download(np.int32), SP.download(np.int32), Y.values()
+    for e in range(E):
+        r = srt[off[e]:off[e + 1]] // k
+        check(y[off[e]:off[e + 1]], t, q[r], sx[r], w[e * N:(e + 1) * N], sw[e * N:(e + 1) * N])
+    assert not y[off[E]:].any()
+
+
 @pytest.mark.parametrize("M", [1, 6, 50, 300])
 def test_in_a_graph(gpu, M):
     """A captured linear on a stream of its own replays on new inputs as the eager call."""

@@ -771,21 +771,21 @@ int pick_tile(const I8Args& a, int cus) {
   return best;
 }
 
-// Grouped, a call takes about t0 + max(K / 1024 * each * n, stream * MB of W) us: the experts'
-// weights come from memory, past the last-level cache, and a tile whose rows are few costs large
-// tiles less.  Fitted to 49 sizes (2 to 160 experts, 1 to 1024 rows each, W of 1 to 1300 MB) and to
-// uniform routing: the tile with the least such time is within 2.3 % of the best in the mean, 21 % at
-// worst; with the costs above, 7.6 and 58 %.  Tiles 16 x 32, 32 x 32, 32 x 64 and 128 x 64 were
-// never the best by more than that.  Example, 64 experts of 2816 x 2048, us: 4 rows each 16 x 64 tiles
-// 63, 64 x 64 72, 256 x 256 90; 32 rows 64 x 64 82, 128 x 128 93; 188 rows 256 x 256 130, 128 x 128 181,
-// 64 x 64 240.
+// Grouped, a call takes about max(n * (fix + K / 1024 * each), stream * MB of W) us and the launch: the
+// experts' weights come from memory, past the last-level cache, and a tile costs the MFMAs of its
+// filled blocks and, around its K loop, `fix`.  Fitted to 60 sizes (1 to 160 experts, 1 to 1300 rows
+// each, K of 130 to 14336, W of 0.1 to 1300 MB) and to uniform routing: the tile with the least such
+// time is within 1.7 % of the best in the mean, 21 % at worst; with the costs above, 8 and 58 %.
+// The other tiles were hardly ever the best here.  Example, 64 experts of 2816 x 2048, us:
+// 4 rows each 16 x 64 tiles 63, 64 x 64 72, 256 x 256 90; 32 rows 64 x 64 82, 128 x 128 93; 188 rows
+// 256 x 256 130, 128 x 128 181, 64 x 64 240.
 struct GroupedCost {
   int tile;  // of kTiles
-  float t0, each, stream;
+  float fix, each, stream;
 };
 constexpr GroupedCost kGroupedTiles[] = {
-    {0, 3.7f, 0.62f, 0.24f}, {2, 3.9f, 1.70f, 0.17f}, {5, 4.1f, 2.31f, 0.19f},  {7, 2.5f, 5.97f, 0.23f},
-    {8, 0.1f, 8.71f, 0.23f}, {9, 0.f, 13.0f, 0.25f},  {10, 0.f, 14.9f, 0.26f}, {11, 0.f, 18.3f, 0.27f},
+    {0, 0.85f, 0.52f, 0.23f}, {2, 1.15f, 1.35f, 0.175f}, {5, 1.1f, 1.88f, 0.18f},  {7, 2.5f, 5.2f, 0.20f},
+    {8, 4.0f, 6.6f, 0.22f},   {9, 2.9f, 10.7f, 0.23f},   {10, 3.7f, 12.1f, 0.235f}, {11, 4.3f, 14.3f, 0.28f},
 };
 
 // Tiles of bm rows that an expert of `mean` rows is expected to need where every row chooses by
@@ -805,7 +805,7 @@ int pick_grouped_tile(const I8Args& a, int cus) {
   for (const GroupedCost& c : kGroupedTiles) {
     const TileCost& z = kTiles[c.tile];
     const float n = std::ceil(used * tiles_of(mean, z.bm) * ((a.N + z.bn - 1) / z.bn) / cus);
-    const float t = c.t0 + std::max(a.nk * (kStep / 1024.f) * c.each * n, c.stream * mb);
+    const float t = std::max(n * (c.fix + a.nk * (kStep / 1024.f) * c.each), c.stream * mb);
     if (t < least) least = t, best = c.tile;
   }
   return best;
