@@ -282,7 +282,8 @@ template <int YT, int BM, int BN, int WVM, int WVN, int S, bool GROUPED>
 __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, NF = WM + WN;
   constexpr int STAGE = (BM + BN) * kStep, INST = STAGE / 1024 / NW;
-  static_assert(WM <= 2 && WM * WVM * 32 == BM && WN * WVN * 32 == BN && INST * NW * 1024 == STAGE, "whole blocks and loads a wave");
+  static_assert(WM * WVM * 32 == BM && WN * WVN * 32 == BN && INST * NW * 1024 == STAGE, "whole blocks and loads a wave");
+  static_assert(WM <= 2, "row blocks that step() tells apart");
   // loads of a stage by the step that issues them: 3 (of the stage before last), 0 and 1
   constexpr int D0 = (INST + 2) / 3, D1 = (INST - D0 + 1) / 2, D2 = INST - D0 - D1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -339,7 +340,8 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   const int wm = wave % WVM, wn = wave / WVM, fr = lane & 31, fh = lane >> 5, turn = (fr >> 1) & 7;
   const uint32_t xrow = (uint32_t)(wm * 32 + fr) * kStep, wrow = (uint32_t)(BM + wn * WN * 32 + fr) * kStep;
   i32x4 xf[2][WM], wf[2][WN];
-  // fragment v of step kk of stage kt into set f: W's first, the m of X, W's others, as the products need them
+  // fragment v of step kk of stage kt into set f: W's first, the m of X, W's others, as the
+  // products need them
   auto fragment = [&](int m, int kt, int kk, int f, int v) __attribute__((always_inline)) {
     const uint8_t* s = lds + ring(kt) * STAGE + ((2 * kk + fh) ^ turn) * 16;
     if (v >= 1 && v <= m) xf[f][v - 1] = *(const i32x4*)(s + xrow + (v - 1) * WVM * 32 * kStep);

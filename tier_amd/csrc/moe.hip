@@ -9,7 +9,7 @@
 // top 8 of 64, rows of 2048, between buffers that the caches do not hold (a large copy moves
 // 5.1 TB/s): sort 53 us fp32 (5.7 TB/s), 27 us bf16; its gradient 54 and 27; the weighted sum's
 // 27.5 in bf16 (5.5); that one's gradient 115 and 62 (4.7-4.9, the same bytes read as written).
-// Eight tokens: 2.4 to 3.6 us replayed from a graph, 3.2 to 3.7 launched one by one.
+// Eight tokens: 2.2 to 2.6 us replayed from a graph, 3.0 to 3.4 launched one by one.
 #include "tm_rows.h"
 
 namespace tiermm {
