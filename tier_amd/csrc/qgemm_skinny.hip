@@ -249,11 +249,16 @@ __device__ __forceinline__ h2v as_h2(uint32_t v) { return __builtin_bit_cast(h2v
 __device__ __forceinline__ uint32_t as_u(h2v v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ h2v dup(float f) { return h2v{(_Float16)f, (_Float16)f}; }
 // Codes are read as fp16 subnormals: the 8-bit code c in a 16-bit lane is c * 2^-24, with no
-// conversion.  A pair of x-ref weights fp16(fma(s, code, m)) from such a pair and s * 2^24: one
-// v_fma_mixlo / _mixhi each (fp32 fma, then rounded to fp16).
+// conversion.  A pair of x-ref weights fp16(fma(s, code, m)) from such a pair and s * 2^24: two
+// v_fma_mix_f32 and one v_cvt_pk_f16_f32.  The empty asm keeps the fp32 values: v_fma_mixlo / _mixhi
+// round the exact sum to fp16 at once, one fp16 step away from fp32-then-fp16 where fp32 lands on a
+// tie (q4_K and q5_K, a weight in about a million), and took longer (q4_K 8 x 14336 x 5120 24.4 -> 22.9 us,
+// 64 experts of one row 68.6 -> 58.4).
 __device__ __forceinline__ uint32_t mix2(uint32_t codes, float s24, float m) {
   const h2v c = as_h2(codes);
-  return as_u(h2v{(_Float16)fmaf((float)c[0], s24, m), (_Float16)fmaf((float)c[1], s24, m)});
+  float a = fmaf((float)c[0], s24, m), b = fmaf((float)c[1], s24, m);
+  asm("" : "+v"(a), "+v"(b));
+  return as_u(h2v{(_Float16)a, (_Float16)b});
 }
 // The same for the four codes of v's bytes in element order
 __device__ __forceinline__ void mix4(uint32_t v, float s24, float m, uint32_t& o0, uint32_t& o1) {
