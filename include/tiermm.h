@@ -318,7 +318,8 @@ size_t tiermm_qgemm_grouped_ws_bytes(const int* qtype_e, const int* expert_offse
                                      int N, int K, int mode);
 /* Per-token weighted combine of the routed outputs: out[t][n] =
  * sum_{j<topk} pair_weight[p] * Y_sorted[p][n], p = token_pairs[t*topk + j],
- * summed in j order.  token_pairs, pair_weight: device arrays. */
+ * summed in j order.  token_pairs, pair_weight: device arrays.  A negative p is a
+ * dropped pair, as tiermm_moe_plan writes it: nothing is read for it. */
 int tiermm_moe_combine(const float* Y_sorted, const int* token_pairs, const float* pair_weight,
                        float* out, int T, int topk, int N, tiermm_stream_t stream);
 

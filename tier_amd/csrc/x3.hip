@@ -331,7 +331,8 @@ __global__ __launch_bounds__(256) void dense_pad_kernel(const uint8_t* __restric
 }
 
 // Weighted combine of routed expert outputs: out[t][n] = sum_j w[p_j] * Y[p_j][n],
-// p_j = token_pairs[t*topk + j], summed in j order (deterministic).
+// p_j = token_pairs[t*topk + j], summed in j order (deterministic).  A negative p_j is a
+// dropped pair (tiermm_moe_plan): it has no row and no weight, and neither is read.
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ Y, const int* __restrict__ tp,
                                                           const float* __restrict__ pw, float* __restrict__ out,
                                                           int topk, int N) {
@@ -340,13 +341,13 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
     float acc = 0.f;
     for (int j = 0; j < topk; ++j) {
       const int p = tp[(size_t)t * topk + j];
-      acc = fmaf(pw[p], Y[(size_t)p * N + n], acc);
+      if (p >= 0) acc = fmaf(pw[p], Y[(size_t)p * N + n], acc);
     }
     out[(size_t)t * N + n] = acc;
   }
 }
 // The same, four columns a thread (N a multiple of 4, Y and out 16-byte aligned, topk
-// at most 16): the token's pairs and weights are read once, then 16-byte loads of
+// 1 to 16): the token's pairs and weights are read once, then 16-byte loads of
 // each pair's row; each column is summed in the same j order.
 __global__ __launch_bounds__(256) void moe_combine4_kernel(const float* __restrict__ Y, const int* __restrict__ tp,
                                                            const float* __restrict__ pw, float* __restrict__ out,
@@ -354,25 +355,33 @@ __global__ __launch_bounds__(256) void moe_combine4_kernel(const float* __restri
   const int t = blockIdx.x;
   int pj[16];
   float wj[16];
+  int least = 0;  // of the pairs' places
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (j < topk) {
-      pj[j] = tp[(size_t)t * topk + j];
-      wj[j] = pw[pj[j]];
-    }
-  for (int n = 4 * threadIdx.x; n < N; n += 1024) {
-    float4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < 16; ++j) pj[j] = tp[(size_t)t * topk + min(j, topk - 1)];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) least = min(least, pj[j]);
+  // tokens without dropped pairs load weights and rows without a branch between them
+  auto sum = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (j < topk) {
-        const float4 y = *(const float4*)(Y + (size_t)pj[j] * N + n);
-        acc.x = fmaf(wj[j], y.x, acc.x);
-        acc.y = fmaf(wj[j], y.y, acc.y);
-        acc.z = fmaf(wj[j], y.z, acc.z);
-        acc.w = fmaf(wj[j], y.w, acc.w);
-      }
-    *(float4*)(out + (size_t)t * N + n) = acc;
-  }
+      if (WHOLE || pj[j] >= 0) wj[j] = pw[pj[j]];
+    for (int n = 4 * threadIdx.x; n < N; n += 1024) {
+      float4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < topk && (WHOLE || pj[j] >= 0)) {
+          const float4 y = *(const float4*)(Y + (size_t)pj[j] * N + n);
+          acc.x = fmaf(wj[j], y.x, acc.x);
+          acc.y = fmaf(wj[j], y.y, acc.y);
+          acc.z = fmaf(wj[j], y.z, acc.z);
+          acc.w = fmaf(wj[j], y.w, acc.w);
+        }
+      *(float4*)(out + (size_t)t * N + n) = acc;
+    }
+  };
+  if (least >= 0) sum(std::true_type());
+  else sum(std::false_type());
 }
 
 // ------------------------------------------------------------- GEMM core
@@ -1916,7 +1925,7 @@ int tiermm_moe_combine(const float* Y_sorted, const int* token_pairs, const floa
   if (T < 0 || topk < 0 || N < 0) return set_error(TIERMM_EINVAL, "tiermm_moe_combine: negative size");
   if (T == 0 || N == 0) return TIERMM_OK;
   if (!Y_sorted || !token_pairs || !pair_weight || !out) return set_error(TIERMM_EINVAL, "tiermm_moe_combine: null buffer");
-  if (N % 4 == 0 && topk <= 16 && ((uintptr_t)Y_sorted & 15) == 0 && ((uintptr_t)out & 15) == 0)
+  if (N % 4 == 0 && topk >= 1 && topk <= 16 && ((uintptr_t)Y_sorted & 15) == 0 && ((uintptr_t)out & 15) == 0)
     moe_combine4_kernel<<<T, 256, 0, (hipStream_t)stream>>>(Y_sorted, token_pairs, pair_weight, out, topk, N);
   else
     moe_combine_kernel<<<T, 256, 0, (hipStream_t)stream>>>(Y_sorted, token_pairs, pair_weight, out, topk, N);
