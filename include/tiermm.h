@@ -401,8 +401,9 @@ size_t tiermm_i8_linear_ws_bytes(int M, int N, int K);
  * weight W + e * N * rbw with the scales sw[e][N].  rows = tiermm_moe_plan's
  * sorted_pairs: the tokens are quantized once and gathered here, without a sorted copy;
  * NULL: row p of Xq.  expert_offsets and rows are DEVICE arrays, read by the kernel: no
- * host copy, and a captured graph follows new routings.  Rows of no expert, and rows
- * whose index points nowhere, become zeros. */
+ * host copy, and a captured graph follows new routings.  Rows of no expert (in front of
+ * the first offset, as where a plan's experts e0 .. are run from expert_offsets + e0, or
+ * from the last one up), and rows whose index points nowhere, become zeros. */
 int tiermm_i8_gemm_grouped(const int8_t* Xq, size_t rbx, const float* sx, const int32_t* rows, int n_rows, int topk,
                            const int32_t* expert_offsets, int n_experts, const int8_t* W, size_t rbw, const float* sw,
                            void* Y, int ytype, size_t ldy, int P, int N, int K, tiermm_stream_t stream);

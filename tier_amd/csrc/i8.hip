@@ -156,10 +156,11 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
   const int lane = threadIdx.x & 63, P = a.M, i = bid >> 3;
   const int t = ((i / a.share) * 8 + (bid & 7)) * a.share + i % a.share;
   int run = 0;
-  for (int e0 = 0; e0 <= a.E; e0 += 64) {
-    // rows of expert e (E: those from off[E] to P), whatever the offsets hold within [0, P]
-    const int e = e0 + lane, b = e <= a.E ? min(max(a.off[e], 0), P) : P;
-    const int end = e < a.E ? min(max(a.off[e + 1], 0), P) : P;
+  for (int e0 = 0; e0 <= a.E + 1; e0 += 64) {
+    // rows of expert e (E: those from off[E] to P, E + 1: those in front of off[0]), whatever the
+    // offsets hold within [0, P]
+    const int e = e0 + lane, b = e <= a.E ? min(max(a.off[e], 0), P) : e == a.E + 1 ? 0 : P;
+    const int end = e == a.E || e > a.E + 1 ? P : min(max(a.off[e < a.E ? e + 1 : 0], 0), P);
     const int rows = max(end - b, 0), n = (rows + BM - 1) / BM * ntn;
     int s = n;
 #pragma unroll
@@ -172,7 +173,7 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
       const int l = __ffsll((unsigned long long)hit) - 1;
       const int r0 = __shfl(b, l, 64), nr = __shfl(rows, l, 64), t0 = run + __shfl(s - n, l, 64);
       const int ntm = (nr + BM - 1) / BM, in = t - t0;
-      tl.e = e0 + l;
+      tl.e = min(e0 + l, a.E);
       tl.tn = in / ntm;
       tl.m0 = r0 + (in % ntm) * BM;
       tl.m1 = min(tl.m0 + BM, r0 + nr);
@@ -443,14 +444,15 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   if constexpr (WN % JB) store(std::integral_constant<int, WN % JB>(), WN - WN % JB);
 }
 
-// Launches fn over the tiles; grouped, every expert may end in a partly filled one.
+// Launches fn over the tiles; grouped, every expert, and the rows in front of the first and behind
+// the last, may end in a partly filled one.
 template <class Fn>
 int launch(Fn* fn, std::atomic<uint64_t>& done, I8Args a, bool grouped, int bm, int bn, int threads, int lds,
            hipStream_t s, const char* who) {
   const int st = lds_attr_once(done, (const void*)fn, lds, who);
   if (st != TIERMM_OK) return st;
   const long long ntn = (a.N + bn - 1) / bn;
-  const long long ntm = grouped ? a.M / bm + std::min(a.E, a.M) + 1 : (a.M + bm - 1) / bm;
+  const long long ntm = grouped ? a.M / bm + std::min(a.E + 2, a.M) : (a.M + bm - 1) / bm;
   a.share = (int)std::min(32ll, (ntm * ntn + 7) / 8);
   const long long step = grouped ? 8ll * a.share : 8, grid = (ntm * ntn + step - 1) / step * step;
   if (grid > (1ll << 22)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, ntm * ntn);
