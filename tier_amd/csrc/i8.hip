@@ -137,7 +137,7 @@ struct I8Args {
 // What a workgroup computes: rows [m0, m1) of Y, column tile tn.
 struct Tile {
   int m0, m1, tn;
-  int e;      // expert; E: rows that no expert has, which become zeros
+  int e;      // expert; E: rows that no expert has, which become zeros (zero_tile)
   bool once;  // no other tile reads these rows of W
 };
 
@@ -156,11 +156,10 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
   const int lane = threadIdx.x & 63, P = a.M, i = bid >> 3;
   const int t = ((i / a.share) * 8 + (bid & 7)) * a.share + i % a.share;
   int run = 0;
-  for (int e0 = 0; e0 <= a.E + 1; e0 += 64) {
-    // rows of expert e (E: those from off[E] to P, E + 1: those in front of off[0]), whatever the
-    // offsets hold within [0, P]
-    const int e = e0 + lane, b = e <= a.E ? min(max(a.off[e], 0), P) : e == a.E + 1 ? 0 : P;
-    const int end = e == a.E || e > a.E + 1 ? P : min(max(a.off[e < a.E ? e + 1 : 0], 0), P);
+  for (int e0 = 0; e0 <= a.E; e0 += 64) {
+    // rows of expert e (E: those from off[E] to P), whatever the offsets hold within [0, P]
+    const int e = e0 + lane, b = e <= a.E ? min(max(a.off[e], 0), P) : P;
+    const int end = e < a.E ? min(max(a.off[e + 1], 0), P) : P;
     const int rows = max(end - b, 0), n = (rows + BM - 1) / BM * ntn;
     int s = n;
 #pragma unroll
@@ -173,7 +172,7 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
       const int l = __ffsll((unsigned long long)hit) - 1;
       const int r0 = __shfl(b, l, 64), nr = __shfl(rows, l, 64), t0 = run + __shfl(s - n, l, 64);
       const int ntm = (nr + BM - 1) / BM, in = t - t0;
-      tl.e = min(e0 + l, a.E);
+      tl.e = e0 + l;
       tl.tn = in / ntm;
       tl.m0 = r0 + (in % ntm) * BM;
       tl.m1 = min(tl.m0 + BM, r0 + nr);
@@ -182,7 +181,15 @@ __device__ __forceinline__ bool grouped_tile(const I8Args& a, int ntn, int bid, 
     }
     run += __shfl(s, 63, 64);
   }
-  return false;
+  // rows in front of off[0], counted from P (zero_tile)
+  const int lead = min(max(a.off[0], 0), P), ntm = (lead + BM - 1) / BM, in = t - run;
+  if (in >= ntm * ntn) return false;
+  tl.e = a.E;
+  tl.tn = in / ntm;
+  tl.m0 = P + (in % ntm) * BM;
+  tl.m1 = min(tl.m0 + BM, P + lead);
+  tl.once = false;
+  return true;
 }
 
 // The tile of this workgroup; false past the last.  Dense tiles go in groups of 4 tile rows,
@@ -221,13 +228,16 @@ __device__ __forceinline__ const uint8_t* stage_row(const I8Args& a, const Tile&
   return W + (size_t)min(n0 + r - BM, a.N - 1) * a.rbw;
 }
 
-// Columns n0 .. n0 + BN - 1 of the tile's rows become zeros.
+// Columns n0 .. n0 + BN - 1 of rows that no expert has become zeros: rows [m0, m1), those from P up
+// being the ones in front of off[0].
 template <class Y, int BN, int THREADS>
 __device__ __forceinline__ void zero_tile(const I8Args& a, const Tile& tl, int n0) {
   const int cols = min(BN, a.N - n0);
-  for (int m = tl.m0; m < tl.m1; ++m)
+  for (int i = tl.m0; i < tl.m1; ++i) {
+    const int m = i < a.M ? i : i - a.M;
     for (int c = threadIdx.x * Y::EPU; c < cols; c += THREADS * Y::EPU)
       Y::set(a.Y + (size_t)m * a.ldy + (size_t)n0 * Y::ES, c, cols, u32x4{0u, 0u, 0u, 0u});
+  }
 }
 
 // One element of Y: the sum rounded to fp32, times sx * sw, plus the bias (0: none).
