@@ -5,8 +5,8 @@ import numpy as np
 import pytest
 
 import tier_amd
-from rows import TYPES, Rows, f32, i32
-from test_gpu_i8 import _routed, check, i8_rows, weight
+from rows import TINY, TYPES, UNIT, Rows, f32, i32
+from test_gpu_i8 import _routed, check, i8_rows, quantize, weight
 from tier_amd import hip
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,72 @@ def test_grouped_without_rows_of_its_experts(gpu):
                                  f32(sw).ptr, Y.ptr, t, N, P, N, K)
         hip.synchronize()
         assert not Y.values().any()
+
+
+# rows of x: the GEMV, the small tiles, 64 x 64, 128 x 128 and 256-row tiles
+ROWS = [(1, 300, 640), (2, 300, 640), (6, 1003, 260), (50, 2501, 260), (50, 5101, 2600), (130, 20001, 130),
+        (2051, 2001, 130)]
+
+
+@pytest.mark.parametrize("t", [tier_amd.F32, tier_amd.BF16])
+@pytest.mark.parametrize("M,N,K", ROWS)
+def test_scales_at_the_ends_of_fp32(gpu, t, M, N, K):
+    """sx * sw below the normal numbers or past the largest one, while the element is not: within the
+    same bound, and a sum of 0 gives the bias.  Elements that are too large themselves are infinite."""
+    rng = np.random.default_rng(M + N)
+    q = rng.integers(-127, 128, (M, K))
+    if M > 2:
+        q[M // 2] = 0
+    sx = np.float32([2.0 ** -120, 2.0 ** 100, 1, 2.0 ** -149, 3 * 2.0 ** -130, 2.0 ** 120, 2.0 ** -64])[rng.permutation(M) % 7]
+    w, _, W, rbw = weight(N, K, M + N)
+    sw = np.float32([2.0 ** -11, 2.0 ** 20, 2.0 ** -60, 2.0 ** 110, 2.0 ** -126, 3, 2.0 ** 63])[rng.permutation(N) % 7]
+    sw *= rng.choice(np.float32([-1, 1]), N)
+    bias = np.where(rng.random(N) < 0.5, 0, rng.standard_normal(N)).astype(np.float32)
+    X, rbx = i8_rows(q)
+    Y = Rows(t, M, N)
+    tier_amd.i8_gemm(X.ptr, rbx, f32(sx).ptr, W.ptr, rbw, f32(sw).ptr, f32(bias).ptr, Y.ptr, t, N, M, N, K)
+    hip.synchronize()
+    y = Y.values()
+    s = (q.astype(np.float64) @ w.T.astype(np.float64)) * sx.astype(np.float64)[:, None] * sw.astype(np.float64)
+    top = 2.0 ** 128 * (1 - 2.0 ** -7)  # (bf16 and roundings at the very end are left out)
+    large, fits = np.abs(s) >= 2.0 ** 128 * (1 + 2.0 ** -20), np.abs(s) < top
+    assert np.array_equal(y[large], np.where(s > 0, np.inf, -np.inf)[large])
+    err = 4 * 2.0 ** -24 * (np.abs(s) + np.abs(bias))
+    unit, tiny = UNIT[t], TINY[tier_amd.F32] + TINY[t]
+    ok = np.abs(y - (s + bias)) <= err + unit * (np.abs(s + bias) + err) + tiny
+    assert ok[fits].all(), np.argwhere(~ok & fits)[:5]
+    if M > 2:
+        assert not s[M // 2].any() and large.any() and (np.abs(s[s != 0]) < 2.0 ** -126).any()
+
+
+@pytest.mark.parametrize("M", [1, 2, 5, 40, 150])
+@pytest.mark.parametrize("down", [100, 120, 130])
+def test_linear_of_tiny_rows(gpu, M, down):
+    """Rows of x of 2^-down times normal numbers: products of their codes to the same bound."""
+    t, N, K = tier_amd.F32, 200, 700
+    x = np.random.default_rng(M).standard_normal((M, K)).astype(np.float32) * np.float32(2.0 ** -down)
+    w, sw, W, rbw = weight(N, K, 4)
+    sw *= np.float32(2.0 ** 10)
+    X, Y = Rows(t, M, K, x), Rows(t, M, N)
+    tier_amd.i8_linear(X.ptr, t, K, W.ptr, rbw, f32(sw).ptr, None, Y.ptr, t, N, M, N, K)
+    hip.synchronize()
+    q, sx = quantize(x)
+    check(Y.values(), t, q, sx, w, sw)
+
+
+def test_grouped_scales_at_the_ends_of_fp32(gpu):
+    """The same of the experts' products, where one token's scale is tiny."""
+    t, T, k, E, N, K = tier_amd.F32, 600, 2, 3, 520, 260
+    q = np.random.default_rng(1).integers(-127, 128, (T, K))
+    X, rb = i8_rows(q)
+    sx = np.float32([1, 2.0 ** -125, 2.0 ** 70])[np.arange(T) % 3]
+    w, sw, W, rbw = weight(E * N, K, 3)
+    P = T * k
+    OF, TP, SP, Y = i32(np.zeros(E + 1)), i32(np.zeros(P)), i32(np.zeros(P)), Rows(t, P, N)
+    tier_amd.moe_plan(i32(_routed(T, k, E, 5)).ptr, T, k, E, OF.ptr, TP.ptr, SP.ptr)
+    tier_amd.i8_gemm_grouped(X.ptr, rb, f32(sx).ptr, SP.ptr, T, k, OF.ptr, E, W.ptr, rbw, f32(sw).ptr, Y.ptr, t, N, P, N, K)
+    hip.synchronize()
+    off, srt, y = OF.download(np.int32), SP.download(np.int32), Y.values()
+    for e in range(E):
+        r = srt[off[e]:off[e + 1]] // k
+        check(y[off[e]:off[e + 1]], t, q[r], sx[r], w[e * N:(e + 1) * N], sw[e * N:(e + 1) * N])

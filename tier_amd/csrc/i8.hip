@@ -240,10 +240,29 @@ __device__ __forceinline__ void zero_tile(const I8Args& a, const Tile& tl, int n
   }
 }
 
-// One element of Y: the sum rounded to fp32, times sx * sw, plus the bias (0: none).
+// One element of Y: the sum rounded to fp32, times sx * sw, plus the bias (0: none).  Where sx * sw
+// is not a normal fp32 number the sum takes the smaller scale first: a product of a whole number that
+// falls below the normal numbers is exact, and it overflows only if the element does.
+__device__ __forceinline__ bool normal(float v) { return __builtin_amdgcn_classf(v, 0x108); }
 __device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias) {
+  const float s = sx * sw;
+  if (__builtin_expect(normal(s), 1)) return fmaf((float)sum, s, bias);
+  const bool x_first = fabsf(sx) < fabsf(sw);  // (NaN: stays in the second product)
+  return fmaf((float)sum * (x_first ? sx : sw), x_first ? sw : sx, bias);
+}
+// The same, bit for bit, for scales of which neither is far: their products are normal, 0 or NaN.
+__device__ __forceinline__ float scaled_near(int sum, float sx, float sw, float bias) {
   return fmaf((float)sum, sx * sw, bias);
 }
+// Scales are far where one is not 0 and below 2^-63, or from 2^63 up.
+struct ScaleRange {
+  float least = 1.f, most = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    least = fminf(least, v == 0.f ? 1.f : fabsf(v));
+    most = fmaxf(most, fabsf(v));
+  }
+  __device__ __forceinline__ bool far() const { return least < 0x1p-63f || most >= 0x1p63f; }
+};
 
 // Waits until no more than n (at most N) stages of INST loads are on their way.
 template <int N, int INST>
@@ -403,6 +422,13 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   }
 #pragma unroll
   for (int v = 0; v < NF; ++v) fragment(WM, 0, 0, 0, v);
+  // whether a scale of this wave's elements is far, for the end
+  ScaleRange range;
+#pragma unroll
+  for (int i = 0; i < WM; ++i) range.add(row_scale[(i * WVM + wm) * 32 + fr]);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) range.add(col_scale[(wn * WN + j) * 32 + fr]);
+  const bool wave_far = __ballot(range.far()) != 0;
   for (int kt = 0; kt < a.nk; ++kt) {
     step(0, kt, 1, kt + S - 1, D0, D1);
     step(1, kt, 2, kt + S - 1, D0 + D1, D2);
@@ -419,7 +445,8 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   constexpr int JB = Y::ES == 2 ? 2 : 1, PART = 4096;
   static_assert(NW * PART <= S * STAGE, "rows of the epilogue in LDS");
   uint8_t* part = lds + wave * PART;
-  auto store = [&](auto jn, int j0) __attribute__((always_inline)) {
+  auto store = [&](auto far_scales, auto jn, int j0) __attribute__((always_inline)) {
+    constexpr bool FAR = decltype(far_scales)::value;
     constexpr int J = decltype(jn)::value, CH = J * 32 * Y::ES / 16;
     const int cw = (wn * WN + j0) * 32, nw = n0 + cw;
 #pragma unroll
@@ -435,7 +462,10 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
           const f32x4 cs = *(const f32x4*)(col_scale + cw + c), cb = *(const f32x4*)(col_bias + cw + c);
           f32x4 v;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = scaled(acc[j0 + j][i][4 * b + k], s, cs[k], cb[k]);
+          for (int k = 0; k < 4; ++k) {
+            const int sum = acc[j0 + j][i][4 * b + k];
+            v[k] = FAR ? scaled(sum, s, cs[k], cb[k]) : scaled_near(sum, s, cs[k], cb[k]);
+          }
           Y::set4(part + out_place<CH>(fr, c * Y::ES), v);
         }
       wave_lds_wait();
@@ -448,10 +478,14 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
       wave_lds_wait();
     }
   };
-  __syncthreads();  // every wave has read its last stage
+  auto store_all = [&](auto far_scales) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j0 = 0; j0 + JB <= WN; j0 += JB) store(std::integral_constant<int, JB>(), j0);
-  if constexpr (WN % JB) store(std::integral_constant<int, WN % JB>(), WN - WN % JB);
+    for (int j0 = 0; j0 + JB <= WN; j0 += JB) store(far_scales, std::integral_constant<int, JB>(), j0);
+    if constexpr (WN % JB) store(far_scales, std::integral_constant<int, WN % JB>(), WN - WN % JB);
+  };
+  __syncthreads();  // every wave has read its last stage
+  if (__builtin_expect(wave_far, 0)) return store_all(std::true_type());
+  store_all(std::false_type());
 }
 
 // Launches fn over the tiles; grouped, every expert, and the rows in front of the first and behind
@@ -599,6 +633,11 @@ __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
   }
   __syncthreads();
 
+  // this lane's channel.  Two rows a wave ask for its scale while W comes (1 x 14336 x 5120 13.4 -> 13.3
+  // us); with one, asking at the end was faster (1 x 1024 x 5120 4.15 us against 4.26).
+  const int n = n0 + (lane >> 4) * R / 4;
+  const bool stores = (lane & 15) == 0 && lane % (64 / R) == 0 && n < a.N;
+  const float early_s = R > 1 && stores ? a.sw[n] : 0.f, early_b = R > 1 && stores && a.bias ? a.bias[n] : 0.f;
   int acc[MX][R] = {};
   for (int c0 = 0; c0 < nc; c0 += U)
 #pragma unroll
@@ -617,12 +656,12 @@ __global__ __launch_bounds__(64 * NW) void i8_gemv_kernel(const I8Args a) {
       if (c + U < nc) load(u, c + U);
     }
   using Y = Rows<YT>;
-  const int n = n0 + (lane >> 4) * R / 4;
 #pragma unroll
   for (int m = 0; m < MX; ++m) {
     const int sum = wave_sums<R>(acc[m]);
-    if (m < a.M && (lane & 15) == 0 && lane % (64 / R) == 0 && n < a.N) {
-      const float v[4] = {scaled(sum, row_scale[m], a.sw[n], a.bias ? a.bias[n] : 0.f), 0.f, 0.f, 0.f};
+    if (m < a.M && stores) {
+      const float cs = R > 1 ? early_s : a.sw[n], cb = R > 1 ? early_b : a.bias ? a.bias[n] : 0.f;
+      const float v[4] = {scaled(sum, row_scale[m], cs, cb), 0.f, 0.f, 0.f};
       Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, v, 1);
     }
   }
@@ -735,11 +774,19 @@ __global__ __launch_bounds__(64 * WVN * WVK) void i8_tile_kernel(const I8Args a)
     for (int w = 1; w < WVK; ++w) v += *(const i32x4*)(sums + (w * BM + r) * LDO + c);
     const int xr = source_row<GROUPED>(a, m);
     const float sc = xr < 0 ? 0.f : a.sx[xr];
-    float o[4];
+    float o[4], cs[4], cb[4];
+    bool near = true;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int nn = min(n + k, a.N - 1);
-      o[k] = scaled(v[k], sc, sw[nn], a.bias ? a.bias[nn] : 0.f);
+      cs[k] = sw[nn];
+      cb[k] = a.bias ? a.bias[nn] : 0.f;
+      o[k] = scaled_near(v[k], sc, cs[k], cb[k]);
+      near &= normal(sc * cs[k]);
+    }
+    if (__builtin_expect(!near, 0)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = scaled(v[k], sc, cs[k], cb[k]);
     }
     Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, min(4, a.N - n));
   }
