@@ -119,3 +119,42 @@ def test_grouped_scales_at_the_ends_of_fp32(gpu):
     for e in range(E):
         r = srt[off[e]:off[e + 1]] // k
         check(y[off[e]:off[e + 1]], t, q[r], sx[r], w[e * N:(e + 1) * N], sw[e * N:(e + 1) * N])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("P,E,N,K", [(9, 3, 70, 130), (40, 3, 1010, 130), (500, 9, 3500, 130), (3000, 33, 300, 512),
+                                     (2200, 3, 1000, 260)])
+def test_rows_that_point_nowhere(gpu, t, P, E, N, K):
+    """Indices below 0 and past the rows of x: zeros, also in channels whose scale is NaN or infinite,
+    where every other row is not finite."""
+    rng = np.random.default_rng(P)
+    T, topk = P // 2 + 1, 2
+    q = rng.integers(1, 128, (T, K))
+    X, rb = i8_rows(q)
+    w, sw, W, rbw = weight(E * N, K, 2)
+    w = np.abs(w) + (w == 0)  # sums above 0
+    W, rbw = i8_rows(w)
+    bad = rng.random(E * N) < 0.02
+    bad[::N] = True
+    sw[bad] = rng.choice(np.float32([np.nan, np.inf, -np.inf]), bad.sum())
+    rows = rng.integers(0, T * topk, P).astype(np.int32)
+    rows[rng.random(P) < 0.2] = -1
+    rows[rng.random(P) < 0.1] = T * topk
+    rows[:2] = [np.iinfo(np.int32).min, np.iinfo(np.int32).max]
+    off = np.sort(rng.integers(0, P + 1, E + 1)).astype(np.int32)
+    off[0], off[E] = 0, P
+    sx = rng.random(T).astype(np.float32)
+    Y = Rows(t, P, N, np.full((P, N), 5.0))
+    tier_amd.i8_gemm_grouped(X.ptr, rb, f32(sx).ptr, i32(rows).ptr, T, topk, i32(off).ptr, E, W.ptr, rbw, f32(sw).ptr,
+                             Y.ptr, t, N, P, N, K)
+    hip.synchronize()
+    y = Y.values()
+    nowhere = (rows < 0) | (rows >= T * topk)
+    assert not y[nowhere].any()
+    for e in range(E):
+        at = np.arange(off[e], off[e + 1])
+        at = at[~nowhere[at]]
+        r, c, b = rows[at] // topk, slice(e * N, (e + 1) * N), bad[e * N:(e + 1) * N]
+        assert not np.isfinite(y[at][:, b]).any()
+        if t != tier_amd.F16:  # (fp16 does not hold these sums)
+            check(y[at][:, ~b], t, q[r], sx[r], w[c][~b], sw[c][~b])

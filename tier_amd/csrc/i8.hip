@@ -348,7 +348,8 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
       for (int u = 0; u < INST; ++u) issue(t, u);
     }
 
-  // the scales of the tile's rows and columns, for the end; NaN-free zeros where a row has no source
+  // the scales of the tile's rows and columns, for the end; a far one where a row has no source, so
+  // that store() looks
   for (int i = tid; i < BN; i += 64 * NW) {
     const int n = min(n0 + i, a.N - 1);
     col_scale[i] = sw[n];
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
   }
   for (int i = tid; i < BM; i += 64 * NW) {
     const int xr = source_row<GROUPED>(a, min(tl.m0 + i, tl.m1 - 1));
-    row_scale[i] = xr < 0 ? 0.f : a.sx[xr];
+    row_scale[i] = xr < 0 ? 0x1p-127f : a.sx[xr];
   }
 
   i32x16 acc[WN][WM];
@@ -454,6 +455,8 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
       const int rw = (i * WVM + wm) * 32, mb = tl.m0 + rw;
       if (mb >= tl.m1) break;
       const float s = row_scale[rw + fr];
+      // rows without a source are zeros, whatever the columns' scales are
+      const bool none = FAR && GROUPED && source_row<GROUPED>(a, min(mb + fr, tl.m1 - 1)) < 0;
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -464,7 +467,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int sum = acc[j0 + j][i][4 * b + k];
-            v[k] = FAR ? scaled(sum, s, cs[k], cb[k]) : scaled_near(sum, s, cs[k], cb[k]);
+            v[k] = none ? 0.f : FAR ? scaled(sum, s, cs[k], cb[k]) : scaled_near(sum, s, cs[k], cb[k]);
           }
           Y::set4(part + out_place<CH>(fr, c * Y::ES), v);
         }
@@ -786,7 +789,7 @@ __global__ __launch_bounds__(64 * WVN * WVK) void i8_tile_kernel(const I8Args a)
     }
     if (__builtin_expect(!near, 0)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = scaled(v[k], sc, cs[k], cb[k]);
+      for (int k = 0; k < 4; ++k) o[k] = xr < 0 ? 0.f : scaled(v[k], sc, cs[k], cb[k]);
     }
     Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, min(4, a.N - n));
   }
