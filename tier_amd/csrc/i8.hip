@@ -421,15 +421,18 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
 #pragma unroll
     for (int u = 0; u < D0; ++u) issue(S - 1, u);
   }
+  // scales of this wave's elements, to see at the end whether one is far
+  float scale_x[WM], scale_w[WN];
 #pragma unroll
-  for (int v = 0; v < NF; ++v) fragment(WM, 0, 0, 0, v);
-  // whether a scale of this wave's elements is far, for the end
-  ScaleRange range;
+  for (int i = 0; i < WM; ++i) scale_x[i] = row_scale[(i * WVM + wm) * 32 + fr];
 #pragma unroll
-  for (int i = 0; i < WM; ++i) range.add(row_scale[(i * WVM + wm) * 32 + fr]);
+  for (int j = 0; j < WN; ++j) scale_w[j] = col_scale[(wn * WN + j) * 32 + fr];
+  __builtin_amdgcn_sched_barrier(0);  // the first fragments in the loop's own order, one wait for each
 #pragma unroll
-  for (int j = 0; j < WN; ++j) range.add(col_scale[(wn * WN + j) * 32 + fr]);
-  const bool wave_far = __ballot(range.far()) != 0;
+  for (int v = 0; v < NF; ++v) {
+    fragment(WM, 0, 0, 0, v);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   for (int kt = 0; kt < a.nk; ++kt) {
     step(0, kt, 1, kt + S - 1, D0, D1);
     step(1, kt, 2, kt + S - 1, D0 + D1, D2);
@@ -486,6 +489,12 @@ __global__ __launch_bounds__(64 * WVM * WVN) void i8_gemm_kernel(const I8Args a)
     for (int j0 = 0; j0 + JB <= WN; j0 += JB) store(far_scales, std::integral_constant<int, JB>(), j0);
     if constexpr (WN % JB) store(far_scales, std::integral_constant<int, WN % JB>(), WN - WN % JB);
   };
+  ScaleRange range;
+#pragma unroll
+  for (int i = 0; i < WM; ++i) range.add(scale_x[i]);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) range.add(scale_w[j]);
+  const bool wave_far = __ballot(range.far()) != 0;
   __syncthreads();  // every wave has read its last stage
   if (__builtin_expect(wave_far, 0)) return store_all(std::true_type());
   store_all(std::false_type());
