@@ -371,13 +371,15 @@ int tiermm_moe_unsort_grad(const void* dout, int ytype, size_t ldo, const void* 
 /* ------------------------------ int8 products with a scale for each token and channel */
 /* No reference function.  Both sides are rows of int8 codes with one fp32 scale a row:
  * Y[m][n] = sx[m] * sw[n] * sum_k Xq[m][k] * Wq[n][k] (+ bias[n]).  The sum is exact
- * (int32 MFMA; K <= 133120, TIERMM_UNSUPPORTED above), then fp32(sum) * (sx * sw) and
+ * (int32 MFMA; K <= 133120, TIERMM_UNSUPPORTED above) for codes from -127 to 127, as the
+ * quantizer makes them; rows from elsewhere may hold -128 up to K = 132104 on one side and
+ * 131071 on both, above which a sum can pass 2^31 and wrap.  Then fp32(sum) * (sx * sw) and
  * the bias in fp32 (where sx * sw is not a normal fp32 number, fp32(sum) times the smaller
- * scale, then times the larger: what fits fp32 is neither lost nor infinite), and one rounding
- * to the output's type: results do not depend on the shape of the call.  An int8 row holds tiermm_i8_row_bytes(K) bytes: K codes, then
- * zeros to a whole number of 128 bytes (rows of x: zeros; what a weight's padding holds
- * does not matter, but it has to be there).  Row strides rb may be longer, in whole
- * 16-byte units, from a 16-byte aligned start.
+ * scale, then times the larger: what fits fp32 is neither lost nor infinite), and one
+ * rounding to the output's type: results do not depend on the shape of the call.  An int8
+ * row holds tiermm_i8_row_bytes(K) bytes: K codes, then zeros to a whole number of 128
+ * bytes (rows of x: zeros; what a weight's padding holds does not matter, but it has to be
+ * there).  Row strides rb may be longer, in whole 16-byte units, from a 16-byte aligned start.
  * A frozen linear's input gradient is the same product on W transposed and quantized by
  * its own rows: dX = dY * W with Wt[K][N], tiermm_i8_linear(dY, Wt). */
 size_t tiermm_i8_row_bytes(int K); /* 0 where K is not supported */

@@ -158,3 +158,27 @@ def test_rows_that_point_nowhere(gpu, t, P, E, N, K):
         assert not np.isfinite(y[at][:, b]).any()
         if t != tier_amd.F16:  # (fp16 does not hold these sums)
             check(y[at][:, ~b], t, q[r], sx[r], w[c][~b], sw[c][~b])
+
+
+@pytest.mark.parametrize("M", [1, 3, 20, 140])
+@pytest.mark.parametrize("x,K", [(127, 132104), (-127, 132104), (-128, 131071)])
+def test_largest_sums_with_codes_of_128(gpu, M, x, K):
+    """Weights of -128 all over against the codes of largest magnitude, at the largest K that the header
+    states for them: the sums are 2^31 - 1024 and thereabouts, and exact."""
+    N, t = 3, tier_amd.F32
+    assert abs(x) * 128 * K < 2 ** 31 <= abs(x) * 128 * (K + 1)
+    w = np.full((N, K), -128, np.int64)
+    w[1] = 127
+    q = np.full((M, K), x, np.int64)
+    W, rbw = i8_rows(w)
+    X, rbx = i8_rows(q)
+    one, Y = np.ones(M, np.float32), Rows(t, M, N)
+    tier_amd.i8_gemm(X.ptr, rbx, f32(one).ptr, W.ptr, rbw, f32(np.ones(N)).ptr, None, Y.ptr, t, N, M, N, K)
+    hip.synchronize()
+    check(Y.values(), t, q, one, w, np.ones(N, np.float32))
+    # and of an expert's rows
+    Z = Rows(t, M, N)
+    tier_amd.i8_gemm_grouped(X.ptr, rbx, f32(one).ptr, None, M, 1, i32([0, M]).ptr, 1, W.ptr, rbw, f32(np.ones(N)).ptr,
+                             Z.ptr, t, N, M, N, K)
+    hip.synchronize()
+    assert np.array_equal(Y.bits(), Z.bits())

@@ -3,9 +3,11 @@
 // makes such rows.  No reference function (the reference's own 8-bit form is q8_0,
 // whose activations stay fp32).
 //
-// The sum is a whole number, exact in int32 for K <= 133152 (2^31 / 127^2), so neither
-// the tile, the order of K nor a split of it changes a result: one rounding of the sum
-// to fp32, two products, the bias, and the output's own rounding.
+// The sum is a whole number.  Codes of the quantizer are -127 to 127, and their sums exact in
+// int32 for K <= 133144 (2^31 / 127^2); a code of -128, which rows from elsewhere may hold, leaves
+// room for K <= 132104 on one side and 131071 on both.  So neither the tile, the order of K nor a
+// split of it changes a result: one rounding of the sum to fp32, two products, the bias, and the
+// output's own rounding.
 //
 // An int8 row is padded with zeros to whole 128-byte steps (i8_row_bytes), so no kernel
 // has a K tail: padding of x adds zeros whatever the padding of W holds.
@@ -22,7 +24,7 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kStep = 128;          // bytes of K a row holds a step
-constexpr int kMaxK = 133120;       // whole steps below 2^31 / 127^2
+constexpr int kMaxK = 133120;       // whole steps up to 2^31 / 127^2
 
 constexpr int padded(int K) { return (K + kStep - 1) / kStep * kStep; }
 
