@@ -83,20 +83,25 @@ class TiermmUnsupported(TiermmError):
     pass
 
 
+# (by its path: `python -m tier_amd.build` would import this package first)
+_BUILD = f"run `python {os.path.join(HERE, 'build.py')}`"
 if not os.path.isfile(LIB_PATH):
-    raise ImportError(f"{LIB_PATH} is not built: run `python -m tier_amd.build` (no CPU fallback exists)")
+    raise ImportError(f"{LIB_PATH} is not built: {_BUILD} (no CPU fallback exists)")
 
 try:
     from . import _call
-except ImportError as e:
-    raise ImportError(f"{os.path.join(HERE, '_call.so')} is not built: run `python -m tier_amd.build`") from e
+except ImportError:  # built without CPython's headers: the same functions are called through ctypes
+    _call = None
 
 _L = ctypes.CDLL(LIB_PATH)
 _vp, _sz, _i, _f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
 
 
 def _sig(name, args, res=ctypes.c_int):
-    fn = getattr(_L, name)
+    try:
+        fn = getattr(_L, name)
+    except AttributeError as e:
+        raise ImportError(f"{LIB_PATH} has no {name}, it is older than this package: {_BUILD}") from e
     fn.argtypes = args
     fn.restype = res
     return fn
@@ -189,9 +194,14 @@ def chat_fp3_noalloc(W: int, x: int, y: int, M: int, K: int, N: int, ldo: int, s
     return True
 
 
-# Entry points whose small calls a ctypes call (1.3 to 2 us) would take longer than: name -> function
-# of the same arguments (integers, addresses, None), the status back.
-_fast = {n: _call.Call(ctypes.cast(getattr(_L, n), _vp).value, len(getattr(_L, n).argtypes))
+def _function(name):
+    """Entry point `name` as a function of integers, addresses and None: through _call where it is built."""
+    f = getattr(_L, name)
+    return _call.Call(ctypes.cast(f, _vp).value, len(f.argtypes)) if _call else f
+
+
+# Entry points whose small calls a ctypes call (1.3 to 2 us) would take longer than.
+_fast = {n: _function(n)
          for n in ("tiermm_moe_plan", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
                    "tiermm_moe_unsort_grad", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
                    "tiermm_i8_gemm_grouped")}

@@ -1,9 +1,10 @@
 """Build libtiermm.so in-tree for gfx950 (hipcc for the kernels, g++ for host-only code).
 
-Run ``python -m tier_amd.build`` or call ``build()``; ``__graft_entry__.build()``
-calls it.  Objects go to ``tier_amd/_build/``; the library to ``tier_amd/libtiermm.so``,
+Run ``python tier_amd/build.py`` (by its path: the package cannot be imported before its
+library is there) or call ``build()``; ``__graft_entry__.build()`` calls it.  Objects go to ``tier_amd/_build/``; the library to ``tier_amd/libtiermm.so``,
 bench.py's measurement kernels (probe.hip) to ``tier_amd/libtiermm_probe.so``, the
-Python calls of the routed-row and int8 entry points (call.c) to ``tier_amd/_call.so``.
+Python calls of the routed-row and int8 entry points (call.c) to ``tier_amd/_call.so``,
+where CPython's headers are installed; without them the package calls through ctypes.
 """
 from __future__ import annotations
 
@@ -72,10 +73,15 @@ def build(verbose: bool = False) -> str:
     tmp = PROBE_LIB + ".tmp"
     _run([HIPCC] + HIP_FLAGS + ["-shared", "-o", tmp, os.path.join(CSRC, "probe.hip")])
     os.replace(tmp, PROBE_LIB)
-    tmp = CALL_LIB + ".tmp"
-    _run(["gcc", "-O2", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", tmp,
-          os.path.join(CSRC, "call.c")])
-    os.replace(tmp, CALL_LIB)
+    include = sysconfig.get_paths()["include"]
+    if os.path.isfile(os.path.join(include, "Python.h")):
+        tmp = CALL_LIB + ".tmp"
+        _run(["gcc", "-O2", "-fPIC", "-shared", "-Wall", "-I", include, "-o", tmp, os.path.join(CSRC, "call.c")])
+        os.replace(tmp, CALL_LIB)
+    else:
+        print(f"{CALL_LIB}: not built, no Python.h in {include}; its entry points are called through ctypes")
+        if os.path.exists(CALL_LIB):  # of older sources
+            os.remove(CALL_LIB)
     return LIB
 
 
