@@ -195,9 +195,15 @@ def chat_fp3_noalloc(W: int, x: int, y: int, M: int, K: int, N: int, ldo: int, s
 
 
 def _function(name):
-    """Entry point `name` as a function of integers, addresses and None: through _call where it is built."""
+    """Entry point `name` as a function of integers and addresses (None: null): through _call where it is built."""
     f = getattr(_L, name)
-    return _call.Call(ctypes.cast(f, _vp).value, len(f.argtypes)) if _call else f
+    if not _call:
+        return f
+    numbers = sum(1 << i for i, a in enumerate(f.argtypes) if a is not _vp)
+    try:
+        return _call.Call(ctypes.cast(f, _vp).value, len(f.argtypes), numbers)
+    except TypeError:  # a _call.so of older sources
+        return f
 
 
 # Entry points whose small calls a ctypes call (1.3 to 2 us) would take longer than.

@@ -21,6 +21,7 @@ typedef struct {
   vectorcallfunc call;
   Fn fn;
   Py_ssize_t n;
+  uint32_t numbers; /* bit i: argument i is a number, which None is not */
 } Call;
 
 static PyObject* call_vector(PyObject* o, PyObject* const* args, size_t nf, PyObject* kw) {
@@ -32,7 +33,11 @@ static PyObject* call_vector(PyObject* o, PyObject* const* args, size_t nf, PyOb
   }
   uint64_t a[MOST] = {0};
   for (Py_ssize_t i = 0; i < n; ++i) {
-    if (args[i] == Py_None) continue; /* a null pointer */
+    if (args[i] == Py_None) { /* a null pointer */
+      if (!(c->numbers >> i & 1)) continue;
+      PyErr_Format(PyExc_TypeError, "argument %zd is None, a number is wanted", i + 1);
+      return NULL;
+    }
     PyObject* v = PyLong_Check(args[i]) ? Py_NewRef(args[i]) : PyNumber_Index(args[i]);
     if (!v) return NULL;
     a[i] = PyLong_AsUnsignedLongLongMask(v);
@@ -50,7 +55,8 @@ static PyObject* call_vector(PyObject* o, PyObject* const* args, size_t nf, PyOb
 static PyObject* call_new(PyTypeObject* t, PyObject* args, PyObject* kw) {
   unsigned long long address;
   Py_ssize_t n;
-  if (!PyArg_ParseTuple(args, "Kn", &address, &n)) return NULL;
+  unsigned numbers = 0;
+  if (!PyArg_ParseTuple(args, "Kn|I", &address, &n, &numbers)) return NULL;
   if (!address || n < 0 || n > MOST) {
     PyErr_SetString(PyExc_ValueError, "Call(address, arguments <= 20)");
     return NULL;
@@ -60,6 +66,7 @@ static PyObject* call_new(PyTypeObject* t, PyObject* args, PyObject* kw) {
   c->call = call_vector;
   c->fn = (Fn)(uintptr_t)address;
   c->n = n;
+  c->numbers = numbers;
   return (PyObject*)c;
 }
 
@@ -68,7 +75,8 @@ static PyMemberDef call_members[] = {
 static PyType_Slot call_slots[] = {{Py_tp_new, call_new},
                                    {Py_tp_call, PyVectorcall_Call},
                                    {Py_tp_members, call_members},
-                                   {Py_tp_doc, "Call(address, n): an int function of n integers or addresses"},
+                                   {Py_tp_doc, "Call(address, n, numbers=0): an int function of n integers or addresses; None is a null\n"
+                                               "address, refused for the arguments whose bit is set in numbers"},
                                    {0, NULL}};
 static PyType_Spec call_spec = {"tier_amd._call.Call", sizeof(Call), 0,
                                 Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL, call_slots};
