@@ -983,7 +983,7 @@ int check_size(const char* who, int M, int N, int K) {
 }
 int check_i8_rows(const char* who, const char* what, const void* p, size_t rb, int K) {
   if (!p) return set_error(TIERMM_EINVAL, "%s: null %s", who, what);
-  if (rb < (size_t)padded(K) || rb % 16 || misaligned(p, 16))
+  if (bad_stride(rb, padded(K)) || rb % 16 || misaligned(p, 16))
     return set_error(TIERMM_EINVAL, "%s: %s rows of %zu bytes (whole 16-byte units from %d up, 16-byte aligned)", who,
                      what, rb, padded(K));
   return TIERMM_OK;
@@ -991,7 +991,7 @@ int check_i8_rows(const char* who, const char* what, const void* p, size_t rb, i
 int check_out(const char* who, const void* Y, int ytype, size_t ldy, int N) {
   const int es = row_elem_bytes(ytype);
   if (!es) return set_error(TIERMM_UNSUPPORTED, "%s: output of type %d", who, ytype);
-  if (ldy < (size_t)N) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, N);
+  if (bad_stride(ldy, N)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, N);
   if (!Y || misaligned(Y, es)) return set_error(TIERMM_EINVAL, "%s: null or misaligned output", who);
   return TIERMM_OK;
 }
@@ -1012,7 +1012,7 @@ int tiermm_i8_quant(const void* x, int xtype, size_t ldx, int8_t* q, size_t rb, 
   if (st != TIERMM_OK) return st;
   const int es = row_elem_bytes(xtype);
   if (!es) return set_error(TIERMM_UNSUPPORTED, "%s: rows of type %d", who, xtype);
-  if (ldx < (size_t)K) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, K);
+  if (bad_stride(ldx, K)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
   if (M == 0) return TIERMM_OK;
   if (!x || misaligned(x, es) || !scale || misaligned(scale, 4))
     return set_error(TIERMM_EINVAL, "%s: null or misaligned buffer", who);
@@ -1049,7 +1049,7 @@ int tiermm_i8_linear(const void* x, int xtype, size_t ldx, const int8_t* W, size
   if (st != TIERMM_OK) return st;
   const int es = row_elem_bytes(xtype);
   if (!es) return set_error(TIERMM_UNSUPPORTED, "%s: x of type %d", who, xtype);
-  if (ldx < (size_t)K) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, K);
+  if (bad_stride(ldx, K)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
   if (M == 0 || N == 0) return TIERMM_OK;
   if (!x || misaligned(x, es)) return set_error(TIERMM_EINVAL, "%s: null or misaligned x", who);
   if ((st = check_out(who, Y, ytype, ldy, N)) != TIERMM_OK) return st;

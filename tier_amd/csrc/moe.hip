@@ -414,7 +414,7 @@ int tiermm_moe_sort(const void* X, int xtype, size_t ldx, const int32_t* token_p
   int es;
   const int st = check_rows(who, xtype, T, topk, K, &es);
   if (st != TIERMM_OK) return st;
-  if (ldx < (size_t)K || lds < (size_t)K) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, K);
+  if (bad_stride(ldx, K) || bad_stride(lds, K)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
   if (T == 0 || topk == 0 || K == 0) return TIERMM_OK;
   if (!X || !token_pairs || !sorted_pairs || !X_sorted) return set_error(TIERMM_EINVAL, "%s: null buffer", who);
   if (misaligned(X, es) || misaligned(X_sorted, es) || misaligned(token_pairs, 4) || misaligned(sorted_pairs, 4))
@@ -438,7 +438,7 @@ int tiermm_moe_sort_grad(const void* dX_sorted, int xtype, size_t lds, const int
   int es;
   const int st = check_rows(who, xtype, T, topk, K, &es);
   if (st != TIERMM_OK) return st;
-  if (ldx < (size_t)K || lds < (size_t)K) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, K);
+  if (bad_stride(ldx, K) || bad_stride(lds, K)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
   if (T == 0 || K == 0) return TIERMM_OK;
   if (!dX || (topk && (!dX_sorted || !token_pairs))) return set_error(TIERMM_EINVAL, "%s: null buffer", who);
   if (misaligned(dX_sorted, es) || misaligned(dX, es) || misaligned(token_pairs, 4))
@@ -461,7 +461,7 @@ int tiermm_moe_unsort(const void* Y_sorted, int ytype, size_t lds, const int32_t
   int es;
   const int st = check_rows(who, ytype, T, topk, N, &es);
   if (st != TIERMM_OK) return st;
-  if (ldo < (size_t)N || lds < (size_t)N) return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, N);
+  if (bad_stride(ldo, N) || bad_stride(lds, N)) return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, N);
   if (T == 0 || N == 0) return TIERMM_OK;
   if (!out || (topk && (!Y_sorted || !token_pairs || !weights)))
     return set_error(TIERMM_EINVAL, "%s: null buffer", who);
@@ -487,8 +487,8 @@ int tiermm_moe_unsort_grad(const void* dout, int ytype, size_t ldo, const void* 
   int es;
   const int st = check_rows(who, ytype, T, topk, N, &es);
   if (st != TIERMM_OK) return st;
-  if (ldo < (size_t)N || lds < (size_t)N || ldd < (size_t)N)
-    return set_error(TIERMM_EINVAL, "%s: row stride below %d", who, N);
+  if (bad_stride(ldo, N) || bad_stride(lds, N) || bad_stride(ldd, N))
+    return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, N);
   if (T == 0 || topk == 0) return TIERMM_OK;
   if (!token_pairs || !sorted_pairs || !weights || !dweights || (N && (!dout || !Y_sorted || !dY_sorted)))
     return set_error(TIERMM_EINVAL, "%s: null buffer", who);

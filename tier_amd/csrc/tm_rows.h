@@ -124,6 +124,10 @@ inline int row_elem_bytes(int xtype) {
   return xtype == QT_F32 ? 4 : xtype == QT_F16 || xtype == QT_BF16 ? 2 : 0;
 }
 
+// Whether rows of `cols` elements (bytes) cannot lie `ld` apart: too close, or as far as only a negative
+// number taken for a size is (2^40 is past the end of any memory).
+inline bool bad_stride(size_t ld, size_t cols) { return ld < cols || ld > (size_t)1 << 40; }
+
 // f(std::integral_constant<int, XT>) for a row type already checked.
 template <class F>
 inline void with_rows(int xtype, F f) {
