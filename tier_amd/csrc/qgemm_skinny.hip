@@ -235,7 +235,7 @@ __global__ __launch_bounds__(1024) void sk_split2(const float* __restrict__ x, c
 // A unit of a row is its bytes of 256 elements.  In LDS it starts at the dword that holds its
 // first byte (ph = 0 or 2 bytes before it) and is CH chunks of 16 bytes long; with TAIL the dword
 // after those lies in a region of its own (tail).  A lane of quarter (kh, t) reads the 16 elements
-// of block 4 kh + 2 (kg / 2) + t that start at 16 (kg % 2).  dec<F32> gives fp16(q_val) for
+// of block 4 kh + 2 (kg / 2) + t that start at 16 (kg % 2).  dec<F32, MT> gives fp16(q_val) for
 // x-ref; for F32 integers times 2^PW or (PLANES == 2) block values in two fp16 parts, and post()
 // is what their sums are multiplied by.
 template <int QT>
@@ -249,21 +249,26 @@ __device__ __forceinline__ h2v as_h2(uint32_t v) { return __builtin_bit_cast(h2v
 __device__ __forceinline__ uint32_t as_u(h2v v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ h2v dup(float f) { return h2v{(_Float16)f, (_Float16)f}; }
 // Codes are read as fp16 subnormals: the 8-bit code c in a 16-bit lane is c * 2^-24, with no
-// conversion.  A pair of x-ref weights fp16(fma(s, code, m)) from such a pair and s * 2^24: two
-// v_fma_mix_f32 and one v_cvt_pk_f16_f32.  The empty asm keeps the fp32 values: v_fma_mixlo / _mixhi
-// round the exact sum to fp16 at once, one fp16 step away from fp32-then-fp16 where fp32 lands on a
-// tie (q4_K and q5_K, a weight in about a million), and took longer (q4_K 8 x 14336 x 5120 24.4 -> 22.9 us,
-// 64 experts of one row 68.6 -> 58.4).
+// conversion.  A pair of x-ref weights fp16(fma(s, code, m)) from such a pair and s * 2^24.
+//
+// APART: two v_fma_mix_f32 and one v_cvt_pk_f16_f32 (the empty asm keeps the fp32 values apart).
+// Otherwise v_fma_mixlo / _mixhi, which round the exact sum to fp16 at once: one fp16 step away from
+// fp32-then-fp16 where fp32 lands on a tie (q4_K and q5_K, a weight in about a million), so only for
+// types whose fp32 sums are exact.  Us, at once -> apart, N = 14336, K = 5120: q4_K M = 2 24.2 -> 21.7,
+// M = 16 26.8 -> 25.6, M = 32 30.2 -> 30.9; q5_K M = 16 28.8 -> 28.1; q6_K M = 16 34.7 -> 32.8; q5_0
+// M = 16 30.9 -> 29.1, M = 32 33.6 -> 34.3; q8_0 M = 4 27.4 -> 27.7, M = 16 38.5 -> 42.4.
+template <bool APART>
 __device__ __forceinline__ uint32_t mix2(uint32_t codes, float s24, float m) {
   const h2v c = as_h2(codes);
   float a = fmaf((float)c[0], s24, m), b = fmaf((float)c[1], s24, m);
-  asm("" : "+v"(a), "+v"(b));
+  if constexpr (APART) asm("" : "+v"(a), "+v"(b));
   return as_u(h2v{(_Float16)a, (_Float16)b});
 }
 // The same for the four codes of v's bytes in element order
+template <bool APART>
 __device__ __forceinline__ void mix4(uint32_t v, float s24, float m, uint32_t& o0, uint32_t& o1) {
-  o0 = mix2(__builtin_amdgcn_perm(0u, v, 0x0c010c00u), s24, m);
-  o1 = mix2(__builtin_amdgcn_perm(0u, v, 0x0c030c02u), s24, m);
+  o0 = mix2<APART>(__builtin_amdgcn_perm(0u, v, 0x0c010c00u), s24, m);
+  o1 = mix2<APART>(__builtin_amdgcn_perm(0u, v, 0x0c030c02u), s24, m);
 }
 // v is NaN where it is not finite: a block with such a scale makes its row NaN
 __device__ __forceinline__ float or_nan(float v) { return __builtin_isfinite(v) ? v : __builtin_nanf(""); }
@@ -339,7 +344,7 @@ struct Sk<QT_Q4_K> {
     h = *(const u32x4*)w;
     q = *(const u32x4*)(w + 16 + 64 * kh + 16 * kg);
   }
-  template <bool F32>
+  template <bool F32, int MT>
   __device__ __forceinline__ void dec(int kh, int t, int kg, uint32_t (&o)[8], uint32_t (&)[8], float) const {
     const int sh = 16 * (kg >> 1) + 8 * t;
     const uint32_t sc = (kq_bytes<false>(h, kh) >> sh) & 0xffu;
@@ -347,7 +352,7 @@ struct Sk<QT_Q4_K> {
       const uint32_t mn = (kq_bytes<true>(h, kh) >> sh) & 0xffu;
       const float dsc = h2f(h[0] & 0xffffu) * (float)sc, dm = h2f(h[0] >> 16) * (float)mn;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mix4((q[k] >> (4 * t)) & 0x0f0f0f0fu, dsc * 0x1p24f, -dm, o[2 * k], o[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) mix4<true>((q[k] >> (4 * t)) & 0x0f0f0f0fu, dsc * 0x1p24f, -dm, o[2 * k], o[2 * k + 1]);
     } else {
       // sc (q - 8) 2^-14, sc |q - 8| at most 504: exact.  q as a subnormal times sc 2^10, less 8 sc 2^-14
       const h2v a = dup((float)(sc << 10)), z = dup((float)sc * -0x1p-11f);
@@ -377,7 +382,7 @@ struct Sk<QT_Q5_K> {
     qh = *(const u32x4*)(w + 16 + 16 * (kg & 1));
     q = *(const u32x4*)(w + 48 + 64 * kh + 16 * kg);
   }
-  template <bool F32>
+  template <bool F32, int MT>
   __device__ __forceinline__ void dec(int kh, int t, int kg, uint32_t (&o)[8], uint32_t (&)[8], float) const {
     const int sb = 4 * kh + 2 * (kg >> 1) + t, sh = 16 * (kg >> 1) + 8 * t;
     const uint32_t sc = (kq_bytes<false>(h, kh) >> sh) & 0xffu;
@@ -388,7 +393,7 @@ struct Sk<QT_Q5_K> {
       const uint32_t mn = (kq_bytes<true>(h, kh) >> sh) & 0xffu;
       const float dsc = h2f(h[0] & 0xffffu) * (float)sc, dm = h2f(h[0] >> 16) * (float)mn;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mix4(v[k], dsc * 0x1p24f, -dm, o[2 * k], o[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) mix4<true>(v[k], dsc * 0x1p24f, -dm, o[2 * k], o[2 * k + 1]);
     } else {  // sc (q - 16) 2^-14, sc |q - 16| at most 1008: exact
       const h2v a = dup((float)(sc << 10)), z = dup((float)sc * -0x1p-10f);
 #pragma unroll
@@ -422,7 +427,7 @@ struct Sk<QT_Q6_K> {
     sc = (int)*(const int8_t*)(so >= 16 * CH ? tail + (so - 16 * CH) : w + so);
     d = half_at(tail + ph);
   }
-  template <bool F32>
+  template <bool F32, int MT>
   __device__ __forceinline__ void dec(int, int t, int kg, uint32_t (&o)[8], uint32_t (&ol)[8], float) const {
     // block r = 2 (kg / 2) + t of the half: nibble kg / 2, qh bits 2 r
     const int n4 = 4 * (kg >> 1), h2 = 4 * (kg >> 1) + 2 * t;
@@ -432,7 +437,7 @@ struct Sk<QT_Q6_K> {
     if constexpr (!F32) {
       const float ds = d * (float)sc;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mix4(v[k], ds * 0x1p22f, -32.f * ds, o[2 * k], o[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) mix4<true>(v[k], ds * 0x1p22f, -32.f * ds, o[2 * k], o[2 * k + 1]);
     } else {
       // sc * (q - 32), at most 4096, in two fp16 parts
       const h2v u = dup(0x1p15f), off = dup(-0.25f), s = dup((float)(sc * 128));
@@ -471,11 +476,11 @@ struct Sk<QT_Q8_0> {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] ^= 0x80808080u;
   }
-  template <bool F32>
+  template <bool F32, int MT>
   __device__ __forceinline__ void dec(int, int, int, uint32_t (&o)[8], uint32_t (&ol)[8], float nm) const {
     if constexpr (!F32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mix4(v[k], d * 0x1p24f, -128.f * d, o[2 * k], o[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) mix4<false>(v[k], d * 0x1p24f, -128.f * d, o[2 * k], o[2 * k + 1]);
     } else {
       block_parts<128>(v, d * nm, o, ol);
     }
@@ -499,11 +504,11 @@ struct Sk<QT_Q5_0> {
     for (int k = 0; k < 4; ++k)
       v[k] = ((v[k] >> (4 * hf)) & 0x0f0f0f0fu) | (((__umul24((q >> (4 * k)) & 15u, 0x00204081u)) & 0x01010101u) << 4);
   }
-  template <bool F32>
+  template <bool F32, int MT>
   __device__ __forceinline__ void dec(int, int, int, uint32_t (&o)[8], uint32_t (&ol)[8], float nm) const {
     if constexpr (!F32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mix4(v[k], d * 0x1p24f, -16.f * d, o[2 * k], o[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) mix4<MT == 1>(v[k], d * 0x1p24f, -16.f * d, o[2 * k], o[2 * k + 1]);
     } else {
       block_parts<16>(v, d * nm, o, ol);
     }
@@ -696,7 +701,7 @@ __global__ __launch_bounds__(256 * sk_rw(MT))
         cur[i].read(ws + row * (16 * CH), ws + L::WG * 1024 + row * 4, (ph[i] + D::UB * u) & 2, kh, t, kg,
                     SK_UNIT * u + 128 * kh + 64 * (kg >> 1) + 32 * t < p.K);
         if constexpr (F32) nm[i] = cur[i].norm();
-        cur[i].template dec<F32>(kh, t, kg, o[i], ol[i], F32 ? nm[i] : 1.f);
+        cur[i].template dec<F32, MT>(kh, t, kg, o[i], ol[i], F32 ? nm[i] : 1.f);
         if (i == 0) {
           ahead = 0;
           if (more(i0)) produce(next);
