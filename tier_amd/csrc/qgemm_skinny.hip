@@ -22,8 +22,8 @@
 //   F32, N = 14336, K = 5120:  q4_K M = 2  58.7 -> 25.9, M = 37  61.3 -> 39.2;  q5_K M = 2  63.5 -> 28.7,
 //     M = 37  66.0 -> 41.9;  q6_K M = 2  61.6 -> 34.6, M = 37  64.2 -> 47.3;  q8_0 M = 2  69.9 -> 32.6
 //   F32, N = 1024, K = 4096:  q4_K M = 2  23.8 -> 14.3, M = 37  25.3 -> 21.0
-//   x-ref, N = 14336, K = 5120:  q4_K M = 2  45.8 -> 24.3, M = 16  47.9 -> 27.3, M = 32  44.3 -> 31.7;
-//     q6_K M = 16  56.9 -> 34.9;  q8_0 M = 16  63.6 -> 38.5;  q5_0 M = 4  49.6 -> 29.0
+//   x-ref, N = 14336, K = 5120:  q4_K M = 2  45.8 -> 21.7, M = 16  47.9 -> 25.6, M = 32  44.3 -> 30.9;
+//     q6_K M = 16  56.9 -> 32.9;  q8_0 M = 16  63.6 -> 38.5;  q5_0 M = 4  49.6 -> 25.9
 // with errors against fp64 no larger (F32 q4_K, N(0, 1): 4.0e-7 -> 1.4e-7).  What is left over the
 // weights' read (8 us at q4_K) is the split and reduce launches (4 to 5 us each) and, at M = 37 in the
 // kernel's 34 us, 15 us of VALU issue (mostly decode), 7 of MFMAs, 6 of LDS reads and 13 of the
@@ -52,7 +52,8 @@ constexpr int SK_WR = 2;          // 16-row W tiles of a wave
 // meeting apart from the ring, so the loads no longer stop between two items.
 // Measured before and after on one card, us a call: 8 tokens, top 8 of 64 experts, hidden 2048, ffn
 // 1408 (both products and the combine) 127 -> 108, 1 token 44.7 -> 41.9; F32 q4_K 14336x5120 M = 8
-// 27.1 -> 26.2.  (The fused kernel took 243 for the 8 tokens.)
+// 27.1 -> 26.2.  (The fused kernel took 243 for the 8 tokens.  With mix2's roundings apart they
+// take 98.)
 constexpr int sk_pack(bool f32) { return f32 ? 8 : 4; }
 // Row waves of a workgroup, each for four K quarters, by the row tiles of x
 constexpr int sk_rw(int mt) { return mt == 1 ? 2 : 4; }
