@@ -411,6 +411,93 @@ int tiermm_i8_gemm_grouped(const int8_t* Xq, size_t rbx, const float* sx, const 
                            const int32_t* expert_offsets, int n_experts, const int8_t* W, size_t rbw, const float* sw,
                            void* Y, int ytype, size_t ldy, int P, int N, int K, tiermm_stream_t stream);
 
+/* -------------------------------------------------- RMS norm in front of a product */
+/* No reference entry points (the engine's norms are kernels of its own, fp32 in and out).  For M rows
+ * of K elements of type xtype (TIERMM_F32, TIERMM_F16 or TIERMM_BF16):
+ *   h = x + residual, rounded to xtype (x itself where residual is NULL)
+ *   r = the fp32 number next to 1 / sqrt(mean(h^2) + eps), the mean held in 64 bits
+ *   y = (h * r) * gain, two fp32 products; gain: K fp32
+ * with an output for each pointer that is not NULL: h and y as rows of xtype, q as int8 codes of y
+ * with scale[m], as tiermm_i8_quant makes them of fp32 rows (tiermm_i8_gemm's operand), and
+ * rstd[m] = r, which the gradient takes.  Strides of rows count elements (not looked at where the
+ * pointer is NULL), rb bytes as in tiermm_i8_quant.  Codes do not depend on the shape of the call.
+ * h may be x or the residual, with that one's stride; other outputs must not overlap inputs or
+ * each other.  K <= 1048576 (with q: 133120). */
+int tiermm_rms_norm(const void* x, int xtype, size_t ldx, const void* residual, size_t ldr, const float* gain,
+                    float eps, void* h, size_t ldh, void* y, size_t ldy, int8_t* q, size_t rb, float* scale,
+                    float* rstd, int M, int K, tiermm_stream_t stream);
+/* The same with microscaled codes of y, as tiermm_mx_quant makes them of fp32 rows (tiermm_mx_gemm's
+ * operand). */
+int tiermm_rms_norm_mx(const void* x, int xtype, size_t ldx, const void* residual, size_t ldr, const float* gain,
+                       float eps, void* h, size_t ldh, void* y, size_t ldy, int fmt, void* q, size_t rb,
+                       uint8_t* scales, size_t sb, float* rstd, int M, int K, tiermm_stream_t stream);
+/* The gradients, of rows of one type: with xh = h * rstd and d = dy * gain,
+ *   dx = rstd * (d - xh * mean(d * xh)) + dh   (of x and of the residual alike; dh: the gradient that
+ *                                               reaches h by other ways, or NULL)
+ *   dgain = sum over the rows of dy * xh       (fp32, written; NULL: not computed)
+ * Sums are fp32 in a fixed order.  dx may be dy or dh, with that one's stride.  Workspace
+ * (tiermm_rms_norm_grad_ws_bytes, 4-byte aligned) only for dgain. */
+int tiermm_rms_norm_grad(const void* dy, int type, size_t ldy, const void* h, size_t ldh, const float* gain,
+                         const float* rstd, const void* dh, size_t lddh, void* dx, size_t lddx, float* dgain, int M,
+                         int K, void* ws, size_t ws_bytes, tiermm_stream_t stream);
+size_t tiermm_rms_norm_grad_ws_bytes(int M, int K);
+
+/* ------------------------------------------------------------ microscaled products */
+/* No reference functions (the reference expands its MXFP4 blocks).  Rows of small floating-point
+ * elements with a power-of-two scale for every 32 of them, in the formats of the OCP Microscaling
+ * specification: elements E2M1 (4 bits, two in a byte, the first in the low bits; largest 6) or E4M3
+ * (8 bits; largest 448), scales E8M0 (the byte b stands for 2^(b - 127), 255 for NaN).  A row holds
+ * tiermm_mx_row_bytes(fmt, K) bytes of elements, padded with zeros to whole 256 of them, and
+ * tiermm_mx_scale_bytes(K) scales, padded with zeros to whole 16; strides rb and sb may be longer, in
+ * whole 16-byte units, from 16-byte aligned starts.  Padding of every operand has to be zeros. */
+enum { TIERMM_MX_E2M1 = 4, TIERMM_MX_E4M3 = 8 }; /* bits of an element */
+size_t tiermm_mx_row_bytes(int fmt, int K); /* 0 where fmt or K (1 to 1048576) is not supported */
+size_t tiermm_mx_scale_bytes(int K);
+/* Codes and scales of M rows of x (TIERMM_F32, TIERMM_F16 or TIERMM_BF16, ldx elements apart): the scale
+ * of a block is 2^(floor(log2 max|x|) - 2) (E4M3: - 8), not below 2^-127; elements are x / scale, exactly,
+ * rounded to nearest even, magnitudes past the largest becoming it.  A block that holds a NaN or an
+ * infinity gets the scale NaN and codes 0, so every product of the row is NaN. */
+int tiermm_mx_quant(const void* x, int xtype, size_t ldx, int fmt, void* q, size_t rb, uint8_t* scales, size_t sb,
+                    int M, int K, tiermm_stream_t stream);
+/* N rows of K columns of TIERMM_MXFP4 blocks (rb bytes apart; a .tq or GGUF matrix), laid out once as
+ * E2M1 rows and their scales, value for value.  (A block scale of 255, 2^128 in that type, becomes NaN.) */
+int tiermm_mx_from_mxfp4(const void* W, size_t rb, void* q, size_t rbq, uint8_t* scales, size_t sb, int N, int K,
+                         tiermm_stream_t stream);
+/* Y[M][N] = X * W^T (+ bias[n], fp32, or NULL): x of xfmt, W E2M1, both with their scales; sums in fp32 on
+ * scaled MFMA, rounded once to ytype (TIERMM_F32, TIERMM_F16 or TIERMM_BF16), in an order that depends on
+ * M, N and K alone.  A frozen linear's input gradient is the same product on W transposed and
+ * quantized by its own rows. */
+int tiermm_mx_gemm(const void* Xq, int xfmt, size_t rbx, const uint8_t* sx, size_t sbx, const void* W, size_t rbw,
+                   const uint8_t* sw, size_t sbw, const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K,
+                   tiermm_stream_t stream);
+/* tiermm_mx_quant and the product in one call.  ws 16-byte aligned. */
+int tiermm_mx_linear(const void* x, int xtype, size_t ldx, int xfmt, const void* W, size_t rbw, const uint8_t* sw,
+                     size_t sbw, const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K, void* ws,
+                     size_t ws_bytes, tiermm_stream_t stream);
+size_t tiermm_mx_linear_ws_bytes(int xfmt, int M, int N, int K);
+
+/* ------------------------------------------------- a routed layer of a few tokens */
+/* No reference function (the reference refuses MoE models, arch.py:158-159).  T tokens (at most
+ * TIERMM_MOE_LAYER_TOKENS) of int8 rows Xq[T][K] with their scales, as tiermm_rms_norm or
+ * tiermm_i8_quant makes them, each through its topk (at most TIERMM_MOE_LAYER_TOPK) experts:
+ *   g, u   = the int8 products with rows 0 .. F - 1 (gate) and F .. 2F - 1 (up) of Wgu[e][2F][K]
+ *   h      = silu(g) * u, in 64 bits, rounded once to fp32
+ *   hq, sh = codes and scale of h's row, as tiermm_i8_quant makes them
+ *   out[t] = sum_j weights[t][j] * (the int8 product of hq with Wd[e][K][F]), in fp32 in j order,
+ *            rounded once to otype (TIERMM_F32, TIERMM_F16 or TIERMM_BF16)
+ * with e = expert_ids[t][j], a device array as the router made it, as weights (fp32) is: nothing of the routing
+ * is read on the host, and a captured graph follows new ones.  A pair whose id lies outside
+ * [0, n_experts) is dropped, its weight with it; a token of dropped pairs alone gives zeros.  Weights
+ * and scales are int8 products' (sgu[e][2F], sd[e][K]); an expert's weights are read once for all its tokens.
+ * Results do not depend on T or on the other tokens.  ws (tiermm_moe_i8_layer_ws_bytes) 16-byte aligned. */
+#define TIERMM_MOE_LAYER_TOKENS 64
+#define TIERMM_MOE_LAYER_TOPK 32
+int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int32_t* expert_ids, const float* weights,
+                        const int8_t* Wgu, size_t rbg, const float* sgu, const int8_t* Wd, size_t rbd, const float* sd,
+                        void* out, int otype, size_t ldo, int T, int topk, int n_experts, int K, int F, void* ws,
+                        size_t ws_bytes, tiermm_stream_t stream);
+size_t tiermm_moe_i8_layer_ws_bytes(int T, int topk, int K, int F);
+
 /* ------------------------------------------------------ host quantizer */
 /* q_row (quant.h:201-204) over `rows` rows of `cols` host floats, writing
  * rows*rb bytes of blocks to host memory `out`: Q8_0 (quant.h:134-136),

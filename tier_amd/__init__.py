@@ -70,6 +70,9 @@ EXPORTS = (
     "tiermm_moe_plan", "tiermm_moe_plan_ws_bytes", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
     "tiermm_moe_unsort_grad", "tiermm_i8_row_bytes", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
     "tiermm_i8_linear_ws_bytes", "tiermm_i8_gemm_grouped",
+    "tiermm_rms_norm", "tiermm_rms_norm_mx", "tiermm_rms_norm_grad", "tiermm_rms_norm_grad_ws_bytes",
+    "tiermm_mx_row_bytes", "tiermm_mx_scale_bytes", "tiermm_mx_quant", "tiermm_mx_from_mxfp4", "tiermm_mx_gemm",
+    "tiermm_mx_linear", "tiermm_mx_linear_ws_bytes", "tiermm_moe_i8_layer", "tiermm_moe_i8_layer_ws_bytes",
 )
 
 
@@ -182,6 +185,21 @@ _sig("tiermm_i8_gemm", [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _i, _sz, _i, _i,
 _sig("tiermm_i8_linear", [_vp, _i, _sz, _vp, _sz, _vp, _vp, _vp, _i, _sz, _i, _i, _i, _vp, _sz, _vp])
 _sig("tiermm_i8_linear_ws_bytes", [_i, _i, _i], _sz)
 _sig("tiermm_i8_gemm_grouped", [_vp, _sz, _vp, _vp, _i, _i, _vp, _i, _vp, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _vp])
+_sig("tiermm_rms_norm", [_vp, _i, _sz, _vp, _sz, _vp, _f, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _i, _i, _vp])
+_sig("tiermm_rms_norm_mx", [_vp, _i, _sz, _vp, _sz, _vp, _f, _vp, _sz, _vp, _sz, _i, _vp, _sz, _vp, _sz, _vp, _i, _i,
+                            _vp])
+_sig("tiermm_rms_norm_grad", [_vp, _i, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _i, _i, _vp, _sz, _vp])
+_sig("tiermm_rms_norm_grad_ws_bytes", [_i, _i], _sz)
+_sig("tiermm_mx_row_bytes", [_i, _i], _sz)
+_sig("tiermm_mx_scale_bytes", [_i], _sz)
+_sig("tiermm_mx_quant", [_vp, _i, _sz, _i, _vp, _sz, _vp, _sz, _i, _i, _vp])
+_sig("tiermm_mx_from_mxfp4", [_vp, _sz, _vp, _sz, _vp, _sz, _i, _i, _vp])
+_sig("tiermm_mx_gemm", [_vp, _i, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _vp])
+_sig("tiermm_mx_linear", [_vp, _i, _sz, _i, _vp, _sz, _vp, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _vp, _sz, _vp])
+_sig("tiermm_mx_linear_ws_bytes", [_i, _i, _i, _i], _sz)
+_sig("tiermm_moe_i8_layer", [_vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _i, _i,
+                             _vp, _sz, _vp])
+_sig("tiermm_moe_i8_layer_ws_bytes", [_i, _i, _i, _i], _sz)
 NOALLOC_SCRATCH_BYTES = 32 << 20  # TIERMM_NOALLOC_SCRATCH_BYTES
 
 
@@ -195,14 +213,16 @@ def chat_fp3_noalloc(W: int, x: int, y: int, M: int, K: int, N: int, ldo: int, s
 
 
 def _function(name):
-    """Entry point `name` as a function of integers and addresses (None: null): through _call where it is built."""
+    """Entry point `name` as a function of integers, addresses (None: null) and one float at most: through
+    _call where it is built."""
     f = getattr(_L, name)
     if not _call:
         return f
     numbers = sum(1 << i for i, a in enumerate(f.argtypes) if a is not _vp)
+    floats = sum(1 << i for i, a in enumerate(f.argtypes) if a is _f)
     try:
-        return _call.Call(ctypes.cast(f, _vp).value, len(f.argtypes), numbers)
-    except TypeError:  # a _call.so of older sources
+        return _call.Call(ctypes.cast(f, _vp).value, len(f.argtypes), numbers, *((floats,) if floats else ()))
+    except (TypeError, ValueError):  # a _call.so of older sources
         return f
 
 
@@ -210,11 +230,15 @@ def _function(name):
 _fast = {n: _function(n)
          for n in ("tiermm_moe_plan", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
                    "tiermm_moe_unsort_grad", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
-                   "tiermm_i8_gemm_grouped")}
+                   "tiermm_i8_gemm_grouped", "tiermm_rms_norm", "tiermm_rms_norm_mx", "tiermm_rms_norm_grad",
+                   "tiermm_mx_quant", "tiermm_mx_gemm", "tiermm_mx_linear", "tiermm_moe_i8_layer")}
 _moe_plan, _moe_sort, _moe_sort_grad = (_fast["tiermm_moe_" + n] for n in ("plan", "sort", "sort_grad"))
 _moe_unsort, _moe_unsort_grad = _fast["tiermm_moe_unsort"], _fast["tiermm_moe_unsort_grad"]
 _i8_quant, _i8_gemm, _i8_linear, _i8_gemm_grouped = (
     _fast["tiermm_i8_" + n] for n in ("quant", "gemm", "linear", "gemm_grouped"))
+_rms_norm, _rms_norm_mx, _rms_norm_grad = (_fast["tiermm_rms_norm" + n] for n in ("", "_mx", "_grad"))
+_mx_quant, _mx_gemm, _mx_linear = (_fast["tiermm_mx_" + n] for n in ("quant", "gemm", "linear"))
+_moe_i8_layer = _fast["tiermm_moe_i8_layer"]
 
 
 def lib():
@@ -560,6 +584,94 @@ def i8_gemm_grouped(Xq: int, rbx: int, sx: int, rows: int | None, n_rows: int, t
     is row rows[p] / topk of Xq times its expert's weight."""
     _check(_i8_gemm_grouped(Xq, rbx, sx, rows, n_rows, topk, expert_offsets, n_experts, W, rbw, sw, Y, ytype, ldy, P,
                             N, K, _s(stream)))
+
+
+# --------------------------------------------------- RMS norm in front of a product
+def rms_norm(x: int, xtype: int, ldx: int, residual: int | None, ldr: int, gain: int, eps: float, h: int | None,
+             ldh: int, y: int | None, ldy: int, q: int | None, rb: int, scale: int | None, rstd: int | None, M: int,
+             K: int, stream=None) -> None:
+    """h = x + residual, y = h / sqrt(mean(h^2) + eps) * gain: h and y as rows of xtype, q as int8 codes of y
+    with their scales (i8_gemm's x), rstd for rms_norm_grad, each where it is not None."""
+    _check(_rms_norm(x, xtype, ldx, residual, ldr, gain, eps, h, ldh, y, ldy, q, rb, scale, rstd, M, K, _s(stream)))
+
+
+def rms_norm_mx(x: int, xtype: int, ldx: int, residual: int | None, ldr: int, gain: int, eps: float, h: int | None,
+                ldh: int, y: int | None, ldy: int, fmt: int, q: int, rb: int, scales: int, sb: int, rstd: int | None,
+                M: int, K: int, stream=None) -> None:
+    """rms_norm with microscaled codes of y (mx_gemm's x)."""
+    _check(_rms_norm_mx(x, xtype, ldx, residual, ldr, gain, eps, h, ldh, y, ldy, fmt, q, rb, scales, sb, rstd, M, K,
+                        _s(stream)))
+
+
+def rms_norm_grad(dy: int, type: int, ldy: int, h: int, ldh: int, gain: int, rstd: int, dh: int | None, lddh: int,
+                  dx: int, lddx: int, dgain: int | None, M: int, K: int, ws: int | None = None, ws_bytes: int = 0,
+                  stream=None) -> None:
+    """Gradients of rms_norm: dx of x and of the residual alike (dh, where given, added), dgain fp32 [K]."""
+    _check(_rms_norm_grad(dy, type, ldy, h, ldh, gain, rstd, dh, lddh, dx, lddx, dgain, M, K, ws, ws_bytes,
+                          _s(stream)))
+
+
+def rms_norm_grad_ws_bytes(M: int, K: int) -> int:
+    return _L.tiermm_rms_norm_grad_ws_bytes(M, K)
+
+
+# ------------------------------------------------------------ microscaled products
+MX_E2M1, MX_E4M3 = 4, 8  # TIERMM_MX_E2M1, TIERMM_MX_E4M3
+
+
+def mx_row_bytes(fmt: int, K: int) -> int:
+    """Bytes of a microscaled row of K elements: zero-padded to whole 256 elements."""
+    return _L.tiermm_mx_row_bytes(fmt, K)
+
+
+def mx_scale_bytes(K: int) -> int:
+    """Bytes of a microscaled row's scales: one for each 32 elements, zero-padded to whole 16."""
+    return _L.tiermm_mx_scale_bytes(K)
+
+
+def mx_quant(x: int, xtype: int, ldx: int, fmt: int, q: int, rb: int, scales: int, sb: int, M: int, K: int,
+             stream=None) -> None:
+    """E2M1 or E4M3 codes and E8M0 scales of M rows of x (F32, F16 or BF16)."""
+    _check(_mx_quant(x, xtype, ldx, fmt, q, rb, scales, sb, M, K, _s(stream)))
+
+
+def mx_from_mxfp4(W: int, rb: int, q: int, rbq: int, scales: int, sb: int, N: int, K: int, stream=None) -> None:
+    """Rows of MXFP4 blocks, laid out as E2M1 rows and their scales for mx_gemm and mx_linear."""
+    _check(_L.tiermm_mx_from_mxfp4(W, rb, q, rbq, scales, sb, N, K, _s(stream)))
+
+
+def mx_gemm(Xq: int, xfmt: int, rbx: int, sx: int, sbx: int, W: int, rbw: int, sw: int, sbw: int, bias: int | None,
+            Y: int, ytype: int, ldy: int, M: int, N: int, K: int, stream=None) -> None:
+    """Y[m][n] = <X[m], W[n]> (+ bias[n]) of microscaled rows: x of xfmt, W E2M1."""
+    _check(_mx_gemm(Xq, xfmt, rbx, sx, sbx, W, rbw, sw, sbw, bias, Y, ytype, ldy, M, N, K, _s(stream)))
+
+
+def mx_linear(x: int, xtype: int, ldx: int, xfmt: int, W: int, rbw: int, sw: int, sbw: int, bias: int | None, Y: int,
+              ytype: int, ldy: int, M: int, N: int, K: int, ws: int | None = None, ws_bytes: int = 0,
+              stream=None) -> None:
+    """mx_quant of x and mx_gemm in one call."""
+    _check(_mx_linear(x, xtype, ldx, xfmt, W, rbw, sw, sbw, bias, Y, ytype, ldy, M, N, K, ws, ws_bytes, _s(stream)))
+
+
+def mx_linear_ws_bytes(xfmt: int, M: int, N: int, K: int) -> int:
+    return _L.tiermm_mx_linear_ws_bytes(xfmt, M, N, K)
+
+
+# ------------------------------------------------- a routed layer of a few tokens
+MOE_LAYER_TOKENS, MOE_LAYER_TOPK = 64, 32  # TIERMM_MOE_LAYER_TOKENS, TIERMM_MOE_LAYER_TOPK
+
+
+def moe_i8_layer(Xq: int, rbx: int, sx: int, expert_ids: int, weights: int, Wgu: int, rbg: int, sgu: int, Wd: int,
+                 rbd: int, sd: int, out: int, otype: int, ldo: int, T: int, topk: int, n_experts: int, K: int, F: int,
+                 ws: int | None = None, ws_bytes: int = 0, stream=None) -> None:
+    """out[t] = sum_j weights[t][j] * down_e(silu(gate_e(x)) * up_e(x)), e = expert_ids[t][j], over int8 experts
+    Wgu[e][2F][K] (gate, then up) and Wd[e][K][F], for at most MOE_LAYER_TOKENS int8 rows."""
+    _check(_moe_i8_layer(Xq, rbx, sx, expert_ids, weights, Wgu, rbg, sgu, Wd, rbd, sd, out, otype, ldo, T, topk,
+                         n_experts, K, F, ws, ws_bytes, _s(stream)))
+
+
+def moe_i8_layer_ws_bytes(T: int, topk: int, K: int, F: int) -> int:
+    return _L.tiermm_moe_i8_layer_ws_bytes(T, topk, K, F)
 
 
 def qlinear(W: int, qtype: int, rb: int, x: int, y: int, M: int, N: int, K: int, ws: int | None = None,

@@ -3,7 +3,7 @@
 Run ``python tier_amd/build.py`` (by its path: the package cannot be imported before its
 library is there) or call ``build()``; ``__graft_entry__.build()`` calls it.  Objects go to ``tier_amd/_build/``; the library to ``tier_amd/libtiermm.so``,
 bench.py's measurement kernels (probe.hip) to ``tier_amd/libtiermm_probe.so``, the
-Python calls of the routed-row and int8 entry points (call.c) to ``tier_amd/_call.so``,
+Python calls of the norm, routed-row, int8 and microscaled entry points (call.c) to ``tier_amd/_call.so``,
 where CPython's headers are installed; without them the package calls through ctypes.
 """
 from __future__ import annotations
@@ -26,7 +26,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = ["dequant.hip", "qgemv.hip", "qgemv_dot.hip", "qgemv_q4k.hip", "qgemv_q4k_ws.hip", "qgemv_q6k.hip", "qgemm_fused.hip", "qgemm_skinny.hip", "x3.hip",
-               "noalloc.hip", "host_dequant.hip", "chat_ops.hip", "moe.hip", "i8.hip"]
+               "noalloc.hip", "host_dequant.hip", "chat_ops.hip", "moe.hip", "i8.hip", "norm.hip", "mx.hip", "moe_layer.hip"]
 CXX_SOURCES = ["api.cpp", "quantize.cpp", "tq.cpp", "chat.cpp"]
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 are generated (hipcc's host pass
