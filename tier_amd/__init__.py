@@ -231,14 +231,13 @@ _fast = {n: _function(n)
          for n in ("tiermm_moe_plan", "tiermm_moe_sort", "tiermm_moe_sort_grad", "tiermm_moe_unsort",
                    "tiermm_moe_unsort_grad", "tiermm_i8_quant", "tiermm_i8_gemm", "tiermm_i8_linear",
                    "tiermm_i8_gemm_grouped", "tiermm_rms_norm", "tiermm_rms_norm_mx", "tiermm_rms_norm_grad",
-                   "tiermm_mx_quant", "tiermm_mx_gemm", "tiermm_mx_linear", "tiermm_moe_i8_layer")}
+                   "tiermm_mx_quant", "tiermm_mx_gemm", "tiermm_mx_linear")}
 _moe_plan, _moe_sort, _moe_sort_grad = (_fast["tiermm_moe_" + n] for n in ("plan", "sort", "sort_grad"))
 _moe_unsort, _moe_unsort_grad = _fast["tiermm_moe_unsort"], _fast["tiermm_moe_unsort_grad"]
 _i8_quant, _i8_gemm, _i8_linear, _i8_gemm_grouped = (
     _fast["tiermm_i8_" + n] for n in ("quant", "gemm", "linear", "gemm_grouped"))
 _rms_norm, _rms_norm_mx, _rms_norm_grad = (_fast["tiermm_rms_norm" + n] for n in ("", "_mx", "_grad"))
 _mx_quant, _mx_gemm, _mx_linear = (_fast["tiermm_mx_" + n] for n in ("quant", "gemm", "linear"))
-_moe_i8_layer = _fast["tiermm_moe_i8_layer"]
 
 
 def lib():
@@ -666,8 +665,8 @@ def moe_i8_layer(Xq: int, rbx: int, sx: int, expert_ids: int, weights: int, Wgu:
                  ws: int | None = None, ws_bytes: int = 0, stream=None) -> None:
     """out[t] = sum_j weights[t][j] * down_e(silu(gate_e(x)) * up_e(x)), e = expert_ids[t][j], over int8 experts
     Wgu[e][2F][K] (gate, then up) and Wd[e][K][F], for at most MOE_LAYER_TOKENS int8 rows."""
-    _check(_moe_i8_layer(Xq, rbx, sx, expert_ids, weights, Wgu, rbg, sgu, Wd, rbd, sd, out, otype, ldo, T, topk,
-                         n_experts, K, F, ws, ws_bytes, _s(stream)))
+    _check(_L.tiermm_moe_i8_layer(Xq, rbx, sx, expert_ids, weights, Wgu, rbg, sgu, Wd, rbd, sd, out, otype, ldo, T,
+                                  topk, n_experts, K, F, ws, ws_bytes, _s(stream)))
 
 
 def moe_i8_layer_ws_bytes(T: int, topk: int, K: int, F: int) -> int:

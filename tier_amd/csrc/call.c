@@ -9,13 +9,13 @@
 #include <stdint.h>
 #include <structmember.h>
 
-#define MOST 24
+#define MOST 20
 
 /* x86-64: integer arguments travel as 64-bit words whatever their C type, and a callee ignores
  * those past its own.  A float travels in a vector register, whatever its place among them. */
 typedef int (*Fn)(uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t,
                   uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t,
-                  uint64_t, uint64_t, uint64_t, uint64_t, float);
+                  float);
 
 typedef struct {
   PyObject_HEAD
@@ -60,7 +60,7 @@ static PyObject* call_vector(PyObject* o, PyObject* const* args, size_t nf, PyOb
   int code;
   Py_BEGIN_ALLOW_THREADS
   code = c->fn(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15],
-               a[16], a[17], a[18], a[19], a[20], a[21], a[22], a[23], f);
+               a[16], a[17], a[18], a[19], f);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(code);
 }
@@ -71,7 +71,7 @@ static PyObject* call_new(PyTypeObject* t, PyObject* args, PyObject* kw) {
   unsigned numbers = 0, floats = 0;
   if (!PyArg_ParseTuple(args, "Kn|II", &address, &n, &numbers, &floats)) return NULL;
   if (!address || n < 0 || n > MOST || (floats & (floats - 1))) {
-    PyErr_SetString(PyExc_ValueError, "Call(address, arguments <= 24, of them one float)");
+    PyErr_SetString(PyExc_ValueError, "Call(address, arguments <= 20, of them one float)");
     return NULL;
   }
   Call* c = (Call*)t->tp_alloc(t, 0);
