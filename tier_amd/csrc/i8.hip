@@ -12,6 +12,7 @@
 // An int8 row is padded with zeros to whole 128-byte steps (i8_row_bytes), so no kernel
 // has a K tail: padding of x adds zeros whatever the padding of W holds.
 #include "tm_i8.h"
+#include "tm_tiles.h"
 
 #include <algorithm>
 #include <cmath>
@@ -98,13 +99,6 @@ struct Tile {
   int e;      // expert; E: rows that no expert has, which become zeros (zero_tile)
   bool once;  // no other tile reads these rows of W
 };
-
-// Tile `t` of the workgroups' sequence in which XCD x (blockIdx % 8) walks the x-th
-// contiguous share, or -1 past the end.
-__device__ __forceinline__ int xcd_share(int bid, int total) {
-  const int x = bid & 7, i = bid >> 3, each = total >> 3, more = total & 7;
-  return i < each + (x < more) ? x * each + min(x, more) + i : -1;
-}
 
 // Tile `bid` over the experts' rows, expert by expert, and in each column by column; false past
 // the last.  XCD x (bid % 8) takes `share` tiles at a time: their rows of W and X meet in its L2.
@@ -207,30 +201,6 @@ struct ScaleRange {
   }
   __device__ __forceinline__ bool far() const { return least < 0x1p-63f || most >= 0x1p63f; }
 };
-
-// Waits until no more than n (at most N) stages of INST loads are on their way.
-template <int N, int INST>
-__device__ __forceinline__ void wait_stages(int n) {
-  if constexpr (N > 0) {
-    if (n >= N) vm_wait<N * INST>();
-    else wait_stages<N - 1, INST>(n);
-  } else {
-    vm_wait<0>();
-  }
-}
-
-// LDS place of byte `o` of row r of CH 16-byte chunks: neighbouring rows' chunks are
-// spread over the 16 chunks that the banks span.
-template <int CH>
-__device__ __forceinline__ int out_place(int r, int o) {
-  const int c = o >> 4, turn = CH >= 16 ? r : r / (16 / CH);
-  return r * CH * 16 + ((c ^ (turn & (CH - 1))) << 4) + (o & 15);
-}
-// One wave's LDS operations are in order; the compiler must keep them so too.
-__device__ __forceinline__ void wave_lds_wait() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
 
 // BM rows of X times BN rows of W by WVM x WVN waves of WM x WN blocks of 32 x 32.
 //

@@ -6,12 +6,18 @@
 // of a step of 128 elements block l / 16 (E2M1: its 16 bytes; E4M3: 16 bytes of each half of the
 // step) and that block's scale.
 #include "tm_mx.h"
+#include "tm_tiles.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
 
 namespace tiermm {
 namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------------- quantizer
 // A thread takes one unit of 16 bytes of a row; the lanes of a block are neighbours.
@@ -100,54 +106,598 @@ __device__ __forceinline__ i32x8 mx_large(const i32x8& x) {
   return y;
 }
 
-// One wave a tile of 16 x 16, operands straight from memory.
-template <int YT, int XF>
-__global__ __launch_bounds__(64) void mx_simple_kernel(const MxArgs a) {
+// What a workgroup computes: rows [m0, m1) of Y, column tile tn.
+struct Tile {
+  int m0, m1, tn;
+  bool once;  // no other tile reads these rows of W
+};
+// The tile of this workgroup; false past the last.  XCD x takes the x-th contiguous share of a walk in groups
+// of 4 tile rows, column by column.
+template <int BM, int BN>
+__device__ __forceinline__ bool find_tile(const MxArgs& a, Tile& tl) {
+  const int ntn = (a.N + BN - 1) / BN, ntm = (a.M + BM - 1) / BM, t = xcd_share(blockIdx.x, ntm * ntn);
+  if (t < 0) return false;
+  constexpr int GM = 4;
+  const int grp = t / (GM * ntn), first = grp * GM, gm = min(GM, ntm - first), in = t - grp * GM * ntn;
+  tl.m0 = (first + in % gm) * BM;
+  tl.m1 = min(tl.m0 + BM, a.M);
+  tl.tn = in / gm;
+  tl.once = ntm == 1;
+  return true;
+}
+
+// v_mfma_scale_f32_32x32x64_f8f6f4 / _16x16x128_ of W (E2M1) and x, with the scales in byte SEL of each word.
+template <int XF, int SEL>
+__device__ __forceinline__ f32x16 mx_mfma32(const i32x8& w, const i32x8& x, const f32x16& c, int sw, int sx) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 4, XF == MX_E2M1 ? 4 : 0, SEL, sw, SEL, sx);
+}
+template <int XF>
+__device__ __forceinline__ f32x4 mx_mfma16(const i32x8& w, const i32x8& x, const f32x4& c, int sw, int sx) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, XF == MX_E2M1 ? 4 : 0, 0, sw, 0, sx);
+}
+__device__ __forceinline__ i32x8 e2m1(const i32x4& v) { return i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
+__device__ __forceinline__ i32x8 e4m3(const i32x4& lo, const i32x4& hi) {
+  return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// BM rows of x times BN rows of W by WVM x WVN waves of WM x WN blocks of 32 x 32.
+//
+// A stage is 256 elements: 128 bytes of every row of W and of E2M1 x, two times 128 of E4M3 x (blocks 0-3
+// of a row, then 4-7), and 8 scales of every row; S stages take turns, brought to LDS by global_load_lds.
+// A row's 16-byte chunk c lies at slot c ^ ((row >> 1) & 7), which spreads the 16 rows that one cycle of a
+// fragment read touches over the banks.  A stage is four MFMA steps; the order of a sum's blocks is free, so
+// step kk takes block kk in the lower half of the wave and 4 + kk in the upper, and the four scales that a
+// lane needs of a row in a stage are one word, of which step kk uses byte kk.  While the products of one
+// step run, the fragments of the next come in, one read between two MFMAs, and the loads of stage kt + S go
+// out, from the step after the barrier that frees their place on.
+//
+// W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y; rows leave
+// through LDS in 16-byte units.
+template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
+__global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a) {
+  constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, XS = XF == MX_E4M3 ? 2 : 1, NF = WN + WM * XS;
+  constexpr int PARTS = kParts<XF, YT>;
+  constexpr int ROWS = BM * XS + BN, CODES = ROWS * 128, SCALES = (BM + BN) * 8, STAGE = CODES + (SCALES + 255) / 256 * 256;
+  constexpr int IC = CODES / 1024 / NW, IS = (SCALES + 256 * NW - 1) / (256 * NW), INST = IC + IS;
+  static_assert(WM * WVM * 32 == BM && WN * WVN * 32 == BN && IC * NW * 1024 == CODES, "whole blocks and loads a wave");
+  // loads of a stage by the step that issues them: 3 (of the stage before last), 0 and 1
+  constexpr int D0 = (INST + 2) / 3, D1 = (INST - D0 + 1) / 2, D2 = INST - D0 - D1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  float* col_bias = (float*)(lds + S * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Tile tl;
+  if (!find_tile<BM, BN>(a, tl)) return;
+  const int n0 = tl.tn * BN;
   using Y = Rows<YT>;
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4, m = blockIdx.y * 16 + r, n0 = blockIdx.x * 16;
-  const int mr = min(m, a.M - 1), nr = min(n0 + r, a.N - 1);
-  const uint8_t *x = a.X + (size_t)mr * a.rbx, *w = a.W + (size_t)nr * a.rbw;
-  const uint8_t *sx = a.sx + (size_t)mr * a.sbx, *sw = a.sw + (size_t)nr * a.sbw;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int t = 0; t < 2 * a.nk; ++t) {
-    const i32x4 wf = *(const i32x4*)(w + (size_t)t * 64 + g * 16);
-    i32x8 A = {wf[0], wf[1], wf[2], wf[3], 0, 0, 0, 0}, B;
-    if constexpr (XF == MX_E2M1) {
-      const i32x4 xf = *(const i32x4*)(x + (size_t)t * 64 + g * 16);
-      B = i32x8{xf[0], xf[1], xf[2], xf[3], 0, 0, 0, 0};
-    } else {
-      const i32x4 lo = *(const i32x4*)(x + (size_t)t * 128 + g * 16), hi = *(const i32x4*)(x + (size_t)t * 128 + 64 + g * 16);
-      B = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+
+  // load u of this wave: rows 8 * (wave + NW * u) .. + 7 of the stage (x's, its second halves, then W's);
+  // from IC on words of scales (the first of every row's two, then the second)
+  const uint8_t* src[INST];
+  int place[IS];
+#pragma unroll
+  for (int u = 0; u < IC; ++u) {
+    const int r = 8 * (wave + NW * u) + (lane >> 3);
+    const uint8_t* row = r < BM * XS ? a.X + (size_t)min(tl.m0 + r % BM, a.M - 1) * a.rbx + r / BM * 128
+                                     : a.W + (size_t)min(n0 + r - BM * XS, a.N - 1) * a.rbw;
+    src[u] = row + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+  }
+#pragma unroll
+  for (int u = 0; u < IS; ++u) {
+    // (words past the end: the last ones again)
+    place[u] = min(64 * (wave + NW * u), SCALES / 4 - 64);
+    const int i = place[u] + lane, h = i / (BM + BN), r = i % (BM + BN);
+    src[IC + u] = (r < BM ? a.sx + (size_t)min(tl.m0 + r, a.M - 1) * a.sbx : a.sw + (size_t)min(n0 + r - BM, a.N - 1) * a.sbw) + 4 * h;
+  }
+  const uint32_t lds0 = lds_addr(lds);
+  auto ring = [](int kt) { return S == 2 ? kt & 1 : S == 4 ? kt & 3 : kt % S; };
+  auto issue = [&](int kt, int u) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + ring(kt) * STAGE;
+    if (u < IC) dma16(src[u] + (size_t)kt * (u * NW * 8 < BM * XS ? 128 * XS : 128), to + (wave + NW * u) * 1024);
+    else dma4(src[u] + (size_t)kt * 8, to + CODES + 4 * place[u - IC]);
+  };
+  static_assert(BM * XS % (8 * NW) == 0, "a load is of x or of W for every wave alike");
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t)
+    if (t < a.nk) {
+#pragma unroll
+      for (int u = 0; u < INST; ++u) issue(t, u);
     }
-    const int ws = sw[t * 4 + g], xs = sx[t * 4 + g];
-    auto product = [&](const i32x8& b) __attribute__((always_inline)) {
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, b, acc, 4, XF == MX_E2M1 ? 4 : 0, 0, ws, 0, xs);
-    };
-    if constexpr (kParts<XF, YT> == 1) {
-      product(B);
+  for (int i = tid; i < BN; i += 64 * NW) col_bias[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.f;
+
+  f32x16 acc[WN][WM];
+#pragma unroll
+  for (int j = 0; j < WN; ++j)
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
+
+  const int wm = wave % WVM, wn = wave / WVM, fr = lane & 31, fh = lane >> 5, turn = (fr >> 1) & 7;
+  const uint32_t xrow = (uint32_t)(wm * WM * 32 + fr) * 128, wrow = (uint32_t)(BM * XS + wn * WN * 32 + fr) * 128;
+  i32x4 xf[2][WM][XS], wf[2][WN];
+  int xs[WM], ws[WN];
+  // fragment v of step kk of stage kt into set f: W's first, those of x, W's others
+  auto fragment = [&](int kt, int kk, int f, int v) __attribute__((always_inline)) {
+    const uint8_t* s = lds + ring(kt) * STAGE;
+    const int xc = ((XS == 2 ? 2 * kk + fh : 4 * fh + kk) ^ turn) * 16, wc = ((4 * fh + kk) ^ turn) * 16;
+    if (v >= 1 && v <= WM * XS) {
+      const int i = (v - 1) / XS, h = (v - 1) % XS;
+      xf[f][i][h] = *(const i32x4*)(s + xc + xrow + (h * BM + i * 32) * 128);
     } else {
-      const i32x8 large = mx_large(B);
-      product(large);
-      product(B ^ large);
+      const int j = v == 0 ? 0 : v - WM * XS;
+      wf[f][j] = *(const i32x4*)(s + wc + wrow + j * 32 * 128);
+    }
+  };
+  auto scales = [&](int kt, int (&x)[WM], int (&w)[WN]) __attribute__((always_inline)) {
+    const int* s = (const int*)(lds + ring(kt) * STAGE + CODES) + fh * (BM + BN) + fr;
+#pragma unroll
+    for (int i = 0; i < WM; ++i) x[i] = s[(wm * WM + i) * 32];
+#pragma unroll
+    for (int j = 0; j < WN; ++j) w[j] = s[BM + (wn * WN + j) * 32];
+  };
+  // The products of step KK of fragments f, with the fragments (kt, kk) into the other set and loads
+  // u0 .. u0 + n - 1 of stage `dt` between them.
+  auto step = [&](auto kc, int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
+    constexpr int KK = decltype(kc)::value, nm = WM * WN;
+    i32x8 x[WM][PARTS];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) {
+      if constexpr (XS == 1) x[i][0] = e2m1(xf[f][i][0]);
+      else x[i][0] = e4m3(xf[f][i][0], xf[f][i][1]);
+      if constexpr (PARTS == 2) {
+        x[i][1] = mx_large(x[i][0]);
+        x[i][0] ^= x[i][1];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < nm; ++q) {
+#pragma unroll
+      for (int v = 0; v < NF; ++v)
+        if (std::max(v * (nm - 2) / NF, 0) == q) fragment(kt, kk, f ^ 1, v);
+#pragma unroll
+      for (int d = 0; d < n; ++d)
+        if (std::min(1 + d * (nm - 1) / n, nm - 1) == q && dt < a.nk) issue(dt, u0 + d);
+      const int j = q / WM, i = q % WM;
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) acc[j][i] = mx_mfma32<XF, KK>(e2m1(wf[f][j]), x[i][p], acc[j][i], ws[j], xs[i]);
+      // the compiler would sink these products past the loads' branches, all to the end of the loop (no
+      // instruction: nothing reads the sum here)
+      asm volatile("" : "+v"(acc[j][i]));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // waits until stage kt has landed, those up to kt + S - 2 being on their way too
+  auto landed = [&](int kt) __attribute__((always_inline)) {
+    const int behind = a.nk - 1 - kt;
+    if (behind >= S - 2) vm_wait<(S - 2) * INST>();
+    else wait_stages<S - 3, INST>(behind);
+  };
+  landed(0);
+  __syncthreads();
+  if (S - 1 < a.nk) {
+#pragma unroll
+    for (int u = 0; u < D0; ++u) issue(S - 1, u);
+  }
+  scales(0, xs, ws);
+  __builtin_amdgcn_sched_barrier(0);  // the first fragments in the loop's own order, one wait for each
+#pragma unroll
+  for (int v = 0; v < NF; ++v) {
+    fragment(0, 0, 0, v);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  for (int kt = 0; kt < a.nk; ++kt) {
+    step(std::integral_constant<int, 0>(), 0, kt, 1, kt + S - 1, D0, D1);
+    step(std::integral_constant<int, 1>(), 1, kt, 2, kt + S - 1, D0 + D1, D2);
+    step(std::integral_constant<int, 2>(), 0, kt, 3, 0, 0, 0);
+    landed(kt + 1);
+    __syncthreads();  // stage kt + 1 has landed for every wave, and stage kt is read
+    // (past the end: the fragments of what the place holds, which nothing uses)
+    int nx[WM], nw[WN];
+    scales(kt + 1, nx, nw);
+    step(std::integral_constant<int, 3>(), 1, kt + 1, 0, kt + S, 0, D0);
+#pragma unroll
+    for (int i = 0; i < WM; ++i) xs[i] = nx[i];
+#pragma unroll
+    for (int j = 0; j < WN; ++j) ws[j] = nw[j];
+  }
+
+  // Element r of a block is column 8 * (r / 4) + 4 * fh + r % 4 of row fr.  Each wave passes 32 rows of one or
+  // two blocks at a time through its part of LDS and stores whole 16-byte units, 8 of them a row.
+  constexpr int JB = Y::ES == 2 ? 2 : 1, PART = 4096;
+  static_assert(NW * PART <= S * STAGE, "rows of the epilogue in LDS");
+  uint8_t* part = lds + wave * PART;
+  auto store = [&](auto jn, int j0) __attribute__((always_inline)) {
+    constexpr int J = decltype(jn)::value, CH = J * 32 * Y::ES / 16;
+    const int cw = (wn * WN + j0) * 32, nw = n0 + cw;
+#pragma unroll
+    for (int i = 0; i < WM; ++i) {
+      const int mb = tl.m0 + (wm * WM + i) * 32;
+      if (mb >= tl.m1) break;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int c = j * 32 + 8 * b + 4 * fh;
+          f32x4 v = *(const f32x4*)(col_bias + cw + c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] += acc[j0 + j][i][4 * b + k];
+          Y::set4(part + out_place<CH>(fr, c * Y::ES), v);
+        }
+      wave_lds_wait();
+#pragma unroll
+      for (int u = 0; u < CH / 2; ++u) {
+        const int r = u * (64 / CH) + lane / CH, c = lane % CH, col = nw + c * Y::EPU;
+        const u32x4 v = *(const u32x4*)(part + out_place<CH>(r, c * 16));
+        if (mb + r < tl.m1 && col < a.N) Y::set(a.Y + (size_t)(mb + r) * a.ldy, col, a.N, v);
+      }
+      wave_lds_wait();
+    }
+  };
+  __syncthreads();  // every wave has read its last stage
+#pragma unroll
+  for (int j0 = 0; j0 + JB <= WN; j0 += JB) store(std::integral_constant<int, JB>(), j0);
+  if constexpr (WN % JB) store(std::integral_constant<int, WN % JB>(), WN - WN % JB);
+}
+
+template <class Fn>
+int launch(Fn* fn, std::atomic<uint64_t>& done, const MxArgs& a, int bm, int bn, int threads, int lds, hipStream_t s,
+           const char* who) {
+  const int st = lds_attr_once(done, (const void*)fn, lds, who);
+  if (st != TIERMM_OK) return st;
+  const long long tiles = ((a.N + bn - 1ll) / bn) * ((a.M + bm - 1ll) / bm), grid = (tiles + 7) / 8 * 8;
+  if (grid > (1ll << 30)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, tiles);
+  fn<<<(unsigned)grid, threads, lds, s>>>(a);
+  TM_LAUNCH_CHECK(who);
+  return TIERMM_OK;
+}
+
+template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
+int launch_gemm(const MxArgs& a, hipStream_t s, const char* who) {
+  constexpr int XS = XF == MX_E4M3 ? 2 : 1;
+  constexpr int LDS = S * ((BM * XS + BN) * 128 + ((BM + BN) * 8 + 255) / 256 * 256) + BN * 4;
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static std::atomic<uint64_t> done{0};
+  return launch(mx_gemm_kernel<YT, XF, BM, BN, WVM, WVN, S>, done, a, BM, BN, 64 * WVM * WVN, LDS, s, who);
+}
+
+// Few rows: the product is bound by the bytes of W.  A workgroup takes a BM x BN tile; its WVN x WVK waves
+// share the columns and the steps of 128 elements of a stage, which holds KS * 256 elements of every row and
+// their scales.  A ring of S stages keeps S - 1 on their way by global_load_lds; one barrier a stage.
+//
+// Of a 128-byte piece of a row lane group g takes blocks 2g and 2g + 1, one a step (E4M3: what the MFMA
+// wants of them, half a block of each half of the step).
+template <int YT, int XF, int BM, int BN, int WVN, int WVK, int KS, int S>
+__global__ __launch_bounds__(64 * WVN * WVK) void mx_tile_kernel(const MxArgs a) {
+  constexpr int NW = WVN * WVK, MB = BM / 16, NB = BN / WVN / 16, KK = 2 * KS / WVK, XS = XF == MX_E4M3 ? 2 : 1;
+  constexpr int PARTS = kParts<XF, YT>;
+  constexpr int ROWS = BM * XS + BN, SUB = ROWS * 128, CODES = KS * SUB, IC = CODES / 1024 / NW;
+  constexpr int CH = KS / 2, UNITS = CH * (BM + BN), IS = (UNITS + 64 * NW - 1) / (64 * NW), INST = IC + IS;
+  constexpr int STAGE = CODES + UNITS * 16;
+  static_assert(UNITS >= 64, "a load of scales fills its place");
+  static_assert(IC * NW * 1024 == CODES && KK * WVK == 2 * KS && NB * WVN * 16 == BN && KS % 2 == 0, "whole loads, steps and blocks a wave");
+  constexpr int LDO = BN + 4;  // words of a row of sums
+  static_assert(WVK * BM * LDO * 4 <= S * STAGE, "sums in LDS");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Tile tl;
+  if (!find_tile<BM, BN>(a, tl)) return;
+  const int n0 = tl.tn * BN;
+  using Y = Rows<YT>;
+
+  // load u of this wave: eight rows of a sub-stage (x's, its second halves, then W's); from IC on 16 scales of
+  // 64 rows (units past the end: the last 64 again)
+  const uint8_t* src[INST];
+#pragma unroll
+  for (int u = 0; u < IC; ++u) {
+    const int r = (8 * (wave + NW * u) + (lane >> 3)) % ROWS;
+    const uint8_t* row = r < BM * XS ? a.X + (size_t)min(tl.m0 + r % BM, a.M - 1) * a.rbx + r / BM * 128
+                                     : a.W + (size_t)min(n0 + r - BM * XS, a.N - 1) * a.rbw;
+    src[u] = row + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+  }
+  int unit[IS], place[IS];  // which 16 of a row's scales in the stage, and the load's first unit
+#pragma unroll
+  for (int u = 0; u < IS; ++u) {
+    place[u] = min(64 * (wave + NW * u), UNITS - 64);
+    const int i = place[u] + lane, r = i % (BM + BN);
+    unit[u] = i / (BM + BN);
+    src[IC + u] = r < BM ? a.sx + (size_t)min(tl.m0 + r, a.M - 1) * a.sbx : a.sw + (size_t)min(n0 + r - BM, a.N - 1) * a.sbw;
+  }
+  const uint32_t lds0 = lds_addr(lds);
+  const int ns = (a.nk + KS - 1) / KS, last_unit = (a.nk - 1) / 2;
+  int put = 0;
+  auto issue = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < IC; ++u) {
+      const int i = 8 * (wave + NW * u), r = i % ROWS;
+      // sub-stages past the end load the last one again, and are not multiplied
+      const size_t k = (size_t)min(st * KS + i / ROWS, a.nk - 1);
+      const uint32_t to = lds0 + put * STAGE + (wave + NW * u) * 1024;
+      if (r < BM * XS) dma16(src[u] + k * 128 * XS, to);
+      else if (tl.once) dma16_nt(src[u] + k * 128, to);
+      else dma16(src[u] + k * 128, to);
+    }
+#pragma unroll
+    for (int u = 0; u < IS; ++u)
+      dma16(src[IC + u] + (size_t)min(st * CH + unit[u], last_unit) * 16, lds0 + put * STAGE + CODES + 16 * place[u]);
+    put = put + 1 == S ? 0 : put + 1;
+  };
+  static_assert(BM * XS % 8 == 0 && BN % 8 == 0, "a load is of x or of W");
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i)
+    if (i < ns) issue(i);
+
+  f32x4 acc[NB][MB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wn = wave % WVN, wk = wave / WVN, fr = lane & 15, fg = lane >> 4, turn = (fr >> 1) & 7;
+  int get = 0;
+  for (int st = 0; st < ns; ++st) {
+    const int after = ns - 1 - st;  // stages on their way behind this one
+    if (after >= S - 2) vm_wait<(S - 2) * INST>();
+    else wait_stages<S - 3, INST>(after);
+    __syncthreads();  // stage st has landed for every wave, and the one before it is read
+    if (st + S - 1 < ns) issue(st + S - 1);
+    const uint8_t* s = lds + get * STAGE;
+    get = get + 1 == S ? 0 : get + 1;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      const int step = wk * KK + k, sub = step >> 1, h = step & 1;
+      if (st * KS + sub >= a.nk) break;
+      const int wc = ((2 * fg + h) ^ turn) * 16, xc = XS == 2 ? ((4 * (fg >> 1) + 2 * h + (fg & 1)) ^ turn) * 16 : wc;
+      const uint8_t* p = s + sub * SUB + fr * 128;
+      const uint8_t* sc = s + CODES + ((sub >> 1) * (BM + BN) + fr) * 16 + (sub & 1) * 8 + 2 * fg + h;
+      i32x8 xf[MB][PARTS], wf[NB];
+      int xs[MB], ws[NB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const uint8_t* x = p + xc + i * 16 * 128;
+        if constexpr (XS == 1) xf[i][0] = e2m1(*(const i32x4*)x);
+        else xf[i][0] = e4m3(*(const i32x4*)x, *(const i32x4*)(x + BM * 128));
+        xs[i] = sc[i * 256];
+        if constexpr (PARTS == 2) {
+          xf[i][1] = mx_large(xf[i][0]);
+          xf[i][0] ^= xf[i][1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        wf[j] = e2m1(*(const i32x4*)(p + wc + (BM * XS + (wn * NB + j) * 16) * 128));
+        ws[j] = sc[(BM + (wn * NB + j) * 16) * 16];
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) acc[j][i] = mx_mfma16<XF>(wf[j], xf[i][q], acc[j][i], ws[j], xs[i]);
     }
   }
-  if (m >= a.M) return;
-  const int n = n0 + 4 * g;
-  float o[4];
+  __syncthreads();
+  // a lane's sum is columns 4 * fg .. + 3 of row fr of each block
+  float* sums = (float*)lds;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = acc[i] + (a.bias ? a.bias[min(n + i, a.N - 1)] : 0.f);
-  if (n < a.N) Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, min(4, a.N - n));
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      *(f32x4*)(sums + (wk * BM + i * 16 + fr) * LDO + (wn * NB + j) * 16 + 4 * fg) = acc[j][i];
+  __syncthreads();
+  for (int q = tid; q < BM * BN / 4; q += 64 * NW) {
+    const int r = q / (BN / 4), c = q % (BN / 4) * 4, m = tl.m0 + r, n = n0 + c;
+    if (m >= tl.m1 || n >= a.N) continue;
+    f32x4 v = *(const f32x4*)(sums + r * LDO + c);
+#pragma unroll
+    for (int w = 1; w < WVK; ++w) {
+      const f32x4 t = *(const f32x4*)(sums + (w * BM + r) * LDO + c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += t[k];
+    }
+    float o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = v[k] + (a.bias ? a.bias[min(n + k, a.N - 1)] : 0.f);
+    Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, min(4, a.N - n));
+  }
+}
+
+template <int YT, int XF, int BM, int BN, int WVN, int WVK, int KS, int S>
+int launch_tile(const MxArgs& a, hipStream_t s, const char* who) {
+  constexpr int XS = XF == MX_E4M3 ? 2 : 1;
+  constexpr int LDS = S * (KS * (BM * XS + BN) * 128 + KS / 2 * (BM + BN) * 16);
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static std::atomic<uint64_t> done{0};
+  return launch(mx_tile_kernel<YT, XF, BM, BN, WVN, WVK, KS, S>, done, a, BM, BN, 64 * WVN * WVK, LDS, s, who);
+}
+
+// ----------------------------------------------------------------- single tokens
+template <int CTRL>
+__device__ __forceinline__ float add_ror(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// Up to MX rows of x, quantized by each workgroup into LDS while its first weights are on the way.  A wave
+// takes R rows of W in 1 KiB pieces, 16 bytes (a block) a lane, so each load is eight whole lines of one row.
+//
+// The piece is the MFMA's first operand as it comes: lane l = 16 g + i holds "row" i's block of group g, which
+// stands for block 16 g + i of the one row of W.  With x's blocks laid out alike as the second, the diagonal of the
+// 16 x 16 result holds sum_g <W block 16 g + i, x block 16 g + i>, and its trace over all pieces is the product.  The
+// other 240 sums are waste, but the matrix cores have a tenth of the bytes' time to spend, and nothing is unpacked.
+template <int YT, int XT, int XF, int MX, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxArgs a) {
+  // [MX][pieces][XB KiB] codes in the order that lanes read them, then [MX][pieces][64] scales
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int XB = XF == MX_E4M3 ? 2048 : 1024, PARTS = kParts<XF, YT>;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int blocks = a.nk * 8, nc = (blocks + 63) >> 6;
+  uint8_t* xsc = lds + MX * nc * XB;
+  const int n0 = (blockIdx.x * NW + wave) * R;
+  const uint8_t *wp[R], *sp[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    wp[r] = a.W + (size_t)min(n0 + r, a.N - 1) * a.rbw + 16 * lane;
+    sp[r] = a.sw + (size_t)min(n0 + r, a.N - 1) * a.sbw + lane;
+  }
+  constexpr int U = 3;  // pieces in flight
+  i32x4 q[U][R];
+  int qs[U][R];
+  auto load = [&](int u, int c) __attribute__((always_inline)) {
+    const bool in = c * 64 + lane < blocks;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      q[u][r] = in ? __builtin_nontemporal_load((const i32x4*)(wp[r] + ((size_t)c << 10))) : i32x4{0, 0, 0, 0};
+      qs[u][r] = in ? sp[r][(size_t)c << 6] : 0;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < nc) load(u, u);
+
+  using X = Rows<XT>;
+  constexpr int EPU = X::EPU, STEP = 64 * NW * EPU;
+  // (whole pieces: blocks past the row become zeros)
+  for (int k = tid * EPU; k < nc * 2048; k += STEP) {
+    u32x4 xu[MX];
+#pragma unroll
+    for (int m = 0; m < MX; ++m)
+      xu[m] = k < a.K ? X::get(a.X + (size_t)min(m, a.M - 1) * a.rbx, k, a.K) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int m = 0; m < MX; ++m) {
+      float v[EPU];
+      X::widen(xu[m], v);
+      uint32_t top = 0, w[2];
+#pragma unroll
+      for (int i = 0; i < EPU; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      const int byte = mx_scale_of<XF>(mx_block_top<32 / EPU>(top));
+      mx_codes<XF>(v, mx_inverse(byte), w);
+      const int piece = k >> 11, b = (k >> 5) & 63, in = k & 31;
+      uint8_t* to = lds + (m * nc + piece) * XB;
+      if constexpr (XF == MX_E2M1) mx_put<XF, EPU>(to + b * 16, in, w);
+      else mx_put<XF, EPU>(to + (b >> 5) * 1024 + (2 * ((b >> 4) & 1) + (in >> 4)) * 256 + (b & 15) * 16, in & 15, w);
+      if (in == 0) xsc[(m * nc + piece) * 64 + b] = (uint8_t)byte;
+    }
+  }
+  __syncthreads();
+
+  f32x4 acc[MX][R];
+#pragma unroll
+  for (int m = 0; m < MX; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < nc; c0 += U)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u;
+      if (c >= nc) break;
+#pragma unroll
+      for (int m = 0; m < MX; ++m) {
+        const uint8_t* xp = lds + (m * nc + c) * XB + 16 * lane;
+        const int xs = xsc[(m * nc + c) * 64 + lane];
+        i32x8 x[PARTS];
+        if constexpr (XF == MX_E2M1) x[0] = e2m1(*(const i32x4*)xp);
+        else x[0] = e4m3(*(const i32x4*)xp, *(const i32x4*)(xp + 1024));
+        if constexpr (PARTS == 2) {
+          x[1] = mx_large(x[0]);
+          x[0] ^= x[1];
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) acc[m][r] = mx_mfma16<XF>(e2m1(q[u][r]), x[p], acc[m][r], qs[u][r], xs);
+      }
+      if (c + U < nc) load(u, c + U);
+    }
+  using Y = Rows<YT>;
+  const int col = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int m = 0; m < MX; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      // the diagonal: row 4 g + i, column `col`
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v = col == 4 * g + i ? acc[m][r][i] : v;
+      v = add_ror<0x121>(add_ror<0x122>(add_ror<0x124>(add_ror<0x128>(v))));  // row_ror 8, 4, 2, 1
+      v = row_sum4(v);
+      const int n = n0 + r;
+      if (lane == 0 && m < a.M && n < a.N) {
+        const float o[4] = {v + (a.bias ? a.bias[n] : 0.f), 0.f, 0.f, 0.f};
+        Y::put4(a.Y + (size_t)m * a.ldy + (size_t)n * Y::ES, o, 1);
+      }
+    }
+}
+
+template <int YT, int XT, int XF, int MX, int R, int NW>
+int launch_gemv(const MxArgs& a, hipStream_t s, const char* who) {
+  const int nc = (a.nk * 8 + 63) / 64;
+  mx_gemv_kernel<YT, XT, XF, MX, R, NW><<<(a.N + NW * R - 1) / (NW * R), 64 * NW, MX * nc * (XF == MX_E4M3 ? 2112 : 1088), s>>>(a);
+  TM_LAUNCH_CHECK(who);
+  return TIERMM_OK;
+}
+
+// One or two rows of x are quantized by the product's own workgroups: a launch less, and each byte of W in whole
+// lines.
+constexpr int kGemvLds = 60 * 1024;
+bool fuses(int xfmt, int M, int K) {
+  return M <= 2 && M * (long long)((mx_padded(K) + 2047) / 2048) * (xfmt == MX_E4M3 ? 2112 : 1088) <= kGemvLds;
+}
+
+int fused(const MxArgs& a, int xtype, int xfmt, int ytype, hipStream_t s, const char* who) {
+  int st = TIERMM_OK;
+  with_rows(ytype, [&](auto yt) {
+    with_rows(xtype, [&](auto xt) {
+      with_mx(xfmt, [&](auto f) {
+        constexpr int YT = decltype(yt)::value, XT = decltype(xt)::value, XF = decltype(f)::value;
+        auto rows = [&](auto mx) {
+          constexpr int MX = decltype(mx)::value;
+          if (a.N < 5120) st = launch_gemv<YT, XT, XF, MX, 1, 8>(a, s, who);
+          else st = launch_gemv<YT, XT, XF, MX, 2, 16>(a, s, who);
+        };
+        if (a.M == 1) rows(std::integral_constant<int, 1>());
+        else rows(std::integral_constant<int, 2>());
+      });
+    });
+  });
+  return st;
+}
+
+int device_tile() {  // (for measurements)
+  const char* e = getenv("MX_TILE");
+  return e ? atoi(e) : -1;
+}
+
+template <int YT, int XF>
+int launch_picked(int tile, const MxArgs& a, hipStream_t s, const char* who) {
+  if constexpr (XF == MX_E2M1) switch (tile) {
+      case 6: return launch_gemm<YT, XF, 256, 128, 4, 2, 3>(a, s, who);
+      case 7: return launch_gemm<YT, XF, 256, 256, 4, 2, 2>(a, s, who);
+      case 8: return launch_gemm<YT, XF, 256, 320, 4, 2, 2>(a, s, who);
+    }
+  else switch (tile) {
+      case 6: return launch_gemm<YT, XF, 128, 256, 2, 4, 2>(a, s, who);
+      case 7: return launch_gemm<YT, XF, 128, 256, 4, 2, 2>(a, s, who);
+      case 8: return launch_gemm<YT, XF, 128, 320, 4, 2, 2>(a, s, who);
+    }
+  switch (tile) {
+    case 0: return launch_tile<YT, XF, 16, 16, 1, 8, 4, 4>(a, s, who);
+    case 1: return launch_tile<YT, XF, 16, 32, 1, 8, 4, 4>(a, s, who);
+    case 2: return launch_tile<YT, XF, 16, 64, 2, 2, 2, 4>(a, s, who);
+    case 3: return launch_tile<YT, XF, 32, 32, 1, 8, 4, 3>(a, s, who);
+    case 4: return launch_tile<YT, XF, 32, 64, 1, 8, 4, XF == MX_E4M3 ? 2 : 3>(a, s, who);
+    default: return launch_gemm<YT, XF, 128, 128, 2, 4, 3>(a, s, who);
+  }
 }
 
 int gemm(const MxArgs& a, int xfmt, int ytype, hipStream_t s, const char* who) {
+  int tile = device_tile(), st = TIERMM_OK;
+  if (tile < 0) tile = a.M <= 16 ? (a.N <= 4096 ? 0 : 2) : a.M <= 64 ? 4 : a.M < 512 ? 5 : 7;
   with_rows(ytype, [&](auto yt) {
-    with_mx(xfmt, [&](auto f) {
-      mx_simple_kernel<decltype(yt)::value, decltype(f)::value>
-          <<<dim3((a.N + 15) / 16, (a.M + 15) / 16), 64, 0, s>>>(a);
-    });
+    with_mx(xfmt, [&](auto f) { st = launch_picked<decltype(yt)::value, decltype(f)::value>(tile, a, s, who); });
   });
-  TM_LAUNCH_CHECK(who);
-  return TIERMM_OK;
+  return st;
 }
 
 bool misaligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
@@ -247,6 +797,11 @@ int tiermm_mx_linear(const void* x, int xtype, size_t ldx, int xfmt, const void*
   if ((st = check_out(who, Y, ytype, ldy, bias, N)) != TIERMM_OK) return st;
   if ((st = check_mx_rows(who, "weight", MX_E2M1, W, rbw, sw, sbw, K)) != TIERMM_OK) return st;
   if (misaligned(ws, 16)) return set_error(TIERMM_EINVAL, "%s: workspace not 16-byte aligned", who);
+  if (fuses(xfmt, M, K)) {
+    const MxArgs a = {(const uint8_t*)x, nullptr, (const uint8_t*)W, sw, bias, (uint8_t*)Y, ldx * es, 0, rbw, sbw,
+                      ldy * row_elem_bytes(ytype), M, N, K, mx_padded(K) / kMxStep};
+    return fused(a, xtype, xfmt, ytype, (hipStream_t)stream, who);
+  }
   void* w = nullptr;
   if ((st = get_workspace(ws, ws_bytes, tiermm_mx_linear_ws_bytes(xfmt, M, N, K), &w, who)) != TIERMM_OK) return st;
   const size_t rbx = mx_row_bytes(xfmt, K), sbx = mx_scales(K);
