@@ -140,10 +140,23 @@ __device__ __forceinline__ i32x8 e4m3(const i32x4& lo, const i32x4& hi) {
   return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// LDS of a workgroup: S stages of codes, then scales of two stages at a time.  With two stages in the ring a wave has
+// x's scales of both in registers before the next two stages' are asked for; W's have two places.
+template <int XF, int BM, int BN, int S>
+struct GemmLds {
+  static constexpr int STAGE = (BM * (XF == MX_E4M3 ? 2 : 1) + BN) * 128, XP = S == 2 ? 1 : 2;
+  static constexpr int XSC = S * STAGE, WSC = XSC + XP * BM * 16, BIAS = WSC + 2 * BN * 16, AHEAD = BIAS + BN * 4, BYTES = AHEAD + 256;
+  static __device__ __forceinline__ int xscales(int kt) { return XSC + (XP == 2 ? (kt >> 1 & 1) * BM * 16 : 0); }
+  static __device__ __forceinline__ int wscales(int kt) { return WSC + (kt >> 1 & 1) * BN * 16; }
+};
+constexpr int kAhead = 1;  // stages behind the last one asked for
+
 // BM rows of x times BN rows of W by WVM x WVN waves of WM x WN blocks of 32 x 32.
 //
 // A stage is 256 elements: 128 bytes of every row of W and of E2M1 x, two times 128 of E4M3 x (blocks 0-3
-// of a row, then 4-7), and 8 scales of every row; S stages take turns, brought to LDS by global_load_lds.
+// of a row, then 4-7), and 8 scales of every row; S stages take turns, brought to LDS by global_load_lds.  The
+// scales come 16 of a row at a time, with every other stage: each row is a cache line of its own for them, and
+// as words of one stage they took as many lines as the codes (4096 x 5120 x 14336: 168 us).
 // A row's 16-byte chunk c lies at slot c ^ ((row >> 1) & 7), which spreads the 16 rows that one cycle of a
 // fragment read touches over the banks.  A stage is four MFMA steps; the order of a sum's blocks is free, so
 // step kk takes block kk in the lower half of the wave and 4 + kk in the upper, and the four scales that a
@@ -154,16 +167,16 @@ __device__ __forceinline__ i32x8 e4m3(const i32x4& lo, const i32x4& hi) {
 // W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y; rows leave
 // through LDS in 16-byte units.
 template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
-__global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a) {
+__global__ __launch_bounds__(64 * WVM * WVN) __attribute__((amdgpu_waves_per_eu(WVM * WVN / 4))) void mx_gemm_kernel(const MxArgs a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, XS = XF == MX_E4M3 ? 2 : 1, NF = WN + WM * XS;
   constexpr int PARTS = kParts<XF, YT>;
-  constexpr int ROWS = BM * XS + BN, CODES = ROWS * 128, SCALES = (BM + BN) * 8, STAGE = CODES + (SCALES + 255) / 256 * 256;
-  constexpr int IC = CODES / 1024 / NW, IS = (SCALES + 256 * NW - 1) / (256 * NW), INST = IC + IS;
-  static_assert(WM * WVM * 32 == BM && WN * WVN * 32 == BN && IC * NW * 1024 == CODES, "whole blocks and loads a wave");
-  // loads of a stage by the step that issues them: 3 (of the stage before last), 0 and 1
-  constexpr int D0 = (INST + 2) / 3, D1 = (INST - D0 + 1) / 2, D2 = INST - D0 - D1;
+  constexpr int ROWS = BM * XS + BN, STAGE = ROWS * 128;
+  constexpr int IC = STAGE / 1024 / NW, IS = (BM + BN + 64 * NW - 1) / (64 * NW), INST = IC + IS;
+  static_assert(WM * WVM * 32 == BM && WN * WVN * 32 == BN && IC * NW * 1024 == STAGE, "whole blocks and loads a wave");
+  static_assert(BM * XS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0, "a load is of x or of W");
+  using Lds = GemmLds<XF, BM, BN, S>;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  float* col_bias = (float*)(lds + S * STAGE);
+  float* col_bias = (float*)(lds + Lds::BIAS);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Tile tl;
@@ -171,38 +184,58 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
   const int n0 = tl.tn * BN;
   using Y = Rows<YT>;
 
-  // load u of this wave: rows 8 * (wave + NW * u) .. + 7 of the stage (x's, its second halves, then W's);
-  // from IC on words of scales (the first of every row's two, then the second)
-  const uint8_t* src[INST];
-  int place[IS];
+  // load u of this wave: rows 8 * (wave + NW * u) .. + 7 of the stage (x's, its second halves, then W's); from IC on
+  // the scales of 64 rows for two stages.  Offsets from the tile's own first row: launch_gemm() sees that they
+  // fit 32 bits.
+  const uint8_t *X = a.X + (size_t)tl.m0 * a.rbx, *W = a.W + (size_t)n0 * a.rbw;
+  const uint8_t *sx = a.sx + (size_t)tl.m0 * a.sbx, *sw = a.sw + (size_t)n0 * a.sbw;
+  auto xr = [&](int r) { return (uint32_t)min(r, a.M - 1 - tl.m0); };
+  auto wr = [&](int r) { return (uint32_t)min(r, a.N - 1 - n0); };
+  const uint32_t rbx = (uint32_t)a.rbx, rbw = (uint32_t)a.rbw;
+  uint32_t off[INST];
 #pragma unroll
   for (int u = 0; u < IC; ++u) {
     const int r = 8 * (wave + NW * u) + (lane >> 3);
-    const uint8_t* row = r < BM * XS ? a.X + (size_t)min(tl.m0 + r % BM, a.M - 1) * a.rbx + r / BM * 128
-                                     : a.W + (size_t)min(n0 + r - BM * XS, a.N - 1) * a.rbw;
-    src[u] = row + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    off[u] = (u * NW * 8 < BM * XS ? xr(r % BM) * rbx + r / BM * 128 : wr(r - BM * XS) * rbw) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
   }
+  // (groups of 64 rows past the end: the last one again)
+  auto group = [&](int u) { return min(wave + NW * u, (BM + BN) / 64 - 1); };
 #pragma unroll
   for (int u = 0; u < IS; ++u) {
-    // (words past the end: the last ones again)
-    place[u] = min(64 * (wave + NW * u), SCALES / 4 - 64);
-    const int i = place[u] + lane, h = i / (BM + BN), r = i % (BM + BN);
-    src[IC + u] = (r < BM ? a.sx + (size_t)min(tl.m0 + r, a.M - 1) * a.sbx : a.sw + (size_t)min(n0 + r - BM, a.N - 1) * a.sbw) + 4 * h;
+    const int r = 64 * group(u) + lane;
+    off[IC + u] = 64 * group(u) < BM ? xr(r) * (uint32_t)a.sbx : wr(r - BM) * (uint32_t)a.sbw;
   }
   const uint32_t lds0 = lds_addr(lds);
-  auto ring = [](int kt) { return S == 2 ? kt & 1 : S == 4 ? kt & 3 : kt % S; };
+  auto ring = [](int kt) { return S == 2 ? kt & 1 : kt % S; };
   auto issue = [&](int kt, int u) __attribute__((always_inline)) {
-    const uint32_t to = lds0 + ring(kt) * STAGE;
-    if (u < IC) dma16(src[u] + (size_t)kt * (u * NW * 8 < BM * XS ? 128 * XS : 128), to + (wave + NW * u) * 1024);
-    else dma4(src[u] + (size_t)kt * 8, to + CODES + 4 * place[u - IC]);
+    if (u < IC) {
+      const uint8_t* from = u * NW * 8 < BM * XS ? X + (size_t)kt * 128 * XS : W + (size_t)kt * 128;
+      dma16(from, off[u], lds0 + ring(kt) * STAGE + (wave + NW * u) * 1024);
+    } else if (!(kt & 1)) {
+      const int g = group(u - IC);
+      const uint8_t* from = (64 * g < BM ? sx : sw) + (size_t)kt * 8;
+      dma16(from, off[u], lds0 + (64 * g < BM ? Lds::xscales(kt) : Lds::wscales(kt) - BM * 16) + g * 1024);
+    }
   };
-  static_assert(BM * XS % (8 * NW) == 0, "a load is of x or of W for every wave alike");
+  // Lines of a later stage into the L2: this workgroup's share of those that its neighbours read too (an eighth of x's,
+  // a fourth of W's), by a load of one word of each to where nothing is read.
+  constexpr int AX = BM * XS / 8, AW = BN / 4, WX = (AX + 63) / 64;
+  static_assert(WX + (AW + 63) / 64 <= NW, "a line a lane");
+  const bool ahead_x = wave < WX;
+  const int al = ahead_x ? min(tid, AX - 1) * 8 + tl.tn % 8 : min(tid - 64 * WX, AW - 1) * 4 + tl.m0 / BM % 4;
+  const uint32_t ahead_off = ahead_x ? xr(al % BM) * rbx + al / BM * 128 : wr(al) * rbw;
+  auto ahead = [&](int kt) __attribute__((always_inline)) {
+    const size_t k = (size_t)min(kt, a.nk - 1) * 128;
+    dma4(ahead_x ? X + k * XS : W + k, ahead_off, lds0 + Lds::AHEAD);
+  };
 #pragma unroll
   for (int t = 0; t < S - 1; ++t)
     if (t < a.nk) {
 #pragma unroll
       for (int u = 0; u < INST; ++u) issue(t, u);
     }
+#pragma unroll
+  for (int t = 0; t <= kAhead; ++t) ahead(S - 1 + t);
   for (int i = tid; i < BN; i += 64 * NW) col_bias[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.f;
 
   f32x16 acc[WN][WM];
@@ -216,7 +249,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
   const int wm = wave % WVM, wn = wave / WVM, fr = lane & 31, fh = lane >> 5, turn = (fr >> 1) & 7;
   const uint32_t xrow = (uint32_t)(wm * WM * 32 + fr) * 128, wrow = (uint32_t)(BM * XS + wn * WN * 32 + fr) * 128;
   i32x4 xf[2][WM][XS], wf[2][WN];
-  int xs[WM], ws[WN];
+  int xs[WM], ws[WN], xs1[WM] = {};  // scales of this stage, and of x in an odd one behind it
   // fragment v of step kk of stage kt into set f: W's first, those of x, W's others
   auto fragment = [&](int kt, int kk, int f, int v) __attribute__((always_inline)) {
     const uint8_t* s = lds + ring(kt) * STAGE;
@@ -230,15 +263,21 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
     }
   };
   auto scales = [&](int kt, int (&x)[WM], int (&w)[WN]) __attribute__((always_inline)) {
-    const int* s = (const int*)(lds + ring(kt) * STAGE + CODES) + fh * (BM + BN) + fr;
+    const int* px = (const int*)(lds + Lds::xscales(kt)) + (wm * WM * 32 + fr) * 4 + fh;
+    const int* pw = (const int*)(lds + Lds::wscales(kt)) + (wn * WN * 32 + fr) * 4 + 2 * (kt & 1) + fh;
 #pragma unroll
-    for (int i = 0; i < WM; ++i) x[i] = s[(wm * WM + i) * 32];
+    for (int i = 0; i < WM; ++i) {
+      int even = xs1[i], odd = 0;
+      if (!(kt & 1)) even = px[i * 128], odd = px[i * 128 + 2];
+      x[i] = even;
+      xs1[i] = odd;
+    }
 #pragma unroll
-    for (int j = 0; j < WN; ++j) w[j] = s[BM + (wn * WN + j) * 32];
+    for (int j = 0; j < WN; ++j) w[j] = pw[j * 128];
   };
-  // The products of step KK of fragments f, with the fragments (kt, kk) into the other set and loads
-  // u0 .. u0 + n - 1 of stage `dt` between them.
-  auto step = [&](auto kc, int f, int kt, int kk, int dt, int u0, int n) __attribute__((always_inline)) {
+  // The products of step KK of fragments f, with the fragments (kt, kk) into the other set and n loads of stage
+  // `dt` between them.
+  auto step = [&](auto kc, int f, int kt, int kk, int dt, int n) __attribute__((always_inline)) {
     constexpr int KK = decltype(kc)::value, nm = WM * WN;
     i32x8 x[WM][PARTS];
 #pragma unroll
@@ -258,27 +297,35 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
         if (std::max(v * (nm - 2) / NF, 0) == q) fragment(kt, kk, f ^ 1, v);
 #pragma unroll
       for (int d = 0; d < n; ++d)
-        if (std::min(1 + d * (nm - 1) / n, nm - 1) == q && dt < a.nk) issue(dt, u0 + d);
+        if (std::min(1 + d * (nm - 1) / n, nm - 1) == q && dt < a.nk) issue(dt, d);
       const int j = q / WM, i = q % WM;
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) acc[j][i] = mx_mfma32<XF, KK>(e2m1(wf[f][j]), x[i][p], acc[j][i], ws[j], xs[i]);
       // the compiler would sink these products past the loads' branches, all to the end of the loop (no
       // instruction: nothing reads the sum here)
-      asm volatile("" : "+v"(acc[j][i]));
+      if constexpr (NW == 4 && WM * WN >= 8) {  // (four waves: sums in the accumulation registers, as many as there are)
+        if (q < 16) asm volatile("" : "+a"(acc[j][i]));
+        else asm volatile("" : "+v"(acc[j][i]));
+      } else {
+        asm volatile("" : "+v"(acc[j][i]));
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   // waits until stage kt has landed, those up to kt + S - 2 being on their way too
   auto landed = [&](int kt) __attribute__((always_inline)) {
-    const int behind = a.nk - 1 - kt;
-    if (behind >= S - 2) vm_wait<(S - 2) * INST>();
-    else wait_stages<S - 3, INST>(behind);
+    static_assert(S <= 3, "stages that one wait may leave on their way");
+    // (each stage's loads are followed by one of a line ahead)
+    if (S == 2) vm_wait<1>();
+    else if (kt + 1 >= a.nk) vm_wait<2>();
+    else if (kt & 1) vm_wait<INST + 2>();  // an even stage brings scales
+    else vm_wait<IC + 2>();
   };
-  landed(0);
+  vm_wait<0>();
   __syncthreads();
   if (S - 1 < a.nk) {
 #pragma unroll
-    for (int u = 0; u < D0; ++u) issue(S - 1, u);
+    for (int u = 0; u < INST; ++u) issue(S - 1, u);
   }
   scales(0, xs, ws);
   __builtin_amdgcn_sched_barrier(0);  // the first fragments in the loop's own order, one wait for each
@@ -288,15 +335,16 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
     __builtin_amdgcn_sched_barrier(0);
   }
   for (int kt = 0; kt < a.nk; ++kt) {
-    step(std::integral_constant<int, 0>(), 0, kt, 1, kt + S - 1, D0, D1);
-    step(std::integral_constant<int, 1>(), 1, kt, 2, kt + S - 1, D0 + D1, D2);
-    step(std::integral_constant<int, 2>(), 0, kt, 3, 0, 0, 0);
+    step(std::integral_constant<int, 0>(), 0, kt, 1, 0, 0);
+    step(std::integral_constant<int, 1>(), 1, kt, 2, 0, 0);
+    ahead(kt + S + kAhead);
+    step(std::integral_constant<int, 2>(), 0, kt, 3, 0, 0);
     landed(kt + 1);
     __syncthreads();  // stage kt + 1 has landed for every wave, and stage kt is read
     // (past the end: the fragments of what the place holds, which nothing uses)
     int nx[WM], nw[WN];
     scales(kt + 1, nx, nw);
-    step(std::integral_constant<int, 3>(), 1, kt + 1, 0, kt + S, 0, D0);
+    step(std::integral_constant<int, 3>(), 1, kt + 1, 0, kt + S, INST);
 #pragma unroll
     for (int i = 0; i < WM; ++i) xs[i] = nx[i];
 #pragma unroll
@@ -355,8 +403,7 @@ int launch(Fn* fn, std::atomic<uint64_t>& done, const MxArgs& a, int bm, int bn,
 
 template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
 int launch_gemm(const MxArgs& a, hipStream_t s, const char* who) {
-  constexpr int XS = XF == MX_E4M3 ? 2 : 1;
-  constexpr int LDS = S * ((BM * XS + BN) * 128 + ((BM + BN) * 8 + 255) / 256 * 256) + BN * 4;
+  constexpr int LDS = GemmLds<XF, BM, BN, S>::BYTES;
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> done{0};
   return launch(mx_gemm_kernel<YT, XF, BM, BN, WVM, WVN, S>, done, a, BM, BN, 64 * WVM * WVN, LDS, s, who);
@@ -671,6 +718,17 @@ int device_tile() {  // (for measurements)
 
 template <int YT, int XF>
 int launch_picked(int tile, const MxArgs& a, hipStream_t s, const char* who) {
+  if constexpr (YT == QT_BF16 && XF == MX_E2M1) switch (tile) {
+      case 10: return launch_gemm<YT, XF, 256, 192, 4, 2, 2>(a, s, who);
+      case 11: return launch_gemm<YT, XF, 192, 256, 2, 4, 2>(a, s, who);
+      case 12: return launch_gemm<YT, XF, 256, 256, 2, 2, 2>(a, s, who);
+      case 13: return launch_gemm<YT, XF, 256, 320, 2, 2, 2>(a, s, who);
+    }
+  if constexpr (YT == QT_BF16 && XF == MX_E4M3) switch (tile) {
+      case 10: return launch_gemm<YT, XF, 128, 256, 2, 4, 2>(a, s, who);
+      case 11: return launch_gemm<YT, XF, 192, 192, 2, 2, 2>(a, s, who);
+      case 12: return launch_gemm<YT, XF, 128, 320, 2, 2, 2>(a, s, who);
+    }
   if constexpr (XF == MX_E2M1) switch (tile) {
       case 6: return launch_gemm<YT, XF, 256, 128, 4, 2, 3>(a, s, who);
       case 7: return launch_gemm<YT, XF, 256, 256, 4, 2, 2>(a, s, who);

@@ -13,9 +13,14 @@ __device__ __forceinline__ int xcd_share(int bid, int total) {
   return i < each + (x < more) ? x * each + min(x, more) + i : -1;
 }
 
-// 4 bytes per lane from p into LDS at lds_addr + 4 * lane, as dma16 brings 16.
-__device__ __forceinline__ void dma4(const void* p, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p),
+// dma16 from a wave-uniform base and each lane's offset of 32 bits, and 4 bytes a lane in the same way.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base),
+               "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+               : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base),
                "s"(__builtin_amdgcn_readfirstlane(lds_addr))
                : "memory");
 }
