@@ -10,6 +10,7 @@
 // 64 bits for the gate: h is then the same fp32 number whatever exp does in its last bits, and its
 // codes with it.
 #include "tm_i8.h"
+#include "tm_tiles.h"
 
 namespace tiermm {
 namespace {
@@ -22,10 +23,12 @@ struct LayerArgs {
   const int32_t* ids;
   float* h;                          // [P][F]
   uint32_t* top;                     // [P][tiles of F]: largest |h|, as bits
+  uint8_t* hq;                       // [P][padded F] codes of h
+  float* sh;                         // [P]
   float* y;                          // [P][K]
   uint8_t* out;
   size_t rbx, rbg, rbd, ldo;         // bytes
-  int T, topk, P, E, K, F, nk, nf;   // nk, nf: 64-byte steps of x's and h's rows
+  int T, topk, P, E, K, F, nk, nf;   // nk, nf: 128-byte steps of x's and h's rows
   int by_pair;                       // slots are pairs (fewer than experts): the first of an expert's acts
 };
 
@@ -47,105 +50,152 @@ __device__ __forceinline__ int find_pairs(const LayerArgs& a, int slot, int& e, 
   return n;
 }
 
-// Tile of 16 rows of the gate and the same 16 of up, times the expert's tokens, 16 at a time; the
-// four waves share K.
-__global__ __launch_bounds__(256) void moe_gate_up_kernel(const LayerArgs a) {
+constexpr int kCols = 64;           // rows of W that a workgroup takes: 32 of the gate and the same 32 of up, or 64 of down
+constexpr int kHalf = kCols / 2;
+
+// An expert's tokens, BM at a time, times 64 rows of its weight.  DOWN false: 32 rows of the gate and the same of up, x
+// the tokens' codes, h out.  DOWN true: x the codes of h, the pairs' fp32 products out.
+//
+// Bound by the weights' bytes: a ring of S stages of 256 bytes of every row (x's, then W's) keeps S - 1 on their way by
+// global_load_lds, whole lines of eight rows a load; the four waves share the columns and the 64-byte steps, one barrier
+// a stage.  An expert of more than BM pairs goes through its weights again, out of the caches.
+template <int BM, int S, bool DOWN>
+__global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
+  constexpr int MB = BM / 16, ROWS = BM + kCols, SUB = ROWS * kStep, STAGE = 2 * SUB, INST = STAGE / 1024 / 4, LDO = kCols + 4;
+  static_assert(INST * 4 * 1024 == STAGE && 2 * BM * LDO * 4 <= S * STAGE, "whole loads a wave, sums in LDS");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ uint16_t list[kPairs];
-  __shared__ __attribute__((aligned(16))) int32_t sums[4][2][16][20];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int e;
   const int n = find_pairs(a, blockIdx.y, e, list);
   if (n == 0) return;
-  const int f0 = blockIdx.x * 16, fr = min(f0 + r, a.F - 1);
-  const uint8_t* wg = a.Wg + ((size_t)e * 2 * a.F + fr) * a.rbg + 16 * g;
-  const uint8_t* wu = wg + (size_t)a.F * a.rbg;
+  const int n0 = blockIdx.x * (DOWN ? kCols : kHalf), N = DOWN ? a.K : a.F, nk = DOWN ? a.nf : a.nk;
+  const size_t rbw = DOWN ? a.rbd : a.rbg, rbx = DOWN ? (size_t)a.nf * kStep : a.rbx;
+  const uint8_t* W = DOWN ? a.Wd + (size_t)e * a.K * rbw : a.Wg + (size_t)e * 2 * a.F * rbw;
+  auto w_row = [&](int r) { return DOWN ? min(n0 + r, N - 1) : (r < kHalf ? 0 : N) + min(n0 + r % kHalf, N - 1); };
+  const uint32_t lds0 = lds_addr(lds);
+  const int ns = (nk + 1) / 2, wn = wave & 1, wk = wave >> 1, fr = lane & 15, fg = lane >> 4, turn = (fr >> 1) & 7;
   __syncthreads();
-  const int s0 = a.nk * wave / 4, s1 = a.nk * (wave + 1) / 4;
-  for (int base = 0; base < n; base += 16) {
-    const uint8_t* x = a.X + (size_t)(list[min(base + r, n - 1)] / a.topk) * a.rbx + 16 * g;
-    i32x4 ag = {0, 0, 0, 0}, au = {0, 0, 0, 0};
-    for (int s = s0; s < s1; ++s) {
-      const i32x4 b = *(const i32x4*)(x + (size_t)s * 64);
-      ag = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(wg + (size_t)s * 64), b, ag, 0, 0, 0);
-      au = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(wu + (size_t)s * 64), b, au, 0, 0, 0);
-    }
-    *(i32x4*)&sums[wave][0][r][4 * g] = ag;
-    *(i32x4*)&sums[wave][1][r][4 * g] = au;
-    __syncthreads();
-    const int c = tid >> 4, f = tid & 15;
-    int sg = 0, su = 0;
+  for (int base = 0; base < n; base += BM) {
+    // load u of this wave: eight rows of a half stage
+    const uint8_t* src[INST];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      sg += sums[w][0][c][f];
-      su += sums[w][1][c][f];
+    for (int u = 0; u < INST; ++u) {
+      const int r = (8 * (wave + 4 * u) + (lane >> 3)) % ROWS;
+      const int p = list[min(base + r, n - 1)];  // (of a row of W: not used)
+      src[u] = (r < BM ? (DOWN ? a.hq : a.X) + (size_t)(DOWN ? p : p / a.topk) * rbx : W + (size_t)w_row(r - BM) * rbw) +
+               ((lane & 7) ^ ((r >> 1) & 7)) * 16;
     }
-    if (base + c < n) {
-      const int p = list[base + c];
-      uint32_t top = 0;
-      if (f0 + f < a.F) {
-        const size_t ch = (size_t)e * 2 * a.F + f0 + f;
-        const float sx = a.sx[p / a.topk];
-        const double gate = scaled(sg, sx, a.sg[ch], 0.f), up = scaled(su, sx, a.sg[ch + a.F], 0.f);
-        const float h = (float)(gate / (1. + exp(-gate)) * up);
-        a.h[(size_t)p * a.F + f0 + f] = h;
-        top = __float_as_uint(h) & 0x7fffffffu;
+    int put = 0;
+    auto issue = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < INST; ++u) {
+        const int i = 8 * (wave + 4 * u), r = i % ROWS;
+        const size_t k = (size_t)min(2 * st + i / ROWS, nk - 1) * kStep;  // (past the end: not multiplied)
+        const uint32_t to = lds0 + put * STAGE + (wave + 4 * u) * 1024;
+        if (r >= BM && n <= BM) dma16_nt(src[u] + k, to);
+        else dma16(src[u] + k, to);
       }
+      put = put + 1 == S ? 0 : put + 1;
+    };
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 16));
-      if (f == 0) a.top[(size_t)p * gridDim.x + blockIdx.x] = top;
+    for (int i = 0; i < S - 1; ++i)
+      if (i < ns) issue(i);
+    i32x4 acc[2][MB] = {};
+    int get = 0;
+    for (int st = 0; st < ns; ++st) {
+      const int after = ns - 1 - st;  // stages on their way behind this one
+      if (after >= S - 2) vm_wait<(S - 2) * INST>();
+      else wait_stages<S - 3, INST>(after);
+      __syncthreads();  // stage st has landed for every wave, and the one before it is read
+      if (st + S - 1 < ns) issue(st + S - 1);
+      const uint8_t* s = lds + get * STAGE + wk * SUB;
+      get = get + 1 == S ? 0 : get + 1;
+      if (2 * st + wk >= nk) continue;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint8_t* p = s + fr * kStep + ((4 * k + fg) ^ turn) * 16;
+        i32x4 xf[MB], wf[2];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) xf[i] = *(const i32x4*)(p + i * 16 * kStep);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) wf[j] = *(const i32x4*)(p + (BM + wn * kHalf + j * 16) * kStep);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+      }
+    }
+    __syncthreads();
+    // a lane's sum is columns 4 * fg .. + 3 of row fr of each block
+    int32_t* sums = (int32_t*)lds;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) *(i32x4*)(sums + (wk * BM + i * 16 + fr) * LDO + wn * kHalf + j * 16 + 4 * fg) = acc[j][i];
+    __syncthreads();
+    if constexpr (DOWN) {
+      for (int q = tid; q < BM * kCols; q += 256) {
+        const int r = q / kCols, c = q % kCols;
+        if (base + r >= n || n0 + c >= N) continue;
+        const int p = list[base + r], sum = sums[r * LDO + c] + sums[(BM + r) * LDO + c];
+        a.y[(size_t)p * a.K + n0 + c] = scaled(sum, a.sh[p], a.sd[(size_t)e * a.K + n0 + c], 0.f);
+      }
+    } else {
+      for (int q = tid; q < BM * kHalf; q += 256) {
+        const int r = q / kHalf, c = q % kHalf, p = list[min(base + r, n - 1)];
+        const bool live = base + r < n;
+        uint32_t top = 0;
+        if (live && n0 + c < N) {
+          const int32_t* g = sums + r * LDO + c;
+          const size_t ch = (size_t)e * 2 * N + n0 + c;
+          const float sx = a.sx[p / a.topk];
+          const double gate = scaled(g[0] + g[BM * LDO], sx, a.sg[ch], 0.f);
+          const double up = scaled(g[kHalf] + g[BM * LDO + kHalf], sx, a.sg[ch + N], 0.f);
+          const float h = (float)(gate / (1. + exp(-gate)) * up);
+          a.h[(size_t)p * N + n0 + c] = h;
+          top = __float_as_uint(h) & 0x7fffffffu;
+        }
+#pragma unroll
+        for (int o = kHalf / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kHalf));
+        if (c == 0 && live) a.top[(size_t)p * gridDim.x + blockIdx.x] = top;
+      }
     }
     __syncthreads();
   }
 }
 
-// Tile of 16 rows of the down weight times the codes of h's rows, which each wave makes of its own
-// share of K.
-__global__ __launch_bounds__(256) void moe_down_kernel(const LayerArgs a) {
-  __shared__ uint16_t list[kPairs];
-  __shared__ __attribute__((aligned(16))) int32_t sums[4][16][20];
-  __shared__ RowScale scale[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-  int e;
-  const int n = find_pairs(a, blockIdx.y, e, list);
-  if (n == 0) return;
-  const int k0 = blockIdx.x * 16, kr = min(k0 + r, a.K - 1), nt = (a.F + 15) / 16;
-  const uint8_t* w = a.Wd + ((size_t)e * a.K + kr) * a.rbd + 16 * g;
+// Codes and scale of a pair's row of h.
+__global__ __launch_bounds__(256) void moe_codes_kernel(const LayerArgs a) {
+  __shared__ uint32_t red[4];
+  const int p = blockIdx.x, tid = threadIdx.x, nt = (a.F + kHalf - 1) / kHalf, Fp = a.nf * kStep;
+  if ((uint32_t)a.ids[p] >= (uint32_t)a.E) return;
+  uint32_t top = 0;
+  for (int i = tid; i < nt; i += 256) top = max(top, a.top[(size_t)p * nt + i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
-  const int s0 = a.nf * wave / 4, s1 = a.nf * (wave + 1) / 4;
-  for (int base = 0; base < n; base += 16) {
-    const int c = tid >> 4, i0 = tid & 15;
-    uint32_t top = 0;
-    for (int i = i0; i < nt; i += 16) top = max(top, a.top[(size_t)list[min(base + c, n - 1)] * nt + i]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 16));
-    if (i0 == 0) scale[c] = row_scale_of(top);
-    __syncthreads();
-    const RowScale rs = scale[r];
-    const float* h = a.h + (size_t)list[min(base + r, n - 1)] * a.F;
-    i32x4 acc = {0, 0, 0, 0};
-    for (int s = s0; s < s1; ++s) {
-      i32x4 b;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int f = s * 64 + 16 * g + 4 * q + i;
-          v[i] = f < a.F ? h[f] : 0.f;
-        }
-        b[q] = (int)codes4(v, rs);
-      }
-      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(w + (size_t)s * 64), b, acc, 0, 0, 0);
-    }
-    *(i32x4*)&sums[wave][r][4 * g] = acc;
-    __syncthreads();
-    int sum = 0;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) sum += sums[v][c][i0];
-    if (base + c < n && k0 + i0 < a.K)
-      a.y[(size_t)list[base + c] * a.K + k0 + i0] = scaled(sum, scale[c].sc, a.sd[(size_t)e * a.K + k0 + i0], 0.f);
-    __syncthreads();
+  const RowScale rs = row_scale_of(max(max(red[0], red[1]), max(red[2], red[3])));
+  const uint8_t* h = (const uint8_t*)(a.h + (size_t)p * a.F);
+  for (int f = (blockIdx.y * 256 + tid) * 4; f < Fp; f += gridDim.y * 1024) {
+    float v[4];
+    Rows<QT_F32>::widen(f < a.F ? Rows<QT_F32>::get(h, f, a.F) : u32x4{0u, 0u, 0u, 0u}, v);
+    *(uint32_t*)(a.hq + (size_t)p * Fp + f) = codes4(v, rs);
   }
+  if (blockIdx.y == 0 && tid == 0) a.sh[p] = rs.sc;
+}
+
+template <int BM, int S, bool DOWN>
+int launch_experts(const LayerArgs& a, int slots, hipStream_t s, const char* who) {
+  constexpr int LDS = S * 2 * (BM + kCols) * kStep;
+  static std::atomic<uint64_t> done{0};
+  const int st = lds_attr_once(done, (const void*)moe_experts_kernel<BM, S, DOWN>, LDS, who);
+  if (st != TIERMM_OK) return st;
+  const int n = DOWN ? kCols : kHalf;
+  moe_experts_kernel<BM, S, DOWN><<<dim3(((DOWN ? a.K : a.F) + n - 1) / n, slots), 256, LDS, s>>>(a);
+  TM_LAUNCH_CHECK(who);
+  return TIERMM_OK;
 }
 
 // out[t] = sum_j weights[t][j] y[t][j], dropped pairs skipped.
@@ -177,7 +227,7 @@ extern "C" {
 size_t tiermm_moe_i8_layer_ws_bytes(int T, int topk, int K, int F) {
   if (T < 1 || topk < 1 || K < 1 || F < 1 || T > kTokens || topk > kTopk || K > kMaxK || F > kMaxK) return 0;
   const size_t P = (size_t)T * topk;
-  return align16(P * F * 4) + align16(P * K * 4) + align16(P * ((F + 15) / 16) * 4);
+  return align16(P * F * 4) + align16(P * K * 4) + align16(P * ((F + kHalf - 1) / kHalf) * 4) + P * padded(F) + align16(P * 4);
 }
 
 int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int32_t* expert_ids, const float* weights,
@@ -205,23 +255,34 @@ int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int
   if (misaligned(sx, 4) || misaligned(expert_ids, 4) || misaligned(weights, 4) || misaligned(sgu, 4) || misaligned(sd, 4))
     return set_error(TIERMM_EINVAL, "%s: misaligned table", who);
   if (misaligned(ws, 16)) return set_error(TIERMM_EINVAL, "%s: workspace not 16-byte aligned", who);
-  const int P = T * topk, nt = (F + 15) / 16;
+  const int P = T * topk;
   void* w = nullptr;
-  const int st = get_workspace(ws, ws_bytes, tiermm_moe_i8_layer_ws_bytes(T, topk, K, F), &w, who);
+  int st = get_workspace(ws, ws_bytes, tiermm_moe_i8_layer_ws_bytes(T, topk, K, F), &w, who);
   if (st != TIERMM_OK) return st;
-  float* h = (float*)w;
-  float* y = (float*)((uint8_t*)w + align16((size_t)P * F * 4));
-  uint32_t* top = (uint32_t*)((uint8_t*)y + align16((size_t)P * K * 4));
-  const LayerArgs a = {(const uint8_t*)Xq, (const uint8_t*)Wgu, (const uint8_t*)Wd, sx, sgu, sd, weights, expert_ids, h, top, y,
-                       (uint8_t*)out, rbx, rbg, rbd, ldo * es, T, topk, P, n_experts, K, F, padded(K) / 64, padded(F) / 64,
+  uint8_t* at = (uint8_t*)w;
+  auto part = [&](size_t bytes) {
+    uint8_t* p = at;
+    at += align16(bytes);
+    return p;
+  };
+  float* h = (float*)part((size_t)P * F * 4);
+  float* y = (float*)part((size_t)P * K * 4);
+  uint32_t* top = (uint32_t*)part((size_t)P * ((F + kHalf - 1) / kHalf) * 4);
+  uint8_t* hq = part((size_t)P * padded(F));
+  float* sh = (float*)part((size_t)P * 4);
+  const LayerArgs a = {(const uint8_t*)Xq, (const uint8_t*)Wgu, (const uint8_t*)Wd, sx, sgu, sd, weights, expert_ids, h, top, hq, sh,
+                       y, (uint8_t*)out, rbx, rbg, rbd, ldo * es, T, topk, P, n_experts, K, F, padded(K) / kStep, padded(F) / kStep,
                        P < n_experts};
   hipStream_t s = (hipStream_t)stream;
   if (P) {
     const int slots = P < n_experts ? P : n_experts;
-    moe_gate_up_kernel<<<dim3(nt, slots), 256, 0, s>>>(a);
-    TM_LAUNCH_CHECK("tiermm_moe_i8_layer: gate and up");
-    moe_down_kernel<<<dim3((K + 15) / 16, slots), 256, 0, s>>>(a);
-    TM_LAUNCH_CHECK("tiermm_moe_i8_layer: down");
+    const bool wide = P > 10 * n_experts;
+    st = wide ? launch_experts<32, 3, false>(a, slots, s, who) : launch_experts<16, 4, false>(a, slots, s, who);
+    if (st != TIERMM_OK) return st;
+    moe_codes_kernel<<<dim3(P, (padded(F) + 4095) / 4096), 256, 0, s>>>(a);
+    TM_LAUNCH_CHECK(who);
+    st = wide ? launch_experts<32, 3, true>(a, slots, s, who) : launch_experts<16, 4, true>(a, slots, s, who);
+    if (st != TIERMM_OK) return st;
   }
   with_rows(otype, [&](auto yt) {
     moe_layer_sum_kernel<decltype(yt)::value><<<dim3(T, (K + 1023) / 1024), 256, 0, s>>>(a);
