@@ -10,9 +10,9 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 namespace tiermm {
+int device_cus(int* cus);
 namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -167,7 +167,7 @@ constexpr int kAhead = 1;  // stages behind the last one asked for
 // W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y; rows leave
 // through LDS in 16-byte units.
 template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
-__global__ __launch_bounds__(64 * WVM * WVN) __attribute__((amdgpu_waves_per_eu(WVM * WVN / 4))) void mx_gemm_kernel(const MxArgs a) {
+__global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, XS = XF == MX_E4M3 ? 2 : 1, NF = WN + WM * XS;
   constexpr int PARTS = kParts<XF, YT>;
   constexpr int ROWS = BM * XS + BN, STAGE = ROWS * 128;
@@ -303,12 +303,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) __attribute__((amdgpu_waves_per_eu(
       for (int p = 0; p < PARTS; ++p) acc[j][i] = mx_mfma32<XF, KK>(e2m1(wf[f][j]), x[i][p], acc[j][i], ws[j], xs[i]);
       // the compiler would sink these products past the loads' branches, all to the end of the loop (no
       // instruction: nothing reads the sum here)
-      if constexpr (NW == 4 && WM * WN >= 8) {  // (four waves: sums in the accumulation registers, as many as there are)
-        if (q < 16) asm volatile("" : "+a"(acc[j][i]));
-        else asm volatile("" : "+v"(acc[j][i]));
-      } else {
-        asm volatile("" : "+v"(acc[j][i]));
-      }
+      asm volatile("" : "+v"(acc[j][i]));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -711,49 +706,72 @@ int fused(const MxArgs& a, int xtype, int xfmt, int ytype, hipStream_t s, const 
   return st;
 }
 
-int device_tile() {  // (for measurements)
-  const char* e = getenv("MX_TILE");
-  return e ? atoi(e) : -1;
+// The tiles, and what one costs: a call takes about t0 + n * (fix + K / 1024 * each) us, n the tiles that the fullest
+// CU runs.  Fitted to measured times of 192 sizes (4 to 4096 rows, 512 to 28672 columns, K of 1024 to 14336), on
+// weights that the last-level cache holds where they fit; the tile with the least such time is within 0.4 % of the
+// best of its list in the mean, 18 % at worst.  E4M3 x has lists of its own, for x as it is and in two parts.  Example,
+// 5120 columns and rows of 5120, E2M1, us: 16 rows 16 x 32 tiles 6.3, 64 x 128 12.4, 128 x 128 16.0; 256 rows 64 x 128
+// 14.1, 128 x 128 18.7, 32 x 64 20.4; 4096 rows 256 x 320 59.6, 256 x 192 70.3, 128 x 128 95.8.
+struct TileCost {
+  int bm, bn;
+  float t0, fix, each;
+};
+constexpr TileCost kE2m1Tiles[] = {
+    {16, 16, 2.51f, 0.62f, 0.26f}, {16, 32, 1.65f, 1.70f, 0.43f}, {16, 64, 1.49f, 1.43f, 1.09f}, {32, 32, 1.59f, 1.65f, 0.54f},
+    {32, 64, 1.20f, 2.49f, 0.79f}, {64, 128, 2.09f, 0.81f, 2.04f}, {128, 128, 0.f, 3.21f, 2.91f}, {256, 128, 0.f, 4.58f, 3.95f},
+    {256, 192, 0.f, 4.98f, 4.84f}, {256, 256, 0.f, 5.93f, 5.39f}, {256, 320, 0.f, 6.89f, 6.61f},
+};
+constexpr TileCost kE4m3Tiles[] = {
+    {16, 16, 1.61f, 1.64f, 0.39f}, {16, 32, 1.73f, 1.51f, 0.53f}, {16, 64, 1.47f, 1.62f, 1.21f}, {32, 32, 1.22f, 2.29f, 0.68f},
+    {32, 64, 1.14f, 2.31f, 1.16f}, {64, 128, 0.47f, 2.41f, 2.51f}, {128, 128, 0.f, 3.37f, 3.97f}, {128, 192, 0.f, 3.48f, 4.85f},
+    {128, 256, 0.f, 4.18f, 5.60f}, {128, 320, 0.f, 5.16f, 6.19f},
+};
+constexpr TileCost kE4m3PartTiles[] = {
+    {16, 16, 1.51f, 1.67f, 0.52f}, {16, 32, 1.63f, 1.53f, 0.66f}, {16, 64, 1.39f, 1.75f, 1.62f}, {32, 32, 1.22f, 2.32f, 0.97f},
+    {32, 64, 1.11f, 2.50f, 1.36f}, {64, 128, 0.19f, 3.28f, 4.70f}, {128, 128, 0.f, 4.52f, 8.03f}, {128, 192, 0.f, 5.50f, 7.41f},
+    {128, 256, 0.f, 6.47f, 9.31f}, {128, 320, 0.f, 7.37f, 10.8f},
+};
+constexpr int kTileKernels = 5;  // the first ones, of mx_tile_kernel
+
+template <int N>
+int pick_of(const TileCost (&tiles)[N], const MxArgs& a, int cus) {
+  int best = 0;
+  float least = 1e30f;
+  for (int i = 0; i < N; ++i) {
+    const TileCost& c = tiles[i];
+    // mx_gemm_kernel's offsets from a tile's first row have 32 bits
+    if (i >= kTileKernels && std::max(a.rbx * c.bm, a.rbw * c.bn) + std::max(a.sbx * c.bm, a.sbw * c.bn) >= (1ull << 32)) continue;
+    const float n = std::ceil(std::ceil((float)a.M / c.bm) * ((a.N + c.bn - 1) / c.bn) / cus);
+    const float t = c.t0 + n * (c.fix + a.nk * (kMxStep / 1024.f) * c.each);
+    if (t < least) least = t, best = i;
+  }
+  return best;
 }
 
 template <int YT, int XF>
-int launch_picked(int tile, const MxArgs& a, hipStream_t s, const char* who) {
-  if constexpr (YT == QT_BF16 && XF == MX_E2M1) switch (tile) {
-      case 10: return launch_gemm<YT, XF, 256, 192, 4, 2, 2>(a, s, who);
-      case 11: return launch_gemm<YT, XF, 192, 256, 2, 4, 2>(a, s, who);
-      case 12: return launch_gemm<YT, XF, 256, 256, 2, 2, 2>(a, s, who);
-      case 13: return launch_gemm<YT, XF, 256, 320, 2, 2, 2>(a, s, who);
-    }
-  if constexpr (YT == QT_BF16 && XF == MX_E4M3) switch (tile) {
-      case 10: return launch_gemm<YT, XF, 128, 256, 2, 4, 2>(a, s, who);
-      case 11: return launch_gemm<YT, XF, 192, 192, 2, 2, 2>(a, s, who);
-      case 12: return launch_gemm<YT, XF, 128, 320, 2, 2, 2>(a, s, who);
-    }
-  if constexpr (XF == MX_E2M1) switch (tile) {
-      case 6: return launch_gemm<YT, XF, 256, 128, 4, 2, 3>(a, s, who);
-      case 7: return launch_gemm<YT, XF, 256, 256, 4, 2, 2>(a, s, who);
-      case 8: return launch_gemm<YT, XF, 256, 320, 4, 2, 2>(a, s, who);
-    }
-  else switch (tile) {
-      case 6: return launch_gemm<YT, XF, 128, 256, 2, 4, 2>(a, s, who);
-      case 7: return launch_gemm<YT, XF, 128, 256, 4, 2, 2>(a, s, who);
-      case 8: return launch_gemm<YT, XF, 128, 320, 4, 2, 2>(a, s, who);
-    }
+int launch_picked(const MxArgs& a, int cus, hipStream_t s, const char* who) {
+  constexpr bool E4 = XF == MX_E4M3;
+  const int tile = !E4 ? pick_of(kE2m1Tiles, a, cus) : kParts<XF, YT> == 1 ? pick_of(kE4m3Tiles, a, cus) : pick_of(kE4m3PartTiles, a, cus);
   switch (tile) {
     case 0: return launch_tile<YT, XF, 16, 16, 1, 8, 4, 4>(a, s, who);
     case 1: return launch_tile<YT, XF, 16, 32, 1, 8, 4, 4>(a, s, who);
     case 2: return launch_tile<YT, XF, 16, 64, 2, 2, 2, 4>(a, s, who);
     case 3: return launch_tile<YT, XF, 32, 32, 1, 8, 4, 3>(a, s, who);
-    case 4: return launch_tile<YT, XF, 32, 64, 1, 8, 4, XF == MX_E4M3 ? 2 : 3>(a, s, who);
-    default: return launch_gemm<YT, XF, 128, 128, 2, 4, 3>(a, s, who);
+    case 4: return launch_tile<YT, XF, 32, 64, 1, 8, 4, E4 ? 2 : 3>(a, s, who);
+    case 5: return launch_gemm<YT, XF, 64, 128, 2, 4, 3>(a, s, who);
+    case 6: return launch_gemm<YT, XF, 128, 128, 2, 4, 3>(a, s, who);
+    case 7: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 192 : 128, 4, 2, E4 ? 2 : 3>(a, s, who);
+    case 8: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 256 : 192, 4, 2, 2>(a, s, who);
+    case 9: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 320 : 256, 4, 2, 2>(a, s, who);
+    default: return launch_gemm<YT, XF, E4 ? 128 : 256, 320, 4, 2, 2>(a, s, who);
   }
 }
 
 int gemm(const MxArgs& a, int xfmt, int ytype, hipStream_t s, const char* who) {
-  int tile = device_tile(), st = TIERMM_OK;
-  if (tile < 0) tile = a.M <= 16 ? (a.N <= 4096 ? 0 : 2) : a.M <= 64 ? 4 : a.M < 512 ? 5 : 7;
+  int cus = 0, st = device_cus(&cus);
+  if (st != TIERMM_OK) return st;
   with_rows(ytype, [&](auto yt) {
-    with_mx(xfmt, [&](auto f) { st = launch_picked<decltype(yt)::value, decltype(f)::value>(tile, a, s, who); });
+    with_mx(xfmt, [&](auto f) { st = launch_picked<decltype(yt)::value, decltype(f)::value>(a, cus, s, who); });
   });
   return st;
 }
