@@ -157,6 +157,18 @@ def test_far_rows(gpu):
     assert np.array_equal(np.concatenate(alone), Y.bits())  # no token depends on the others, bit for bit
 
 
+def test_results_do_not_depend_on_the_call(gpu):
+    """64 tokens at once, and the same in calls of 1, 5 and 33: bit for bit."""
+    E, K, F, k = 9, 260, 200, 4
+    ex = Experts(E, K, F, 70)
+    q, sx = tokens(64, K, 71)
+    ids, w = routes(64, k, E, 72)
+    whole = run(ex, q, sx, ids, w).bits()
+    for n in (1, 5, 33):
+        parts = [run(ex, q[i:i + n], sx[i:i + n], ids[i:i + n], w[i:i + n]).bits() for i in range(0, 64, n)]
+        assert np.array_equal(np.concatenate(parts), whole), n
+
+
 def test_every_code(gpu):
     """Codes of -127 and 127 everywhere: the largest sums."""
     E, K, F = 2, 1024, 640
@@ -172,7 +184,7 @@ def test_every_code(gpu):
     check(run(ex, q, sx, ids, w), ex, q, sx, ids, w)
 
 
-@pytest.mark.parametrize("T,k,E", [(1, 2, 8), (7, 3, 5)])
+@pytest.mark.parametrize("T,k,E", [(1, 2, 8), (7, 3, 5), (16, 4, 6), (2, 2, 40)])
 def test_captured_follows_the_routing(gpu, T, k, E):
     """Replays of one graph on new routings and rows, its own workspace, eager calls of another between them."""
     K, F, st = 256, 130, hip.Stream()
@@ -212,9 +224,10 @@ def test_captured_follows_the_routing(gpu, T, k, E):
         st.destroy()
 
 
-def test_two_streams(gpu):
+@pytest.mark.parametrize("T,k", [(8, 4), (30, 4), (1, 8)])
+def test_two_streams(gpu, T, k):
     """Two calls at once, each with its own workspace."""
-    T, k, E, K, F = 8, 4, 12, 512, 384
+    E, K, F = 12, 512, 384
     ex, streams = Experts(E, K, F, 40), [hip.Stream(), hip.Stream()]
     n, jobs = tier_amd.moe_i8_layer_ws_bytes(T, k, K, F), []
     for i, st in enumerate(streams):

@@ -171,7 +171,37 @@ def test_codes_do_not_depend_on_the_launch(gpu):
         assert np.array_equal(q, got[0][0]) and s == got[0][1]
 
 
+@pytest.mark.parametrize("t,M,K", [(BF16, 4100, 4701), (F32, 2100, 4704), (F16, 700, 30000)])
+def test_streamed_rows(gpu, t, M, K):
+    """More bytes than the last-level cache keeps: rows past the caches, codes and sums as ever."""
+    X, R, g, H = Rows(t, M, K, rows(M, K, 60)), Rows(t, M, K, rows(M, K, 61)), gains(K), Rows(t, M, K)
+    h, r, y = forward(t, X.values(), R.values(), g)
+    rb = tier_amd.i8_row_bytes(K)
+    Q, S, RS = hip.DeviceBuffer(M * rb), f32(np.zeros(M)), f32(np.zeros(M))
+    tier_amd.rms_norm(X.ptr, t, K, R.ptr, K, f32(g).ptr, EPS, H.ptr, K, None, 0, Q.ptr, rb, S.ptr, RS.ptr, M, K)
+    hip.synchronize()
+    q, s = quantize(y)
+    assert np.array_equal(Q.download(np.int8).reshape(M, rb)[:, :K], q) and np.array_equal(S.download(np.float32), s)
+    assert np.array_equal(H.bits(), to_bits(t, h)) and np.array_equal(RS.download(np.float32), r)
+    DX, DG = Rows(t, M, K), f32(np.zeros(K))
+    tier_amd.rms_norm_grad(X.ptr, t, K, H.ptr, K, f32(g).ptr, RS.ptr, R.ptr, K, DX.ptr, K, DG.ptr, M, K)
+    hip.synchronize()
+    check_grad(DX, DG.download(np.float32), X, H, R, r, g)
+
+
 # -------------------------------------------------------------------- gradient
+def check_grad(DX, got, DY, H, DH, r, g):
+    """dx and dgain within the bound of the header comment."""
+    M, K, t = H.rows, H.cols, H.t
+    dhv, dyv, r64 = None if DH is None else DH.values(), DY.values(), r.astype(np.float64)
+    want, dgain, xh, d, m = grad64(dyv, H.values(), r64, g.astype(np.float64), dhv)
+    off = (64 + 6 + 16 + K / 1024) * U * np.abs(d * xh).mean(1, keepdims=True)
+    err = 8 * U * (r64[:, None] * (np.abs(d) + np.abs(xh * m)) + (0 if dhv is None else np.abs(dhv))) + r64[:, None] * np.abs(xh) * off
+    ok = np.abs(DX.values() - want) <= err + UNIT[t] * (np.abs(want) + err) + TINY[t]
+    assert ok.all(), np.argwhere(~ok)[:5]
+    assert (np.abs(got[:K] - dgain) <= (M + 64) * U * np.abs(dyv * xh).sum(0) + 1e-38).all()
+
+
 def grad64(dy, h, r, g, dh):
     xh, d = h * r[:, None], dy * g
     m = (d * xh).mean(1, keepdims=True)
@@ -192,15 +222,9 @@ def test_gradient(gpu, t, M, K, pad, skip):
         tier_amd.rms_norm_grad(DY.ptr, t, DY.ld, H.ptr, H.ld, f32(g).ptr, f32(r).ptr, dh and dh.ptr, DH.ld, DX.ptr, DX.ld,
                                DG.ptr, M, K, ws.ptr if own_ws else None, n if own_ws else 0)
         hip.synchronize()
-        r64, g64 = r.astype(np.float64), g.astype(np.float64)
-        dhv = None if dh is None else dh.values()
-        want, dgain, xh, d, m = grad64(DY.values(), H.values(), r64, g64, dhv)
-        off = (64 + 6 + 16 + K / 1024) * U * np.abs(d * xh).mean(1, keepdims=True)
-        err = 8 * U * (r64[:, None] * (np.abs(d) + np.abs(xh * m)) + (0 if dhv is None else np.abs(dhv))) + r64[:, None] * np.abs(xh) * off
-        ok = np.abs(DX.values() - want) <= err + UNIT[t] * (np.abs(want) + err) + TINY[t]
-        assert ok.all(), np.argwhere(~ok)[:5]
         got = DG.download(np.float32)
-        assert (np.abs(got[:K] - dgain) <= (M + 64) * U * np.abs(DY.values() * xh).sum(0) + 1e-38).all() and got[K] == 5
+        check_grad(DX, got, DY, H, dh, r, g)
+        assert got[K] == 5
         assert DX.outside_kept() and (ws.download(np.uint8)[n:] == 0x55).all()
         # without dgain: the same dx, no workspace
         D2 = Rows(t, M, K)

@@ -96,8 +96,8 @@ constexpr int kParts = XF == MX_E4M3 && YT == QT_F32 ? 2 : 1;
 
 // The codes of magnitude 2 and more, whose bit 6 is set, and zeros.
 __device__ __forceinline__ uint32_t mx_large(uint32_t c) {
-  const uint32_t bit = c & 0x40404040u, top = bit << 1;
-  return c & (top | (top - (bit >> 6)));
+  const uint32_t one = (c & 0x40404040u) >> 6;
+  return c & ((one << 8) - one);
 }
 __device__ __forceinline__ i32x8 mx_large(const i32x8& x) {
   i32x8 y;

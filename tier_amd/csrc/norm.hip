@@ -61,16 +61,23 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// One row a workgroup of NT threads.  R > 0: the row has at most R * NT units of 16 bytes and stays
-// in registers, all its loads on their way at once; R = 0: any row, read again from h (or x and
-// the residual) for each pass.
-template <int XT, int Q, int NT, int R>
-__global__ __launch_bounds__(NT) void norm_kernel(const NormArgs a) {
+// One row a workgroup.  R > 0: the row has at most R units of 16 bytes a thread and stays in
+// registers, all its loads on their way at once; R = 0: any row, read again from h (or x and
+// the residual) for each pass.  STREAM: rows come from past the caches, and h goes there.
+//
+// Bound by memory: 4096 x 5120 bf16 with a residual, int8 out, 28.0 us (5.2 TB/s, where a large copy moves 4.8), through
+// the caches 31.4, and 38.7 with 256 threads of 4 units (the last ones idle) for 640 units.  8 rows of 5120 fp32 4.5 us.
+template <int XT, int Q, int R, bool STREAM>
+__global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
   using X = Rows<XT>;
   constexpr int EPU = X::EPU, NU = R > 0 ? R : 1;
-  __shared__ double sums[NT / 64];
-  __shared__ uint32_t tops[NT / 64];
-  const int m = blockIdx.x, tid = threadIdx.x, k0 = tid * EPU, step = NT * EPU, K = a.K;
+  __shared__ double sums[16];
+  __shared__ uint32_t tops[16];
+  const int m = blockIdx.x, tid = threadIdx.x, k0 = tid * EPU, step = blockDim.x * EPU, K = a.K, nw = blockDim.x / 64;
+  auto get = [](const uint8_t* row, int k, int n) __attribute__((always_inline)) {
+    if constexpr (STREAM) return X::get_nt(row, k, n);
+    else return X::get(row, k, n);
+  };
   const uint8_t* xr = a.x + (size_t)m * a.ldx;
   const uint8_t* rr = a.res ? a.res + (size_t)m * a.ldr : nullptr;
   uint8_t* hr = a.h ? a.h + (size_t)m * a.ldh : nullptr;
@@ -94,11 +101,11 @@ __global__ __launch_bounds__(NT) void norm_kernel(const NormArgs a) {
   float g[NU][EPU];
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) u[i] = k0 + i * step < K ? X::get(xr, k0 + i * step, K) : none;
+    for (int i = 0; i < R; ++i) u[i] = k0 + i * step < K ? get(xr, k0 + i * step, K) : none;
     if (rr) {
       u32x4 w[NU];
 #pragma unroll
-      for (int i = 0; i < R; ++i) w[i] = k0 + i * step < K ? X::get(rr, k0 + i * step, K) : none;
+      for (int i = 0; i < R; ++i) w[i] = k0 + i * step < K ? get(rr, k0 + i * step, K) : none;
 #pragma unroll
       for (int i = 0; i < R; ++i) u[i] = add(u[i], w[i]);
     }
@@ -111,7 +118,10 @@ __global__ __launch_bounds__(NT) void norm_kernel(const NormArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (hr && k0 + i * step < K) X::set(hr, k0 + i * step, K, u[i]);
+      if (hr && k0 + i * step < K) {
+        if constexpr (STREAM) X::set_nt(hr, k0 + i * step, K, u[i]);
+        else X::set(hr, k0 + i * step, K, u[i]);
+      }
       squares(u[i]);
     }
   } else {
@@ -126,8 +136,7 @@ __global__ __launch_bounds__(NT) void norm_kernel(const NormArgs a) {
   if ((tid & 63) == 0) sums[tid >> 6] = s;
   __syncthreads();
   s = sums[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) s += sums[w];
+  for (int w = 1; w < nw; ++w) s += sums[w];
   const float r = (float)(1. / sqrt(s / K + (double)a.eps));
   if (a.rstd && tid == 0) a.rstd[m] = r;
 
@@ -196,8 +205,7 @@ __global__ __launch_bounds__(NT) void norm_kernel(const NormArgs a) {
     for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) top = max(top, tops[w]);
+    for (int w = 0; w < nw; ++w) top = max(top, tops[w]);
     const RowScale rs = row_scale_of(top);
     auto put = [&](int k, const float (&t)[EPU]) __attribute__((always_inline)) {
       if constexpr (EPU == 8) *(u32x2*)(q + k) = u32x2{codes4(t, rs), codes4(t + 4, rs)};
@@ -232,13 +240,17 @@ struct GradArgs {
 };
 
 // A workgroup takes rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns of dgain in
-// registers (R = 0: in its row of `part`).
-template <int XT, int NT, int R>
-__global__ __launch_bounds__(NT) void norm_grad_kernel(const GradArgs a) {
+// registers (R = 0: in its row of `part`).  STREAM: rows come from past the caches.
+template <int XT, int R, bool STREAM>
+__global__ __launch_bounds__(1024) void norm_grad_kernel(const GradArgs a) {
   using X = Rows<XT>;
   constexpr int EPU = X::EPU, NU = R > 0 ? R : 1;
-  __shared__ float sums[2][NT / 64];
-  const int tid = threadIdx.x, k0 = tid * EPU, step = NT * EPU, K = a.K;
+  __shared__ float sums[2][16];
+  const int tid = threadIdx.x, k0 = tid * EPU, step = blockDim.x * EPU, K = a.K, nw = blockDim.x / 64;
+  auto get = [](const uint8_t* row, int k, int n) __attribute__((always_inline)) {
+    if constexpr (STREAM) return X::get_nt(row, k, n);
+    else return X::get(row, k, n);
+  };
   const u32x4 none = {0u, 0u, 0u, 0u};
   float* part = a.part ? a.part + (size_t)blockIdx.x * K : nullptr;
   float g[NU][EPU], dg[NU][EPU];
@@ -257,8 +269,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(const GradArgs a) {
     if ((tid & 63) == 0) sums[turn][tid >> 6] = s;
     __syncthreads();
     s = sums[turn][0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) s += sums[turn][w];
+    for (int w = 1; w < nw; ++w) s += sums[turn][w];
     turn ^= 1;  // the next row's sums do not meet slow readers of this one's
     return s;
   };
@@ -293,9 +304,9 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(const GradArgs a) {
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const int k = k0 + i * step;
-        dyu[i] = k < K ? X::get(dyr, k, K) : none;
-        hu[i] = k < K ? X::get(hr, k, K) : none;
-        dhu[i] = dhr && k < K ? X::get(dhr, k, K) : none;
+        dyu[i] = k < K ? get(dyr, k, K) : none;
+        hu[i] = k < K ? get(hr, k, K) : none;
+        dhu[i] = dhr && k < K ? get(dhr, k, K) : none;
       }
       float d[NU][EPU], xh[NU][EPU];
 #pragma unroll
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(const GradArgs a) {
 }
 
 // dgain[k] = sum of n partial rows, in a fixed order.
-constexpr int kSumCols = 16, kSumParts = 16;
+constexpr int kSumCols = 32, kSumParts = 32;
 __global__ __launch_bounds__(kSumCols * kSumParts) void norm_gain_kernel(const float* __restrict__ part, int n, int K,
                                                                          float* __restrict__ dgain) {
   __shared__ float s[kSumParts][kSumCols];
@@ -351,34 +362,49 @@ __global__ __launch_bounds__(kSumCols * kSumParts) void norm_gain_kernel(const f
   }
 }
 
-// Rows up to which a row gets 1024 threads: few rows wait for their latency.
+// Rows up to which a thread takes one unit where that is enough: few rows wait for their latency, many for memory, and
+// take two.  Bytes of rows from which on they are streamed: what the last-level cache does not keep for the next call.
 constexpr int kNormWide = 512;
+constexpr size_t kNormStream = (size_t)72 << 20;
+
+// Units a thread (0: any number) and threads for rows of so many units.
+struct Shape {
+  int r, threads;
+};
+Shape shape_of(int units, bool one, int most) {
+  for (int r = one || units <= 128 ? 1 : 2; r <= most; r *= 2) {
+    const int threads = (units + 64 * r - 1) / (64 * r) * 64;
+    if (threads <= 1024) return {r, threads};
+  }
+  return {0, 1024};
+}
+template <class F>
+void with_shape(Shape h, F f) {
+  if (h.r == 1) f(std::integral_constant<int, 1>());
+  else if (h.r == 2) f(std::integral_constant<int, 2>());
+  else if (h.r == 4) f(std::integral_constant<int, 4>());
+  else f(std::integral_constant<int, 0>());
+}
 
 template <int Q>
 int norm(const NormArgs& a, int xtype, int M, hipStream_t s, const char* who) {
   with_rows(xtype, [&](auto xt) {
-    constexpr int XT = decltype(xt)::value;
-    const int units = ((Q == Q_NONE ? a.K : a.Kp) + Rows<XT>::EPU - 1) / Rows<XT>::EPU;
-#define NORM(NT, R) norm_kernel<XT, Q, NT, R><<<M, NT, 0, s>>>(a)
-    if (M <= kNormWide) {
-      if (units <= 1024) NORM(1024, 1);
-      else if (units <= 2048) NORM(1024, 2);
-      else if (units <= 4096) NORM(1024, 4);
-      else NORM(1024, 0);
-    } else {
-      if (units <= 512) NORM(256, 2);
-      else if (units <= 1024) NORM(256, 4);
-      else if (units <= 2048) NORM(512, 4);
-      else if (units <= 4096) NORM(1024, 4);
-      else NORM(1024, 0);
-    }
-#undef NORM
+    constexpr int XT = decltype(xt)::value, EPU = Rows<XT>::EPU;
+    const Shape h = shape_of(((Q == Q_NONE ? a.K : a.Kp) + EPU - 1) / EPU, M <= kNormWide, 4);
+    const bool stream = (size_t)M * a.K * Rows<XT>::ES * (a.res ? 2 : 1) >= kNormStream;
+    with_shape(h, [&](auto r) {
+      constexpr int R = decltype(r)::value;
+      if (R && stream) norm_kernel<XT, Q, R, R != 0><<<M, h.threads, 0, s>>>(a);
+      else norm_kernel<XT, Q, R, false><<<M, h.threads, 0, s>>>(a);
+    });
   });
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
 }
 
-// Workgroups of the gradient, each with its rows' part of dgain.
+// Workgroups of the gradient, each with its rows' part of dgain.  4096 x 5120 bf16 with dh 39.3 us, both kernels (4.3 TB/s);
+// 256 workgroups 44, 768 50 (their rows are no whole rounds), and 8 us more where 16 columns of all parts were a
+// workgroup's.
 constexpr int kGradGrid = 512;
 int grad_grid(int M) { return M < kGradGrid ? M : kGradGrid; }
 
@@ -474,15 +500,16 @@ int tiermm_rms_norm_grad(const void* dy, int type, size_t ldy, const void* h, si
                         ldy * es, ldh * es, lddh * es, lddx * es, M, K};
     with_rows(type, [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
-      const int units = (K + Rows<XT>::EPU - 1) / Rows<XT>::EPU;
-#define GRAD(NT, R) norm_grad_kernel<XT, NT, R><<<grid, NT, 0, s>>>(a)
-      if (units <= 256) GRAD(256, 1);
-      else if (units <= 512) GRAD(256, 2);
-      else if (units <= 1024) GRAD(512, 2);
-      else if (units <= 2048) GRAD(1024, 2);
-      else if (units <= 4096) GRAD(1024, 4);
-      else GRAD(1024, 0);
-#undef GRAD
+      // (four units of 16 bits do not fit the registers of 1024 threads)
+      const Shape shape = shape_of((K + Rows<XT>::EPU - 1) / Rows<XT>::EPU, true, XT == QT_F32 ? 4 : 2);
+      const bool stream = (size_t)M * K * es * (dh ? 3 : 2) >= kNormStream;
+      with_shape(shape, [&](auto r) {
+        constexpr int R = decltype(r)::value;
+        if constexpr (R < 4 || XT == QT_F32) {
+          if (R && stream) norm_grad_kernel<XT, R, R != 0><<<grid, shape.threads, 0, s>>>(a);
+          else norm_grad_kernel<XT, R, false><<<grid, shape.threads, 0, s>>>(a);
+        }
+      });
     });
     TM_LAUNCH_CHECK(who);
   }
