@@ -37,12 +37,15 @@ struct LayerArgs {
 // An id outside [0, E) is a dropped pair.
 __device__ __forceinline__ int find_pairs(const LayerArgs& a, int slot, int& e, uint16_t* list) {
   const int lane = threadIdx.x & 63;
+  int id = a.ids[min(lane, a.P - 1)];  // on its way with the slot's own
   e = a.by_pair ? a.ids[slot] : slot;
+  asm volatile("" : "+v"(id));
   if ((uint32_t)e >= (uint32_t)a.E) return 0;
   int n = 0;
   for (int p0 = 0; p0 < a.P; p0 += 64) {
     const int p = p0 + lane;
-    const uint64_t hit = __ballot(p < a.P && a.ids[min(p, a.P - 1)] == e);
+    if (p0) id = a.ids[min(p, a.P - 1)];
+    const uint64_t hit = __ballot(p < a.P && id == e);
     if (a.by_pair && hit && n == 0 && p0 + __ffsll((unsigned long long)hit) - 1 < slot) return 0;
     // (every wave writes the same list)
     if (hit >> lane & 1) list[n + __popcll(hit & ((1ull << lane) - 1))] = (uint16_t)p;
@@ -223,18 +226,23 @@ __global__ __launch_bounds__(256) void moe_down_few_kernel(const LayerArgs a) {
     const int rows = min(kFew, n - base), nt = (a.F + kTile - 1) / kTile;
     for (int r = 0; r < rows; ++r) {
       const int p = list[base + r];
+      const uint8_t* h = (const uint8_t*)(a.h + (size_t)p * a.F);
+      auto load = [&](int f) { return f < a.F ? Rows<QT_F32>::get(h, f, a.F) : u32x4{0u, 0u, 0u, 0u}; };
+      const u32x4 h0 = load(tid * 4), h1 = load(tid * 4 + 1024);  // on their way while the scale is found
       uint32_t top = 0;
       for (int i = lane; i < nt; i += 64) top = max(top, a.top[(size_t)p * nt + i]);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
       const RowScale rs = row_scale_of(top);
       if (tid == 0) scale[r] = rs.sc;
-      const uint8_t* h = (const uint8_t*)(a.h + (size_t)p * a.F);
-      for (int f = tid * 4; f < Fp; f += 1024) {
+      auto put = [&](int f, u32x4 u) {
         float v[4];
-        Rows<QT_F32>::widen(f < a.F ? Rows<QT_F32>::get(h, f, a.F) : u32x4{0u, 0u, 0u, 0u}, v);
+        Rows<QT_F32>::widen(u, v);
         *(uint32_t*)(codes + r * Fp + (f ^ (r << 4))) = codes4(v, rs);
-      }
+      };
+      if (tid * 4 < Fp) put(tid * 4, h0);
+      if (tid * 4 + 1024 < Fp) put(tid * 4 + 1024, h1);
+      for (int f = tid * 4 + 2048; f < Fp; f += 1024) put(f, load(f));
     }
     i32x4 acc = {0, 0, 0, 0};
     const int xr = min(fr, rows - 1);
