@@ -1,6 +1,6 @@
 // moe_layer.hip -- a routed layer of a few tokens over int8 experts: gate and up, the gate's
-// activation, down, and the weighted sum of a token's experts, in two kernels for few pairs and four for more.  No reference function (the
-// reference refuses MoE models, arch.py:158-159).
+// activation, down, and the weighted sum of a token's experts, in two kernels for few pairs and four
+// for more.  No reference function (the reference refuses MoE models, arch.py:158-159).
 //
 //   g, u = int8 products of x with an expert's gate and up rows (tm_i8.h: exact sums, fp32 scales)
 //   h = fp32(silu(g) u), in 64 bits, rounded once

@@ -20,29 +20,43 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------------- quantizer
-// A thread takes one unit of 16 bytes of a row; the lanes of a block are neighbours.
-template <int XT, int FMT>
-__global__ __launch_bounds__(256) void mx_quant_kernel(const uint8_t* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
-                                                       size_t rb, uint8_t* __restrict__ scales, size_t sb, int K, int Kp) {
+// A thread takes R units of 16 bytes of a row; the lanes of a block are neighbours.  Bound by memory: 4096 rows of
+// 5120 bfloat16 11.7 us to E2M1 (4.5 TB/s, 53 MB), 13.2 to E4M3 with two units a thread, 16.5 and 15.8 with one and
+// 256 threads.
+template <int XT, int FMT, int R>
+__global__ __launch_bounds__(1024) void mx_quant_kernel(const uint8_t* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
+                                                        size_t rb, uint8_t* __restrict__ scales, size_t sb, int K, int Kp) {
   using X = Rows<XT>;
-  const int m = blockIdx.x, k = (blockIdx.y * 256 + threadIdx.x) * X::EPU;
+  const int m = blockIdx.x, step = blockDim.x * X::EPU, k = blockIdx.y * R * step + threadIdx.x * X::EPU;
   uint8_t* sc = scales + (size_t)m * sb;
   const int b = Kp / 32 + threadIdx.x;  // scales of blocks behind the padded row
   if (blockIdx.y == 0 && b < mx_scales(K)) sc[b] = 0;
-  if (k >= Kp) return;
-  float v[X::EPU];
-  X::widen(k < K ? X::get(x + (size_t)m * ldx, k, K) : u32x4{0u, 0u, 0u, 0u}, v);
-  mx_store<FMT>(q + (size_t)m * rb, sc, k, v);
+  u32x4 u[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) u[i] = k + i * step < K ? X::get_nt(x + (size_t)m * ldx, k + i * step, K) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (k + i * step >= Kp) break;
+    float v[X::EPU];
+    X::widen(u[i], v);
+    mx_store<FMT>(q + (size_t)m * rb, sc, k + i * step, v);
+  }
 }
 
+// Few rows wait for their latency and take a unit a thread (37 rows of 5120 fp32 4.8 us), many two.
 int quant(const void* x, int xtype, size_t ldx, int fmt, void* q, size_t rb, uint8_t* scales, size_t sb, int M, int K,
           hipStream_t s, const char* who) {
   with_rows(xtype, [&](auto xt) {
     with_mx(fmt, [&](auto f) {
       constexpr int XT = decltype(xt)::value, FMT = decltype(f)::value, EPU = Rows<XT>::EPU;
-      const dim3 grid(M, (mx_padded(K) / EPU + 255) / 256);
-      mx_quant_kernel<XT, FMT><<<grid, 256, 0, s>>>((const uint8_t*)x, ldx * Rows<XT>::ES, (uint8_t*)q, rb, scales, sb, K,
-                                                    mx_padded(K));
+      auto run = [&](auto rc) {
+        constexpr int R = decltype(rc)::value;
+        const int units = mx_padded(K) / EPU, threads = std::min(1024, (units + 64 * R - 1) / (64 * R) * 64);
+        mx_quant_kernel<XT, FMT, R><<<dim3(M, (units + R * threads - 1) / (R * threads)), threads, 0, s>>>(
+            (const uint8_t*)x, ldx * Rows<XT>::ES, (uint8_t*)q, rb, scales, sb, K, mx_padded(K));
+      };
+      if (M <= 512) run(std::integral_constant<int, 1>());
+      else run(std::integral_constant<int, 2>());
     });
   });
   TM_LAUNCH_CHECK(who);
@@ -158,14 +172,18 @@ constexpr int kAhead = 1;  // stages behind the last one asked for
 // scales come 16 of a row at a time, with every other stage: each row is a cache line of its own for them, and
 // as words of one stage they took as many lines as the codes (4096 x 5120 x 14336: 168 us).
 // A row's 16-byte chunk c lies at slot c ^ ((row >> 1) & 7), which spreads the 16 rows that one cycle of a
-// fragment read touches over the banks.  A stage is four MFMA steps; the order of a sum's blocks is free, so
-// step kk takes block kk in the lower half of the wave and 4 + kk in the upper, and the four scales that a
-// lane needs of a row in a stage are one word, of which step kk uses byte kk.  While the products of one
+// fragment read touches over the banks.  A stage is four MFMA steps of two blocks, one for each half of the wave; a
+// lane's four scales of a row in a stage become one word, of which step kk uses byte kk.  While the products of one
 // step run, the fragments of the next come in, one read between two MFMAs, and the loads of stage kt + S go
 // out, from the step after the barrier that frees their place on.
 //
 // W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y; rows leave
 // through LDS in 16-byte units.
+//
+// 4096 x 14336 x 5120, bfloat16 Y: E2M1 170 us on random codes (256 x 320 tiles, 3.5 PFLOP/s) and 137 on zeros, E4M3
+// 274 (128 x 320, 2.2) and 233.  The MFMAs alone reach 6.2 and 4.0 on random codes and 9.6 and 4.9 on zeros: the
+// card's power bounds the product as much as its instructions do.  With four waves of 128 x 128 225 us against 208
+// with eight.
 template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
 __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, XS = XF == MX_E4M3 ? 2 : 1, NF = WN + WM * XS;
@@ -253,27 +271,38 @@ __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a)
   // fragment v of step kk of stage kt into set f: W's first, those of x, W's others
   auto fragment = [&](int kt, int kk, int f, int v) __attribute__((always_inline)) {
     const uint8_t* s = lds + ring(kt) * STAGE;
-    const int xc = ((XS == 2 ? 2 * kk + fh : 4 * fh + kk) ^ turn) * 16, wc = ((4 * fh + kk) ^ turn) * 16;
+    const int wc = ((2 * kk + fh) ^ turn) * 16;
     if (v >= 1 && v <= WM * XS) {
       const int i = (v - 1) / XS, h = (v - 1) % XS;
-      xf[f][i][h] = *(const i32x4*)(s + xc + xrow + (h * BM + i * 32) * 128);
+      // (E4M3: half a block of the step's first one, and of its second)
+      const int xc = XS == 1 ? wc : ((4 * (kk & 1) + 2 * h + fh) ^ turn) * 16;
+      xf[f][i][h] = *(const i32x4*)(s + xc + xrow + ((XS == 1 ? 0 : (kk >> 1) * BM) + i * 32) * 128);
     } else {
       const int j = v == 0 ? 0 : v - WM * XS;
       wf[f][j] = *(const i32x4*)(s + wc + wrow + j * 32 * 128);
     }
   };
+  // (every other byte of two words: the blocks of this half of the wave)
+  const uint32_t mine = fh ? 0x07050301u : 0x06040200u;
   auto scales = [&](int kt, int (&x)[WM], int (&w)[WN]) __attribute__((always_inline)) {
-    const int* px = (const int*)(lds + Lds::xscales(kt)) + (wm * WM * 32 + fr) * 4 + fh;
-    const int* pw = (const int*)(lds + Lds::wscales(kt)) + (wn * WN * 32 + fr) * 4 + 2 * (kt & 1) + fh;
+    const uint8_t* px = lds + Lds::xscales(kt) + (wm * WM * 32 + fr) * 16;
+    const uint8_t* pw = lds + Lds::wscales(kt) + (wn * WN * 32 + fr) * 16 + 8 * (kt & 1);
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
       int even = xs1[i], odd = 0;
-      if (!(kt & 1)) even = px[i * 128], odd = px[i * 128 + 2];
+      if (!(kt & 1)) {
+        const u32x4 v = *(const u32x4*)(px + i * 512);
+        even = (int)__builtin_amdgcn_perm(v[1], v[0], mine);
+        odd = (int)__builtin_amdgcn_perm(v[3], v[2], mine);
+      }
       x[i] = even;
       xs1[i] = odd;
     }
 #pragma unroll
-    for (int j = 0; j < WN; ++j) w[j] = pw[j * 128];
+    for (int j = 0; j < WN; ++j) {
+      const u32x2 v = *(const u32x2*)(pw + j * 512);
+      w[j] = (int)__builtin_amdgcn_perm(v[1], v[0], mine);
+    }
   };
   // The products of step KK of fragments f, with the fragments (kt, kk) into the other set and n loads of stage
   // `dt` between them.
@@ -409,7 +438,10 @@ int launch_gemm(const MxArgs& a, hipStream_t s, const char* who) {
 // their scales.  A ring of S stages keeps S - 1 on their way by global_load_lds; one barrier a stage.
 //
 // Of a 128-byte piece of a row lane group g takes blocks 2g and 2g + 1, one a step (E4M3: what the MFMA
-// wants of them, half a block of each half of the step).
+// wants of them, half a block of each half of the step).  (g and 4 + g: 2 % fewer cycles on banks, 1 % more time.)
+//
+// 14336 x 5120: E2M1 and bfloat16 Y 10.1 us for 8 rows (3.9 TB/s), 14.3 for 37, E4M3 and fp32 Y 12.1 and 19.4.  With
+// both operands straight from memory into registers instead, 8 rows of E4M3 took 3.7 us more, 37 2.3.
 template <int YT, int XF, int BM, int BN, int WVN, int WVK, int KS, int S>
 __global__ __launch_bounds__(64 * WVN * WVK) void mx_tile_kernel(const MxArgs a) {
   constexpr int NW = WVN * WVK, MB = BM / 16, NB = BN / WVN / 16, KK = 2 * KS / WVK, XS = XF == MX_E4M3 ? 2 : 1;
@@ -567,6 +599,8 @@ __device__ __forceinline__ float add_ror(float v) {
 // stands for block 16 g + i of the one row of W.  With x's blocks laid out alike as the second, the diagonal of the
 // 16 x 16 result holds sum_g <W block 16 g + i, x block 16 g + i>, and its trace over all pieces is the product.  The
 // other 240 sums are waste, but the matrix cores have a tenth of the bytes' time to spend, and nothing is unpacked.
+// 1 x 14336 x 5120, E2M1 and bfloat16: 8.1 us, 4.8 TB/s (a large copy reaches 4.8); 1 x 1024 x 5120, E4M3 and fp32:
+// 3.5 us, of which the launch and one latency are most.
 template <int YT, int XT, int XF, int MX, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxArgs a) {
   // [MX][pieces][XB KiB] codes in the order that lanes read them, then [MX][pieces][64] scales
