@@ -33,9 +33,7 @@ SIZES = [(17, 33), (2000, 33), (65, 3200), (2050, 33), (2050, 101), (2050, 250),
          (2000, 3200), (2050, 4003), (1025, 7000), (1025, 10001), (1025, 14000)]
 
 
-@pytest.mark.parametrize("K", [100, 1100])
-@pytest.mark.parametrize("M,N", SIZES)
-def test_every_tile(gpu, M, N, K):
+def every_output(M, N, K):
     wc, ws = random_rows(E2M1, N, K, N + K)
     W, w = MxRows(E2M1, N, K, wc, ws), mx.values(E2M1, wc, ws)
     bias = np.random.default_rng(1).standard_normal(N).astype(np.float32) * 100
@@ -49,6 +47,18 @@ def test_every_tile(gpu, M, N, K):
             hip.synchronize()
             check(Y.values()[pick], t, xfmt, x, w, bias)
             assert Y.outside_kept()
+
+
+@pytest.mark.parametrize("K", [100, 1100])
+@pytest.mark.parametrize("M,N", SIZES)
+def test_every_tile(gpu, M, N, K):
+    every_output(M, N, K)
+
+
+# rings of the tiles for few rows that turn more than once
+@pytest.mark.parametrize("M,N", [(20, 65), (17, 3200), (3, 14000), (33, 5000), (20, 5000), (33, 6000), (40, 10001)])
+def test_few_rows_of_many_stages(gpu, M, N):
+    every_output(M, N, 4500)
 
 
 class FarRows:

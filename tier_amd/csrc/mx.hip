@@ -440,8 +440,9 @@ int launch_gemm(const MxArgs& a, hipStream_t s, const char* who) {
 // Of a 128-byte piece of a row lane group g takes blocks 2g and 2g + 1, one a step (E4M3: what the MFMA
 // wants of them, half a block of each half of the step).  (g and 4 + g: 2 % fewer cycles on banks, 1 % more time.)
 //
-// 14336 x 5120: E2M1 and bfloat16 Y 10.1 us for 8 rows (3.9 TB/s), 14.3 for 37, E4M3 and fp32 Y 12.1 and 19.4.  With
-// both operands straight from memory into registers instead, 8 rows of E4M3 took 3.7 us more, 37 2.3.
+// 14336 x 5120: E2M1 and bfloat16 Y 9.7 us for 8 rows (4.0 TB/s), 13.2 for 37, E4M3 and fp32 Y 10.5 and 16.1; 37 rows
+// in two tiles of 32 of each column took 14.3 and 19.4, one of 48 by four waves 13.0 and 19.4.  With both operands
+// straight from memory into registers 8 rows of E4M3 took 13.9 us, 37 21.7.
 template <int YT, int XF, int BM, int BN, int WVN, int WVK, int KS, int S>
 __global__ __launch_bounds__(64 * WVN * WVK) void mx_tile_kernel(const MxArgs a) {
   constexpr int NW = WVN * WVK, MB = BM / 16, NB = BN / WVN / 16, KK = 2 * KS / WVK, XS = XF == MX_E4M3 ? 2 : 1;
@@ -742,30 +743,31 @@ int fused(const MxArgs& a, int xtype, int xfmt, int ytype, hipStream_t s, const 
 
 // The tiles, and what one costs: a call takes about t0 + n * (fix + K / 1024 * each) us, n the tiles that the fullest
 // CU runs.  Fitted to measured times of 192 sizes (4 to 4096 rows, 512 to 28672 columns, K of 1024 to 14336), on
-// weights that the last-level cache holds where they fit; the tile with the least such time is within 0.4 % of the
-// best of its list in the mean, 18 % at worst.  E4M3 x has lists of its own, for x as it is and in two parts.  Example,
-// 5120 columns and rows of 5120, E2M1, us: 16 rows 16 x 32 tiles 6.3, 64 x 128 12.4, 128 x 128 16.0; 256 rows 64 x 128
-// 14.1, 128 x 128 18.7, 32 x 64 20.4; 4096 rows 256 x 320 59.6, 256 x 192 70.3, 128 x 128 95.8.
+// weights that the last-level cache holds where they fit; the tile with the least such time is within 0.9 % of the
+// best of its list in the mean up to 256 rows and within 0.4 % over all, 26 % at worst.  E4M3 x has lists of its own,
+// for x as it is and in two parts.  Example, 5120 columns and rows of 5120, E2M1, us: 16 rows 16 x 32 tiles 6.3,
+// 64 x 128 12.4, 128 x 128 16.0; 256 rows 64 x 128 14.1, 128 x 128 18.7, 32 x 64 20.4; 4096 rows 256 x 320 59.6,
+// 256 x 192 70.3, 128 x 128 95.8.
 struct TileCost {
   int bm, bn;
   float t0, fix, each;
 };
 constexpr TileCost kE2m1Tiles[] = {
-    {16, 16, 2.51f, 0.62f, 0.26f}, {16, 32, 1.65f, 1.70f, 0.43f}, {16, 64, 1.49f, 1.43f, 1.09f}, {32, 32, 1.59f, 1.65f, 0.54f},
-    {32, 64, 1.20f, 2.49f, 0.79f}, {64, 128, 2.09f, 0.81f, 2.04f}, {128, 128, 0.f, 3.21f, 2.91f}, {256, 128, 0.f, 4.58f, 3.95f},
-    {256, 192, 0.f, 4.98f, 4.84f}, {256, 256, 0.f, 5.93f, 5.39f}, {256, 320, 0.f, 6.89f, 6.61f},
+    {16, 16, 2.64f, 0.60f, 0.26f}, {16, 32, 1.65f, 1.70f, 0.43f}, {16, 64, 1.36f, 2.10f, 0.65f}, {32, 32, 1.59f, 1.65f, 0.54f},
+    {32, 64, 1.18f, 2.49f, 0.79f}, {48, 64, 1.09f, 2.61f, 1.08f}, {64, 128, 2.09f, 0.81f, 2.04f}, {128, 128, 0.f, 3.22f, 2.91f},
+    {256, 128, 0.f, 4.51f, 3.96f}, {256, 192, 0.f, 4.90f, 4.87f}, {256, 256, 0.f, 5.89f, 5.41f}, {256, 320, 0.f, 6.88f, 6.62f},
 };
 constexpr TileCost kE4m3Tiles[] = {
-    {16, 16, 1.61f, 1.64f, 0.39f}, {16, 32, 1.73f, 1.51f, 0.53f}, {16, 64, 1.47f, 1.62f, 1.21f}, {32, 32, 1.22f, 2.29f, 0.68f},
-    {32, 64, 1.14f, 2.31f, 1.16f}, {64, 128, 0.47f, 2.41f, 2.51f}, {128, 128, 0.f, 3.37f, 3.97f}, {128, 192, 0.f, 3.48f, 4.85f},
-    {128, 256, 0.f, 4.18f, 5.60f}, {128, 320, 0.f, 5.16f, 6.19f},
+    {16, 16, 1.61f, 1.64f, 0.39f}, {16, 32, 1.73f, 1.51f, 0.53f}, {16, 64, 1.41f, 2.28f, 0.75f}, {32, 32, 1.22f, 2.29f, 0.68f},
+    {32, 64, 1.13f, 2.31f, 1.16f}, {48, 64, 1.17f, 2.61f, 1.38f}, {64, 128, 0.47f, 2.41f, 2.51f}, {128, 128, 0.f, 3.37f, 3.97f},
+    {128, 192, 0.f, 3.46f, 4.85f}, {128, 256, 0.f, 4.21f, 5.59f}, {128, 320, 0.f, 5.20f, 6.17f},
 };
 constexpr TileCost kE4m3PartTiles[] = {
-    {16, 16, 1.51f, 1.67f, 0.52f}, {16, 32, 1.63f, 1.53f, 0.66f}, {16, 64, 1.39f, 1.75f, 1.62f}, {32, 32, 1.22f, 2.32f, 0.97f},
-    {32, 64, 1.11f, 2.50f, 1.36f}, {64, 128, 0.19f, 3.28f, 4.70f}, {128, 128, 0.f, 4.52f, 8.03f}, {128, 192, 0.f, 5.50f, 7.41f},
-    {128, 256, 0.f, 6.47f, 9.31f}, {128, 320, 0.f, 7.37f, 10.8f},
+    {16, 16, 1.51f, 1.67f, 0.52f}, {16, 32, 1.63f, 1.53f, 0.66f}, {16, 64, 1.36f, 2.30f, 0.91f}, {32, 32, 1.22f, 2.32f, 0.97f},
+    {32, 64, 1.10f, 2.53f, 1.34f}, {48, 64, 1.15f, 2.65f, 2.11f}, {64, 128, 0.19f, 3.28f, 4.70f}, {128, 128, 0.f, 4.54f, 8.01f},
+    {128, 192, 0.f, 5.50f, 7.41f}, {128, 256, 0.f, 6.44f, 9.32f}, {128, 320, 0.f, 7.33f, 10.8f},
 };
-constexpr int kTileKernels = 5;  // the first ones, of mx_tile_kernel
+constexpr int kTileKernels = 6;  // the first ones, of mx_tile_kernel
 
 template <int N>
 int pick_of(const TileCost (&tiles)[N], const MxArgs& a, int cus) {
@@ -789,15 +791,16 @@ int launch_picked(const MxArgs& a, int cus, hipStream_t s, const char* who) {
   switch (tile) {
     case 0: return launch_tile<YT, XF, 16, 16, 1, 8, 4, 4>(a, s, who);
     case 1: return launch_tile<YT, XF, 16, 32, 1, 8, 4, 4>(a, s, who);
-    case 2: return launch_tile<YT, XF, 16, 64, 2, 2, 2, 4>(a, s, who);
+    case 2: return launch_tile<YT, XF, 16, 64, 1, 8, 4, 3>(a, s, who);
     case 3: return launch_tile<YT, XF, 32, 32, 1, 8, 4, 3>(a, s, who);
     case 4: return launch_tile<YT, XF, 32, 64, 1, 8, 4, E4 ? 2 : 3>(a, s, who);
-    case 5: return launch_gemm<YT, XF, 64, 128, 2, 4, 3>(a, s, who);
-    case 6: return launch_gemm<YT, XF, 128, 128, 2, 4, 3>(a, s, who);
-    case 7: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 192 : 128, 4, 2, E4 ? 2 : 3>(a, s, who);
-    case 8: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 256 : 192, 4, 2, 2>(a, s, who);
-    case 9: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 320 : 256, 4, 2, 2>(a, s, who);
-    default: return launch_gemm<YT, XF, E4 ? 128 : 256, 320, 4, 2, 2>(a, s, who);
+    case 5: return launch_tile<YT, XF, 48, 64, 2, 4, E4 ? 2 : 4, E4 ? 3 : 2>(a, s, who);
+    case 6: return launch_gemm<YT, XF, 64, 128, 2, 4, 3>(a, s, who);
+    case 7: return launch_gemm<YT, XF, 128, 128, 2, 4, 3>(a, s, who);
+    case 8: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 192 : 128, 4, 2, E4 ? 2 : 3>(a, s, who);
+    case 9: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 256 : 192, 4, 2, 2>(a, s, who);
+    case 10: return launch_gemm<YT, XF, E4 ? 128 : 256, E4 ? 320 : 256, 4, 2, 2>(a, s, who);
+    default: return launch_gemm<YT, XF, E4 ? 128 : 256, 320, 4, 2, 2>(a, s, who);  // (E2M1)
   }
 }
 
