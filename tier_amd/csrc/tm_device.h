@@ -154,7 +154,8 @@ __device__ __forceinline__ void ktile_unit(size_t u, size_t rows, size_t& row, i
 // compiler, which treats M0 as reserved (an "m0" clobber is not honoured).  That is
 // sound while the compiler puts nothing of its own in M0 in the kernels that call
 // them: no LDS-DMA builtins, s_sendmsg, indexed register access or LDS-direct reads;
-// in their gfx950 code the only M0 references are these writes.  The loads are
+// in their gfx950 code the only M0 references are these writes.  A load to LDS wants one
+// wait state behind a write of M0 (the compiler's own form has it too): the s_nop.  The loads are
 // invisible to the compiler's wait insertion, so every pipeline waits with explicit
 // vm_wait counts.  __builtin_amdgcn_global_load_lds, which lets the compiler own M0,
 // makes the loads visible to it instead, and it then waits for all of them
@@ -163,14 +164,14 @@ __device__ __forceinline__ void ktile_unit(size_t u, size_t rows, size_t& row, i
 // vmcnt waits and x3.hip 4408 -> 4746, and the stage in flight behind a
 // flag drains before the flag is set.  So the asm form stays.
 __device__ __forceinline__ void dma16(const void* p, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p),
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p),
                "s"(__builtin_amdgcn_readfirstlane(lds_addr))
                : "memory");
 }
 // The same with the non-temporal hint: the bytes are streamed once and should not
 // displace what the caches hold.
 __device__ __forceinline__ void dma16_nt(const void* p, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p),
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p),
                "s"(__builtin_amdgcn_readfirstlane(lds_addr))
                : "memory");
 }
