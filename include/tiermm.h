@@ -422,7 +422,7 @@ int tiermm_i8_gemm_grouped(const int8_t* Xq, size_t rbx, const float* sx, const 
  * rstd[m] = r, which the gradient takes.  Strides of rows count elements (not looked at where the
  * pointer is NULL), rb bytes as in tiermm_i8_quant.  Codes do not depend on the shape of the call.
  * h may be x or the residual, with that one's stride; other outputs must not overlap inputs or
- * each other.  K <= 1048576 (with q: 133120). */
+ * each other.  M < 4194304, K <= 1048576 (with q: 133120). */
 int tiermm_rms_norm(const void* x, int xtype, size_t ldx, const void* residual, size_t ldr, const float* gain,
                     float eps, void* h, size_t ldh, void* y, size_t ldy, int8_t* q, size_t rb, float* scale,
                     float* rstd, int M, int K, tiermm_stream_t stream);
@@ -456,7 +456,8 @@ size_t tiermm_mx_scale_bytes(int K);
 /* Codes and scales of M rows of x (TIERMM_F32, TIERMM_F16 or TIERMM_BF16, ldx elements apart): the scale
  * of a block is 2^(floor(log2 max|x|) - 2) (E4M3: - 8), not below 2^-127; elements are x / scale, exactly,
  * rounded to nearest even, magnitudes past the largest becoming it.  A block that holds a NaN or an
- * infinity gets the scale NaN and codes 0, so every product of the row is NaN. */
+ * infinity gets the scale NaN and codes 0, so every product of the row is NaN.  M <= 1048576 here and below,
+ * N < 16777216. */
 int tiermm_mx_quant(const void* x, int xtype, size_t ldx, int fmt, void* q, size_t rb, uint8_t* scales, size_t sb,
                     int M, int K, tiermm_stream_t stream);
 /* N rows of K columns of TIERMM_MXFP4 blocks (rb bytes apart; a .tq or GGUF matrix), laid out once as

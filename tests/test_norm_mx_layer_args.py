@@ -216,3 +216,12 @@ def test_float_arguments_arrive():
 @pytest.mark.parametrize("stride", [-16, -(1 << 62), 1 << 62, (1 << 40) + 16])
 def test_strides_past_any_memory(call, name, stride):
     assert call(**{name: stride}) == EINVAL and tier_amd.last_error()
+
+
+# A launch has less than 2^32 threads: 1024 for a row of a norm, 256 for a row of blocks.
+@pytest.mark.parametrize("call,kw", [(norm, {"M": 1 << 22}), (norm_mx, {"M": 1 << 22}), (grad, {"M": 1 << 22}),
+                                     (blocks, {"N": 1 << 24}), (gemm, {"N": 1 << 24, "ldy": 1 << 24}),
+                                     (linear, {"N": 1 << 24, "ldy": 1 << 24})])
+def test_more_rows_than_a_launch_has_threads_for(call, kw):
+    assert call(**kw) == UNSUPPORTED and "at most" in tier_amd.last_error()
+    assert tier_amd.rms_norm_grad_ws_bytes(1 << 22, 300) == 0

@@ -419,7 +419,7 @@ int launch(Fn* fn, std::atomic<uint64_t>& done, const MxArgs& a, int bm, int bn,
   const int st = lds_attr_once(done, (const void*)fn, lds, who);
   if (st != TIERMM_OK) return st;
   const long long tiles = ((a.N + bn - 1ll) / bn) * ((a.M + bm - 1ll) / bm), grid = (tiles + 7) / 8 * 8;
-  if (grid > (1ll << 30)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, tiles);
+  if (grid * threads >= (1ll << 32)) return set_error(TIERMM_UNSUPPORTED, "%s: %lld tiles", who, tiles);
   fn<<<(unsigned)grid, threads, lds, s>>>(a);
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
@@ -819,7 +819,8 @@ int check_size(const char* who, int M, int N, int K) {
   if (M < 0 || N < 0 || K < 1) return set_error(TIERMM_EINVAL, "%s: bad size %d x %d x %d", who, M, N, K);
   if (K > kMxMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: K = %d, at most %d", who, K, kMxMaxK);
   if (M > (1 << 20)) return set_error(TIERMM_UNSUPPORTED, "%s: %d rows, at most %d", who, M, 1 << 20);
-  if (N > (1 << 26)) return set_error(TIERMM_UNSUPPORTED, "%s: %d columns, at most %d", who, N, 1 << 26);
+  // (a launch has less than 2^32 threads, of which a row of W may have 256)
+  if (N >= (1 << 24)) return set_error(TIERMM_UNSUPPORTED, "%s: %d columns, at most %d", who, N, (1 << 24) - 1);
   return TIERMM_OK;
 }
 int check_fmt(const char* who, int fmt) {

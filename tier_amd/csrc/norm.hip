@@ -408,13 +408,15 @@ int norm(const NormArgs& a, int xtype, int M, hipStream_t s, const char* who) {
 constexpr int kGradGrid = 512;
 int grad_grid(int M) { return M < kGradGrid ? M : kGradGrid; }
 
+constexpr int kRows = (1 << 22) - 1;  // a launch has less than 2^32 threads
+
 // Checks of what the forward entry points share; *es = bytes of an element.
 int check_norm(const char* who, const void* x, int xtype, size_t ldx, const void* res, size_t ldr, const float* gain,
                float eps, const void* h, size_t ldh, const void* y, size_t ldy, const float* rstd, int M, int K, int* es) {
   *es = row_elem_bytes(xtype);
   if (!*es) return set_error(TIERMM_UNSUPPORTED, "%s: rows of type %d", who, xtype);
   if (M < 0 || K < 1) return set_error(TIERMM_EINVAL, "%s: bad size %d x %d", who, M, K);
-  if (M > (1 << 23) || K > kMxMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: %d x %d, at most %d x %d", who, M, K, 1 << 23, kMxMaxK);
+  if (M > kRows || K > kMxMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: %d x %d, at most %d x %d", who, M, K, kRows, kMxMaxK);
   if (!(eps >= 0.f) || std::isinf(eps)) return set_error(TIERMM_EINVAL, "%s: eps = %g", who, eps);
   if (bad_stride(ldx, K) || (res && bad_stride(ldr, K)) || (h && bad_stride(ldh, K)) || (y && bad_stride(ldy, K)))
     return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
@@ -470,7 +472,7 @@ int tiermm_rms_norm_mx(const void* x, int xtype, size_t ldx, const void* residua
 }
 
 size_t tiermm_rms_norm_grad_ws_bytes(int M, int K) {
-  if (M < 1 || K < 1 || M > (1 << 23) || K > kMxMaxK) return 0;
+  if (M < 1 || K < 1 || M > kRows || K > kMxMaxK) return 0;
   return (size_t)grad_grid(M) * K * sizeof(float);
 }
 
@@ -481,7 +483,7 @@ int tiermm_rms_norm_grad(const void* dy, int type, size_t ldy, const void* h, si
   const int es = row_elem_bytes(type);
   if (!es) return set_error(TIERMM_UNSUPPORTED, "%s: rows of type %d", who, type);
   if (M < 0 || K < 1) return set_error(TIERMM_EINVAL, "%s: bad size %d x %d", who, M, K);
-  if (M > (1 << 23) || K > kMxMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: %d x %d, at most %d x %d", who, M, K, 1 << 23, kMxMaxK);
+  if (M > kRows || K > kMxMaxK) return set_error(TIERMM_UNSUPPORTED, "%s: %d x %d, at most %d x %d", who, M, K, kRows, kMxMaxK);
   if (bad_stride(ldy, K) || bad_stride(ldh, K) || (dh && bad_stride(lddh, K)) || bad_stride(lddx, K))
     return set_error(TIERMM_EINVAL, "%s: row stride below %d or past 2^40", who, K);
   if (M && (!dy || !h || !gain || !rstd || !dx)) return set_error(TIERMM_EINVAL, "%s: null buffer", who);
