@@ -210,7 +210,7 @@ def grad64(dy, h, r, g, dh):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("M,K,pad,skip", SIZES + [(1100, 640, 0, 0)])
+@pytest.mark.parametrize("M,K,pad,skip", SIZES + [(1100, 640, 0, 0), (150, 17000, 1, 0), (390, 1000, 0, 2), (2100, 200, 0, 0)])
 def test_gradient(gpu, t, M, K, pad, skip):
     H, DY, DH = Rows(t, M, K, rows(M, K, 11), pad, skip), Rows(t, M, K, rows(M, K, 12, 0.1), pad + 1), Rows(t, M, K, rows(M, K, 13, 0.1), 0, skip)
     g = gains(K)

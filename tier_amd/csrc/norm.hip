@@ -402,11 +402,12 @@ int norm(const NormArgs& a, int xtype, int M, hipStream_t s, const char* who) {
   return TIERMM_OK;
 }
 
-// Workgroups of the gradient, each with its rows' part of dgain.  4096 x 5120 bf16 with dh 39.3 us, both kernels (4.3 TB/s);
-// 256 workgroups 44, 768 50 (their rows are no whole rounds), and 8 us more where 16 columns of all parts were a
-// workgroup's.
-constexpr int kGradGrid = 512;
-int grad_grid(int M) { return M < kGradGrid ? M : kGradGrid; }
+// Workgroups of the gradient, each with its rows' part of dgain: more of them read the rows faster, and leave more parts
+// to add.  Rows of 5120 bf16 with dh, us with 64 / 128 / 256 / 512 workgroups: 128 rows 9.0 / 9.1, 256 rows 11.6 / 10.4 /
+// 12.3, 512 rows 17.6 / 13.5 / 14.6 / 20.7, 1024 rows 27.1 / 19.3 / 17.5 / 21.1, 2048 rows 53 / 30 / 25.2 / 27.2, 4096 rows
+// 256 44, 512 39.3 (4.3 TB/s), 768 50 (their rows are no whole rounds).  8 us more there where 16 columns of all parts
+// were a workgroup's.
+int grad_grid(int M) { return M > 2048 ? 512 : M > 384 ? 256 : std::min(M, 128); }
 
 constexpr int kRows = (1 << 22) - 1;  // a launch has less than 2^32 threads
 
