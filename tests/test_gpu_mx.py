@@ -57,7 +57,8 @@ def check(got, t, fmt, x, w, bias=None):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,K,pad,skip", [(1, 1, 0, 0), (3, 31, 0, 1), (2, 32, 1, 0), (5, 1408, 0, 0), (2, 5121, 2, 3),
-                                          (1, 257, 0, 0), (3, 512, 1, 8), (70, 300, 1, 1)])
+                                          (1, 257, 0, 0), (3, 512, 1, 8), (70, 300, 1, 1), (2, 20000, 0, 0),
+                                          (600, 1, 0, 0), (600, 1408, 1, 1), (513, 5121, 0, 0), (515, 17000, 1, 3)])
 def test_quant(gpu, fmt, t, M, K, pad, skip):
     X = Rows(t, M, K, _x(M, K, K + M), pad, skip)
     Q = MxRows(fmt, M, K, pad=pad)
