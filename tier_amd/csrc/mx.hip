@@ -437,8 +437,8 @@ int launch_gemm(const MxArgs& a, hipStream_t s, const char* who) {
 // share the columns and the steps of 128 elements of a stage, which holds KS * 256 elements of every row and
 // their scales.  A ring of S stages keeps S - 1 on their way by global_load_lds; one barrier a stage.
 //
-// Of a 128-byte piece of a row lane group g takes blocks 2g and 2g + 1, one a step (E4M3: what the MFMA
-// wants of them, half a block of each half of the step).  (g and 4 + g: 2 % fewer cycles on banks, 1 % more time.)
+// Of a 128-byte piece of a row lane group g takes blocks g and 4 + g, one a step (E4M3: what the MFMA wants, half a
+// block of each half of the step).
 //
 // 14336 x 5120: E2M1 and bfloat16 Y 9.7 us for 8 rows (4.0 TB/s), 13.2 for 37, E4M3 and fp32 Y 10.5 and 16.1; 37 rows
 // in two tiles of 32 of each column took 14.3 and 19.4, one of 48 by four waves 13.0 and 19.4.  With both operands
@@ -523,16 +523,16 @@ __global__ __launch_bounds__(64 * WVN * WVK) void mx_tile_kernel(const MxArgs a)
     for (int k = 0; k < KK; ++k) {
       const int step = wk * KK + k, sub = step >> 1, h = step & 1;
       if (st * KS + sub >= a.nk) break;
-      const int wc = ((2 * fg + h) ^ turn) * 16, xc = XS == 2 ? ((4 * (fg >> 1) + 2 * h + (fg & 1)) ^ turn) * 16 : wc;
+      const int wc = ((4 * h + fg) ^ turn) * 16;
       const uint8_t* p = s + sub * SUB + fr * 128;
-      const uint8_t* sc = s + CODES + ((sub >> 1) * (BM + BN) + fr) * 16 + (sub & 1) * 8 + 2 * fg + h;
+      const uint8_t* sc = s + CODES + ((sub >> 1) * (BM + BN) + fr) * 16 + (sub & 1) * 8 + 4 * h + fg;
       i32x8 xf[MB][PARTS], wf[NB];
       int xs[MB], ws[NB];
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
-        const uint8_t* x = p + xc + i * 16 * 128;
-        if constexpr (XS == 1) xf[i][0] = e2m1(*(const i32x4*)x);
-        else xf[i][0] = e4m3(*(const i32x4*)x, *(const i32x4*)(x + BM * 128));
+        const uint8_t* x = p + ((XS == 1 ? 0 : h * BM) + i * 16) * 128;
+        if constexpr (XS == 1) xf[i][0] = e2m1(*(const i32x4*)(x + wc));
+        else xf[i][0] = e4m3(*(const i32x4*)(x + (fg ^ turn) * 16), *(const i32x4*)(x + ((4 + fg) ^ turn) * 16));
         xs[i] = sc[i * 256];
         if constexpr (PARTS == 2) {
           xf[i][1] = mx_large(xf[i][0]);
