@@ -70,7 +70,8 @@ constexpr int kTile = 16;           // columns of h whose largest magnitude is k
 // call 71 and 114.  Rings of 80 KB, two workgroups a CU: 94 and 164.
 template <int BM, int COLS, int KS, int S, bool DOWN>
 __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
-  constexpr int MB = BM / 16, HALF = COLS / 2, NB = HALF / 16, ROWS = BM + COLS, SUB = ROWS * kStep, STAGE = KS * SUB, INST = STAGE / 1024 / 4, LDO = COLS + 4;
+  constexpr int MB = BM / 16, HALF = COLS / 2, NB = HALF / 16, ROWS = BM + COLS, SUB = ROWS * kStep;
+  constexpr int STAGE = KS * SUB, INST = STAGE / 1024 / 4, LDO = COLS + 4;
   static_assert(INST * 4 * 1024 == STAGE && 2 * BM * LDO * 4 <= S * STAGE, "whole loads a wave, sums in LDS");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ uint16_t list[kPairs];
