@@ -7,9 +7,10 @@
 //   r = fp32((mean(h^2) + eps)^-1/2)
 //   y = (h r) gain              two fp32 products
 //
-// The mean and r's root are held in 64 bits: r is then the same fp32 number whatever the order of
-// the sum (but for one in some 2^28 that falls next to a border), and with it every code behind
-// it, in any launch shape.
+// The mean and r's root are held in 64 bits, and the squares of a row are added in one order whatever the number of rows:
+// 16 bytes by a lane (in rows of more than 4096 such units what one of 1024 threads takes), the sums of 64 lanes in
+// pairs, and those of up to 64 such groups in pairs.  r and every code behind it is then the same in any call.  (Another
+// order gives another r where it falls next to a border between two fp32 numbers, one row in some 2^25.)
 #include "tm_i8.h"
 #include "tm_mx.h"
 
@@ -50,10 +51,39 @@ __device__ __forceinline__ void load_gain(const float* gain, int c, int K, float
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
+// What f makes of a value of all lanes (f commutes), in every lane: in a row of 16 with lanes 1, 2, 7 and 15 away, which
+// by then hold what lanes 4 and 8 away do, then the rows.  Moves within the registers: shuffles go through LDS.
+template <class T, class F>
+__device__ __forceinline__ T wave_join(T v, F f) {
+  constexpr int N = sizeof(T) / 4;
+  struct Words {
+    uint32_t w[N];
+  };
+  auto lanes = [&](auto ctrl) __attribute__((always_inline)) {
+    Words t = __builtin_bit_cast(Words, v);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int i = 0; i < N; ++i) t.w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)t.w[i], decltype(ctrl)::value, 0xf, 0xf, true);
+    v = f(v, __builtin_bit_cast(T, t));
+  };
+  lanes(std::integral_constant<int, 0xB1>());   // quad_perm [1, 0, 3, 2]
+  lanes(std::integral_constant<int, 0x4E>());   // quad_perm [2, 3, 0, 1]
+  lanes(std::integral_constant<int, 0x141>());  // row_half_mirror
+  lanes(std::integral_constant<int, 0x140>());  // row_mirror
+  auto rows = [&](auto swap) __attribute__((always_inline)) {
+    Words a = __builtin_bit_cast(Words, v), b = a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const auto t = swap(a.w[i]);
+      a.w[i] = t[0], b.w[i] = t[1];
+    }
+    v = f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+  };
+  rows([](uint32_t a) { return __builtin_amdgcn_permlane16_swap(a, a, false, false); });
+  rows([](uint32_t a) { return __builtin_amdgcn_permlane32_swap(a, a, false, false); });
   return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  return wave_join(v, [](double a, double b) { return a + b; });
 }
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -71,7 +101,7 @@ template <int XT, int Q, int R, bool STREAM>
 __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
   using X = Rows<XT>;
   constexpr int EPU = X::EPU, NU = R > 0 ? R : 1;
-  __shared__ double sums[16];
+  __shared__ double sums[NU * 16];
   __shared__ uint32_t tops[16];
   const int m = blockIdx.x, tid = threadIdx.x, k0 = tid * EPU, step = blockDim.x * EPU, K = a.K, nw = blockDim.x / 64;
   auto get = [](const uint8_t* row, int k, int n) __attribute__((always_inline)) {
@@ -90,13 +120,16 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
     for (int i = 0; i < EPU; ++i) v[i] += w[i];
     return X::narrow(v);
   };
-  double s = 0.;
-  auto squares = [&](u32x4 u) __attribute__((always_inline)) {
+  auto squares = [&](u32x4 u, double s) __attribute__((always_inline)) {
     float v[EPU];
     X::widen(u, v);
 #pragma unroll
     for (int i = 0; i < EPU; ++i) s = fma((double)v[i], (double)v[i], s);
+    return s;
   };
+  double part[NU];  // of this lane's units, one by one (R = 0: of all)
+#pragma unroll
+  for (int i = 0; i < NU; ++i) part[i] = 0.;
   u32x4 u[NU];
   float g[NU][EPU];
   if constexpr (R > 0) {
@@ -122,21 +155,24 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
         if constexpr (STREAM) X::set_nt(hr, k0 + i * step, K, u[i]);
         else X::set(hr, k0 + i * step, K, u[i]);
       }
-      squares(u[i]);
+      part[i] = squares(u[i], 0.);
     }
   } else {
     for (int k = k0; k < K; k += step) {
       u32x4 v = X::get(xr, k, K);
       if (rr) v = add(v, X::get(rr, k, K));
       if (hr) X::set(hr, k, K, v);
-      squares(v);
+      part[0] = squares(v, part[0]);
     }
   }
-  s = wave_sum(s);
-  if ((tid & 63) == 0) sums[tid >> 6] = s;
+#pragma unroll
+  for (int i = 0; i < NU; ++i) part[i] = wave_sum(part[i]);
+  if ((tid & 63) == 0)  // group i * nw + wave of 64 units
+#pragma unroll
+    for (int i = 0; i < NU; ++i) sums[i * nw + (tid >> 6)] = part[i];
   __syncthreads();
-  s = sums[0];
-  for (int w = 1; w < nw; ++w) s += sums[w];
+  const int lane = tid & 63;
+  const double s = wave_sum(lane < NU * nw ? sums[lane] : 0.);
   const float r = (float)(1. / sqrt(s / K + (double)a.eps));
   if (a.rstd && tid == 0) a.rstd[m] = r;
 
@@ -201,8 +237,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
     if (b < mx_scales(K)) sc[b] = 0;
   }
   if constexpr (Q == Q_I8) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    top = wave_join(top, [](uint32_t a, uint32_t b) { return max(a, b); });
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
     for (int w = 0; w < nw; ++w) top = max(top, tops[w]);
