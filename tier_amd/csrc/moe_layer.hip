@@ -293,15 +293,16 @@ __global__ __launch_bounds__(256) void moe_down_few_kernel(const LayerArgs a) {
     float v = 0.f;
     for (int j0 = 0; j0 < a.topk; j0 += 8) {
       float w[8], y[8];
+      bool live[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int p = t * a.topk + min(j0 + j, a.topk - 1);
-        const bool live = j0 + j < a.topk && (uint32_t)a.ids[p] < (uint32_t)a.E;
-        w[j] = live ? a.weights[p] : 0.f;
-        y[j] = live ? __hip_atomic_load(a.y + (size_t)p * a.K + n0 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+        live[j] = j0 + j < a.topk && (uint32_t)a.ids[p] < (uint32_t)a.E;
+        w[j] = live[j] ? a.weights[p] : 0.f;
+        y[j] = live[j] ? __hip_atomic_load(a.y + (size_t)p * a.K + n0 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v = fmaf(w[j], y[j], v);
+      for (int j = 0; j < 8; ++j) v = live[j] ? fmaf(w[j], y[j], v) : v;  // (adding 0 would lose a zero's sign)
     }
     const float o[4] = {v, 0.f, 0.f, 0.f};
     Y::put4(a.out + (size_t)t * a.ldo + (size_t)(n0 + c) * Y::ES, o, 1);
