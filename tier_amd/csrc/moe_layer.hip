@@ -58,20 +58,20 @@ constexpr int kFew = 8;             // pairs of an expert that moe_down_few_kern
 constexpr int kFewCols = 32;        // its columns of out a workgroup
 constexpr int kTile = 16;           // columns of h whose largest magnitude is kept
 
-// An expert's tokens, BM at a time, times 64 rows of its weight.  DOWN false: 32 rows of the gate and the same of up, x
-// the tokens' codes, h out.  DOWN true: x the codes of h, the pairs' fp32 products out.
+// An expert's tokens, BM at a time, times COLS rows of its weight.  DOWN false: half of them the gate's and the same of
+// up, x the tokens' codes, h out.  DOWN true: x the codes of h, the pairs' fp32 products out.
 //
-// Bound by the weights' bytes: a ring of S stages of KS * 128 bytes of every row (x's, then W's) keeps S - 1 on their way by
-// global_load_lds, whole lines of eight rows a load; the four waves share the columns and the 64-byte steps, one barrier
-// a stage.  An expert of more than BM pairs goes through its weights again, out of the caches.
+// Bound by the weights' bytes: a ring of S stages of 128 bytes of every row (x's, then W's) keeps S - 1 on their way by
+// global_load_lds, whole lines of eight rows a load; the four waves share the columns and the two 64-byte steps, one
+// barrier a stage.  An expert of more than BM pairs goes through its weights again, out of the caches.
 //
 // Four workgroups a CU, each with a small ring, hide one another's start (its pairs, then its first weights) and
 // end.  8 of 64 experts of 2048 x 1408, gate and up: 8 tokens 40.5 us (6.0 TB/s), 64 tokens 69 (5.3); the whole
 // call 71 and 114.  Rings of 80 KB, two workgroups a CU: 94 and 164.
-template <int BM, int COLS, int KS, int S, bool DOWN>
+template <int BM, int COLS, int S, bool DOWN>
 __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
-  constexpr int MB = BM / 16, HALF = COLS / 2, NB = HALF / 16, ROWS = BM + COLS, SUB = ROWS * kStep;
-  constexpr int STAGE = KS * SUB, INST = STAGE / 1024 / 4, LDO = COLS + 4;
+  constexpr int MB = BM / 16, HALF = COLS / 2, NB = HALF / 16, ROWS = BM + COLS;
+  constexpr int STAGE = ROWS * kStep, INST = STAGE / 1024 / 4, LDO = COLS + 4;
   static_assert(INST * 4 * 1024 == STAGE && 2 * BM * LDO * 4 <= S * STAGE, "whole loads a wave, sums in LDS");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ uint16_t list[kPairs];
@@ -86,14 +86,14 @@ __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
   const uint8_t* W = DOWN ? a.Wd + (size_t)e * a.K * rbw : a.Wg + (size_t)e * 2 * a.F * rbw;
   auto w_row = [&](int r) { return DOWN ? min(n0 + r, N - 1) : (r < HALF ? 0 : N) + min(n0 + r % HALF, N - 1); };
   const uint32_t lds0 = lds_addr(lds);
-  const int ns = (nk + KS - 1) / KS, wn = wave & 1, wk = wave >> 1, fr = lane & 15, fg = lane >> 4, turn = (fr >> 1) & 7;
+  const int wn = wave & 1, wk = wave >> 1, fr = lane & 15, fg = lane >> 4, turn = (fr >> 1) & 7;
   __syncthreads();
   for (int base = 0; base < n; base += BM) {
-    // load u of this wave: eight rows of a half stage
+    // load u of this wave: eight rows of a stage
     const uint8_t* src[INST];
 #pragma unroll
     for (int u = 0; u < INST; ++u) {
-      const int r = (8 * (wave + 4 * u) + (lane >> 3)) % ROWS;
+      const int r = 8 * (wave + 4 * u) + (lane >> 3);
       const int p = list[min(base + r, n - 1)];  // (of a row of W: not used)
       src[u] = (r < BM ? (DOWN ? a.hq : a.X) + (size_t)(DOWN ? p : p / a.topk) * rbx : W + (size_t)w_row(r - BM) * rbw) +
                ((lane & 7) ^ ((r >> 1) & 7)) * 16;
@@ -102,42 +102,36 @@ __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
     auto issue = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < INST; ++u) {
-        const int i = 8 * (wave + 4 * u), r = i % ROWS;
-        const size_t k = (size_t)min(KS * st + i / ROWS, nk - 1) * kStep;  // (past the end: not multiplied)
+        const uint8_t* from = src[u] + (size_t)st * kStep;
         const uint32_t to = lds0 + put * STAGE + (wave + 4 * u) * 1024;
-        if (r >= BM && n <= BM) dma16_nt(src[u] + k, to);
-        else dma16(src[u] + k, to);
+        if (8 * (wave + 4 * u) >= BM && n <= BM) dma16_nt(from, to);
+        else dma16(from, to);
       }
       put = put + 1 == S ? 0 : put + 1;
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
-      if (i < ns) issue(i);
+      if (i < nk) issue(i);
     i32x4 acc[NB][MB] = {};
     int get = 0;
-    for (int st = 0; st < ns; ++st) {
-      const int after = ns - 1 - st;  // stages on their way behind this one
+    for (int st = 0; st < nk; ++st) {
+      const int after = nk - 1 - st;  // stages on their way behind this one
       if (after >= S - 2) vm_wait<(S - 2) * INST>();
       else wait_stages<S - 3, INST>(after);
       __syncthreads();  // stage st has landed for every wave, and the one before it is read
-      if (st + S - 1 < ns) issue(st + S - 1);
+      if (st + S - 1 < nk) issue(st + S - 1);
       const uint8_t* s = lds + get * STAGE;
       get = get + 1 == S ? 0 : get + 1;
+      const uint8_t* p = s + fr * kStep + ((4 * wk + fg) ^ turn) * 16;
+      i32x4 xf[MB], wf[NB];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int step = wk * KS + k, sub = step >> 1;
-        if (KS > 1 && KS * st + sub >= nk) break;
-        const uint8_t* p = s + sub * SUB + fr * kStep + ((4 * (step & 1) + fg) ^ turn) * 16;
-        i32x4 xf[MB], wf[NB];
+      for (int i = 0; i < MB; ++i) xf[i] = *(const i32x4*)(p + i * 16 * kStep);
 #pragma unroll
-        for (int i = 0; i < MB; ++i) xf[i] = *(const i32x4*)(p + i * 16 * kStep);
+      for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(p + (BM + wn * HALF + j * 16) * kStep);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(p + (BM + wn * HALF + j * 16) * kStep);
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
-      }
+        for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
     }
     __syncthreads();
     // a lane's sum is columns 4 * fg .. + 3 of row fr of each block
@@ -184,7 +178,7 @@ __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
 // experts of 2048 x 1408, the whole call with it and with moe_codes_kernel, moe_experts_kernel and
 // moe_layer_sum_kernel: 1 token 22.2 and 24.8 us, 2 tokens 34.5 and 36.8, 4 tokens 53.3 and 54.4, 8 tokens 75.4 and 71.5;
 // 2 of 8 experts of 4096 x 2816 1 token 23.6 and 27.6, 8 tokens 62.2 and 60.1.
-constexpr int kFewPairs = 32, kFewCodes = 24 * 1024;  // pairs, and bytes of codes in LDS (two workgroups a CU)
+constexpr int kFewPairs = 32, kFewCodes = 24 * 1024;  // pairs, and bytes of codes in LDS (three workgroups a CU)
 bool takes_few(int P, int F) { return P <= kFewPairs && kFew * padded(F) <= kFewCodes; }
 
 template <int KS, int S, int YT>
@@ -330,14 +324,14 @@ __global__ __launch_bounds__(256) void moe_codes_kernel(const LayerArgs a) {
   if (blockIdx.y == 0 && tid == 0) a.sh[p] = rs.sc;
 }
 
-template <int BM, int COLS, int KS, int S, bool DOWN>
+template <int BM, int COLS, int S, bool DOWN>
 int launch_experts(const LayerArgs& a, int slots, hipStream_t s, const char* who) {
-  constexpr int LDS = S * KS * (BM + COLS) * kStep;
+  constexpr int LDS = S * (BM + COLS) * kStep;
   static std::atomic<uint64_t> done{0};
-  const int st = lds_attr_once(done, (const void*)moe_experts_kernel<BM, COLS, KS, S, DOWN>, LDS, who);
+  const int st = lds_attr_once(done, (const void*)moe_experts_kernel<BM, COLS, S, DOWN>, LDS, who);
   if (st != TIERMM_OK) return st;
   const int n = DOWN ? COLS : COLS / 2;
-  moe_experts_kernel<BM, COLS, KS, S, DOWN><<<dim3(((DOWN ? a.K : a.F) + n - 1) / n, slots), 256, LDS, s>>>(a);
+  moe_experts_kernel<BM, COLS, S, DOWN><<<dim3(((DOWN ? a.K : a.F) + n - 1) / n, slots), 256, LDS, s>>>(a);
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
 }
@@ -361,10 +355,9 @@ __global__ __launch_bounds__(256) void moe_layer_sum_kernel(const LayerArgs a) {
 
 template <int KS, int S, int YT>
 int launch_few(const LayerArgs& a, int slots, hipStream_t s, const char* who) {
-  const int lds = S * KS * kFewCols * kStep + kFew * a.nf * kStep;
-  static std::atomic<uint64_t> done{0};
-  const int st = lds_attr_once(done, (const void*)moe_down_few_kernel<KS, S, YT>, 160 * 1024 - 8192, who);
-  if (st != TIERMM_OK) return st;
+  constexpr int RING = S * KS * kFewCols * kStep;
+  static_assert(RING + kFewCodes + kPairs * 2 + 64 <= 64 * 1024, "LDS that a launch has without asking");
+  const int lds = RING + kFew * a.nf * kStep;  // (takes_few)
   moe_down_few_kernel<KS, S, YT><<<dim3((a.K + kFewCols - 1) / kFewCols, slots), 256, lds, s>>>(a);
   TM_LAUNCH_CHECK(who);
   return TIERMM_OK;
@@ -436,7 +429,7 @@ int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int
     // Few pairs take tiles of half the columns, so that every CU has some: 1 token 24.6 us against 27.1, 8 tokens 71.2
     // against 70.7, 64 tokens 130 against 114.
     const bool small = P <= 16;
-    st = small ? launch_experts<32, 32, 1, 4, false>(a, slots, s, who) : launch_experts<32, 64, 1, 3, false>(a, slots, s, who);
+    st = small ? launch_experts<32, 32, 4, false>(a, slots, s, who) : launch_experts<32, 64, 3, false>(a, slots, s, who);
     if (st != TIERMM_OK) return st;
     if (takes_few(P, F)) {
       with_rows(otype, [&](auto yt) { st = launch_few<2, 3, decltype(yt)::value>(a, slots, s, who); });
@@ -444,7 +437,7 @@ int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int
     }
     moe_codes_kernel<<<dim3(P, (padded(F) + 4095) / 4096), 256, 0, s>>>(a);
     TM_LAUNCH_CHECK(who);
-    st = small ? launch_experts<32, 32, 1, 4, true>(a, slots, s, who) : launch_experts<32, 64, 1, 3, true>(a, slots, s, who);
+    st = small ? launch_experts<32, 32, 4, true>(a, slots, s, who) : launch_experts<32, 64, 3, true>(a, slots, s, who);
     if (st != TIERMM_OK) return st;
   }
   with_rows(otype, [&](auto yt) {
