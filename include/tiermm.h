@@ -469,8 +469,8 @@ int tiermm_mx_from_mxfp4(const void* W, size_t rb, void* q, size_t rbq, uint8_t*
  * the sizes and types, so a call repeats its bits, and tiermm_mx_linear of one or two rows has another order.
  * Every product of two elements keeps its bits, whatever lies next to it: the MFMA drops what lies below 2^-13
  * of the largest of eight neighbouring products, with E2M1 x nothing, and E4M3 x is taken in two parts of which
- * it drops nothing either, at twice the matrix operations.  A frozen linear's input gradient is the same product on W
- * transposed and quantized by its own rows. */
+ * it drops nothing either, at twice the matrix operations.  A linear's input gradient is no such product: W transposed
+ * has its scales along the other axis, and quantized by rows of its own it stands for other numbers. */
 int tiermm_mx_gemm(const void* Xq, int xfmt, size_t rbx, const uint8_t* sx, size_t sbx, const void* W, size_t rbw,
                    const uint8_t* sw, size_t sbw, const float* bias, void* Y, int ytype, size_t ldy, int M, int N, int K,
                    tiermm_stream_t stream);
@@ -492,7 +492,8 @@ size_t tiermm_mx_linear_ws_bytes(int xfmt, int M, int N, int K);
  * with e = expert_ids[t][j], a device array as the router made it, as weights (fp32) is: nothing of the routing
  * is read on the host, and a captured graph follows new ones.  A pair whose id lies outside
  * [0, n_experts) is dropped, its weight with it; a token of dropped pairs alone gives zeros.  Weights
- * and scales are int8 products' (sgu[e][2F], sd[e][K]); an expert's weights are read once for all its tokens.
+ * and scales are int8 products' (sgu[e][2F], sd[e][K]); an expert's weights are read once for every
+ * 32 of its pairs (in calls of 32 pairs at most its down weights for every 8).
  * Results do not depend on T or on the other tokens.  ws (tiermm_moe_i8_layer_ws_bytes) 16-byte aligned. */
 #define TIERMM_MOE_LAYER_TOKENS 64
 #define TIERMM_MOE_LAYER_TOPK 32
