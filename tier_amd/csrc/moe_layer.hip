@@ -67,7 +67,7 @@ constexpr int kTile = 16;           // columns of h whose largest magnitude is k
 //
 // Four workgroups a CU, each with a small ring, hide one another's start (its pairs, then its first weights) and
 // end.  8 of 64 experts of 2048 x 1408, gate and up: 8 tokens 40.5 us (6.0 TB/s), 64 tokens 69 (5.3); the whole
-// call 71 and 114.  Rings of 80 KB, two workgroups a CU: 94 and 164.
+// call 71 and 113.  Rings of 80 KB, two workgroups a CU: 94 and 164.
 template <int BM, int COLS, int S, bool DOWN>
 __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
   constexpr int MB = BM / 16, HALF = COLS / 2, NB = HALF / 16, ROWS = BM + COLS;
@@ -176,8 +176,8 @@ __global__ __launch_bounds__(256) void moe_experts_kernel(const LayerArgs a) {
 // workgroup makes for itself while its first weights are on the way; then the last of the workgroups that share the
 // columns adds the tokens' experts.  That spares two launches and repeats the codes in every workgroup: 8 of 64
 // experts of 2048 x 1408, the whole call with it and with moe_codes_kernel, moe_experts_kernel and
-// moe_layer_sum_kernel: 1 token 22.2 and 24.8 us, 2 tokens 34.5 and 36.8, 4 tokens 53.3 and 54.4, 8 tokens 75.4 and 71.5;
-// 2 of 8 experts of 4096 x 2816 1 token 23.6 and 27.6, 8 tokens 62.2 and 60.1.
+// moe_layer_sum_kernel: 1 token 21.4 and 23.7 us, 2 tokens 33.6 and 35.4, 4 tokens 52.2 and 53.1, 8 tokens 74.3 and
+// 70.5; 2 of 8 experts of 4096 x 2816 1 token 22.8 and 26.1, 8 tokens 61.7 and 59.2, 16 tokens 75 and 64.
 constexpr int kFewPairs = 32, kFewCodes = 24 * 1024;  // pairs, and bytes of codes in LDS (three workgroups a CU)
 bool takes_few(int P, int F) { return P <= kFewPairs && kFew * padded(F) <= kFewCodes; }
 
@@ -426,8 +426,10 @@ int tiermm_moe_i8_layer(const int8_t* Xq, size_t rbx, const float* sx, const int
   hipStream_t s = (hipStream_t)stream;
   if (P) {
     const int slots = P < n_experts ? P : n_experts;
-    // Few pairs take tiles of half the columns, so that every CU has some: 1 token 24.6 us against 27.1, 8 tokens 71.2
-    // against 70.7, 64 tokens 130 against 114.
+    // Few pairs take tiles of half the columns, so that every CU has some.  us with half and whole tiles: 64 experts
+    // of 1408, top 8 (K 2048) 1 token 21.4 / 22.6, 2 tokens 33.6 / 31.5, 4 tokens 51.7 / 52.5, 8 tokens 73.8 / 71.4,
+    // 64 tokens 129 / 114; 8 of 2816, top 2 (K 4096) 1 token 22.8 / 26.7, 4 tokens 42.0 / 43.4, 8 tokens 61.5 / 60.2;
+    // 128 of 768, top 4 (K 2048) 4 tokens 22.5 / 23.4, 8 tokens 37.3 / 34.5.
     const bool small = P <= 16;
     st = small ? launch_experts<32, 32, 4, false>(a, slots, s, who) : launch_experts<32, 64, 3, false>(a, slots, s, who);
     if (st != TIERMM_OK) return st;

@@ -21,8 +21,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------------- quantizer
 // A thread takes R units of 16 bytes of a row; the lanes of a block are neighbours.  Bound by memory: 4096 rows of
-// 5120 bfloat16 11.7 us to E2M1 (4.5 TB/s, 53 MB), 13.2 to E4M3 with two units a thread, 16.5 and 15.8 with one and
-// 256 threads.
+// 5120 bfloat16 11.1 us to E2M1 (4.8 TB/s, 53 MB) and 12.7 to E4M3 with two units a thread, 12.9 and 14.3 with one.
 template <int XT, int FMT, int R>
 __global__ __launch_bounds__(1024) void mx_quant_kernel(const uint8_t* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
                                                         size_t rb, uint8_t* __restrict__ scales, size_t sb, int K, int Kp) {
@@ -43,7 +42,10 @@ __global__ __launch_bounds__(1024) void mx_quant_kernel(const uint8_t* __restric
   }
 }
 
-// Few rows wait for their latency and take a unit a thread (37 rows of 5120 fp32 4.8 us), many two.
+// Few rows wait for their latency and take a unit a thread, many two.  bfloat16 to E2M1, us with one and two: 2048
+// columns 512 rows 2.2 / 2.3, 2048 rows 3.1 / 3.1, 4096 rows 5.5 / 4.8; 5120 columns 256 rows 2.4 / 2.4, 512 3.0 /
+// 3.0, 640 3.7 / 3.3; 14336 columns 128 rows 2.7 / 3.0, 256 3.4 / 3.4, 512 5.2 / 4.5.  (fp32 rows would change over
+// at 200: 5120 columns 512 rows 4.2 / 3.3.)
 int quant(const void* x, int xtype, size_t ldx, int fmt, void* q, size_t rb, uint8_t* scales, size_t sb, int M, int K,
           hipStream_t s, const char* who) {
   with_rows(xtype, [&](auto xt) {
@@ -180,10 +182,13 @@ constexpr int kAhead = 1;  // stages behind the last one asked for
 // W is the MFMA's first operand, so a lane holds four neighbouring columns of one row of Y; rows leave
 // through LDS in 16-byte units.
 //
-// 4096 x 14336 x 5120, bfloat16 Y: E2M1 170 us on random codes (256 x 320 tiles, 3.5 PFLOP/s) and 137 on zeros, E4M3
-// 274 (128 x 320, 2.2) and 233.  The MFMAs alone reach 6.2 and 4.0 on random codes and 9.6 and 4.9 on zeros: the
-// card's power bounds the product as much as its instructions do.  With four waves of 128 x 128 225 us against 208
-// with eight.
+// 4096 x 14336 x 5120, bfloat16 Y: E2M1 170 us on random codes (256 x 320 tiles, 3.5 PFLOP/s) and 138 on zeros, E4M3
+// 398 (128 x 320, 1.5) and 362; the MFMAs alone, at their rates on random codes, 98 and 300.  The cycles are the same
+// on zeros (E2M1 330000 to 340000, E4M3 880000), so power takes what the clock falls by, from 2.4 to 1.9 and 2.1 GHz.
+// Of the cycles MFMAs are busy in 44 and 66 %.  A stage takes 5500 and 7300, its MFMAs 2560 and 5120, and its 224 KB
+// of fragment reads and 74 KB of loads into LDS 2400 at 128 bytes a cycle: the two hardly overlap, which is what is
+// left to gain here.  With four waves of 128 x 128 (E2M1) 225 us against 208 with eight, before scales came in units
+// and lines ahead.
 template <int YT, int XF, int BM, int BN, int WVM, int WVN, int S>
 __global__ __launch_bounds__(64 * WVM * WVN) void mx_gemm_kernel(const MxArgs a) {
   constexpr int NW = WVM * WVN, WM = BM / WVM / 32, WN = BN / WVN / 32, XS = XF == MX_E4M3 ? 2 : 1, NF = WN + WM * XS;
@@ -600,8 +605,8 @@ __device__ __forceinline__ float add_ror(float v) {
 // stands for block 16 g + i of the one row of W.  With x's blocks laid out alike as the second, the diagonal of the
 // 16 x 16 result holds sum_g <W block 16 g + i, x block 16 g + i>, and its trace over all pieces is the product.  The
 // other 240 sums are waste, but the matrix cores have a tenth of the bytes' time to spend, and nothing is unpacked.
-// 1 x 14336 x 5120, E2M1 and bfloat16: 8.1 us, 4.8 TB/s (a large copy reaches 4.8); 1 x 1024 x 5120, E4M3 and fp32:
-// 3.5 us, of which the launch and one latency are most.
+// 1 x 14336 x 5120, E2M1 and bfloat16: 8.0 us, 4.9 TB/s (a large copy reaches 4.8), E4M3 11.7, for its MFMAs take
+// four times as long; 1 x 1024 x 5120, E4M3 and fp32: 3.5 us, of which the launch and one latency are most.
 template <int YT, int XT, int XF, int MX, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxArgs a) {
   // [MX][pieces][XB KiB] codes in the order that lanes read them, then [MX][pieces][64] scales
@@ -716,7 +721,9 @@ int launch_gemv(const MxArgs& a, hipStream_t s, const char* who) {
 }
 
 // One or two rows of x are quantized by the product's own workgroups: a launch less, and each byte of W in whole
-// lines.
+// lines.  Two tokens of 4096 x 4096, us, against the quantizer (2.2) and the tiles: E2M1 4.2 and 6.5, E4M3 5.5 and
+// 7.2; of 14336 x 5120 E2M1 11.4 and 11.4, E4M3 15.8 and 12.0, whose MFMAs for two rows take longer than W's bytes.
+// (That one stays here all the same: a call of one or two rows needs no workspace.)
 constexpr int kGemvLds = 60 * 1024;
 bool fuses(int xfmt, int M, int K) {
   return M <= 2 && M * (long long)((mx_padded(K) + 2047) / 2048) * (xfmt == MX_E4M3 ? 2112 : 1088) <= kGemvLds;
@@ -730,6 +737,11 @@ int fused(const MxArgs& a, int xtype, int xfmt, int ytype, hipStream_t s, const 
         constexpr int YT = decltype(yt)::value, XT = decltype(xt)::value, XF = decltype(f)::value;
         auto rows = [&](auto mx) {
           constexpr int MX = decltype(mx)::value;
+          // Short products take workgroups of 8 rows, so that every CU has some; long ones of 32, which prepare x
+          // fewer times.  us with 8 and 32 rows, 1 token of K = 5120: E2M1 1024 columns 3.3 / 4.7, 4096 4.2 / 5.1,
+          // 5120 5.0 / 5.2, 8192 5.9 / 5.9, 14336 9.2 / 8.2; E4M3 4096 5.2 / 6.1, 5120 6.4 / 6.3, 8192 7.7 / 7.0.  K
+          // = 14336 crosses between 4096 and 5120 columns too, K = 2048 at 5120 (E4M3) or past 8192 (E2M1: 3.5 / 3.8
+          // there, 14336 5.5 / 4.5).
           if (a.N < 5120) st = launch_gemv<YT, XT, XF, MX, 1, 8>(a, s, who);
           else st = launch_gemv<YT, XT, XF, MX, 2, 16>(a, s, who);
         };
@@ -744,9 +756,9 @@ int fused(const MxArgs& a, int xtype, int xfmt, int ytype, hipStream_t s, const 
 // The tiles, and what one costs: a call takes about t0 + n * (fix + K / 1024 * each) us, n the tiles that the fullest
 // CU runs.  Fitted to measured times of 192 sizes (4 to 4096 rows, 512 to 28672 columns, K of 1024 to 14336), on
 // weights that the last-level cache holds where they fit; the tile with the least such time is within 0.9 % of the
-// best of its list in the mean up to 256 rows and within 0.4 % over all, 26 % at worst.  E4M3 x, in its
-// two parts, has a list of its own (fitted on fp32 Y).  Example, 5120 columns and rows of 5120, E2M1, us: 16 rows 16 x 32 tiles 6.3,
-// 64 x 128 12.4, 128 x 128 16.0; 256 rows 64 x 128 14.1, 128 x 128 18.7, 32 x 64 20.4; 4096 rows 256 x 320 59.6,
+// best of its list in the mean up to 256 rows and within 0.4 % over all, 26 % at worst.  E4M3 x, in its two parts,
+// has a list of its own (fitted on fp32 Y).  Example, 5120 columns and rows of 5120, E2M1, us: 16 rows 16 x 32 tiles
+// 6.3, 64 x 128 12.4, 128 x 128 16.0; 256 rows 64 x 128 14.1, 128 x 128 18.7, 32 x 64 20.4; 4096 rows 256 x 320 59.6,
 // 256 x 192 70.3, 128 x 128 95.8.
 struct TileCost {
   int bm, bn;

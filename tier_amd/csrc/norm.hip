@@ -62,7 +62,8 @@ __device__ __forceinline__ T wave_join(T v, F f) {
   auto lanes = [&](auto ctrl) __attribute__((always_inline)) {
     Words t = __builtin_bit_cast(Words, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) t.w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)t.w[i], decltype(ctrl)::value, 0xf, 0xf, true);
+    for (int i = 0; i < N; ++i)
+      t.w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)t.w[i], decltype(ctrl)::value, 0xf, 0xf, true);
     v = f(v, __builtin_bit_cast(T, t));
   };
   lanes(std::integral_constant<int, 0xB1>());   // quad_perm [1, 0, 3, 2]
@@ -95,8 +96,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 // registers, all its loads on their way at once; R = 0: any row, read again from h (or x and
 // the residual) for each pass.  STREAM: rows come from past the caches, and h goes there.
 //
-// Bound by memory: 4096 x 5120 bf16 with a residual, int8 out, 28.0 us (5.2 TB/s, where a large copy moves 4.8), through
-// the caches 31.4, and 38.7 with 256 threads of 4 units (the last ones idle) for 640 units.  8 rows of 5120 fp32 4.5 us.
+// Bound by memory: 4096 x 5120 bf16 with a residual, int8 out, 28.5 us (5.2 TB/s, where a large copy moves 4.8),
+// through the caches 32.6, and 38.3 with one unit a thread.  8 rows of 5120 fp32 4.7 us.
 template <int XT, int Q, int R, bool STREAM>
 __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
   using X = Rows<XT>;
@@ -398,8 +399,15 @@ __global__ __launch_bounds__(kSumCols * kSumParts) void norm_gain_kernel(const f
 }
 
 // Rows up to which a thread takes one unit where that is enough: few rows wait for their latency, many for memory, and
-// take two.  Bytes of rows from which on they are streamed: what the last-level cache does not keep for the next call.
+// take two.  int8 out of bf16 rows and a residual, us with one and two units: 2048 columns 64 rows 3.4 / 3.7, 512 4.0
+// / 4.4, 768 4.7 / 4.7, 1024 5.8 / 5.3, 4096 15.2 / 12.6; 5120 columns 64 rows 4.1 / 4.3, 256 4.7 / 4.7, 512 7.1 /
+// 6.5, 1024 12.0 / 10.5, 4096 38 / 28.5.  (Long rows would change over at fewer rows: 8192 columns 64 rows 4.7 /
+// 4.2.)
 constexpr int kNormWide = 512;
+// Bytes read by a call from which on its rows are streamed: what the last-level cache does not keep for the next
+// call. Streamed / through the caches, us, bf16 rows of 5120 columns: with a residual 32 MiB read 14.3 / 13.7, 48
+// 19.4 / 19.1, 64 24.1 / 27.2, 80 28.6 / 32.6, 192 60 / 66; without 32 MiB 16.2 / 13.8, 64 26.7 / 27.6, 80 31.8 /
+// 34.1, 128 51.1 / 50.5; the gradient with dh 48 MiB 25.2 / 22.0, 64 28.9 / 27.9, 80 31.4 / 33.3, 192 54 / 61.
 constexpr size_t kNormStream = (size_t)72 << 20;
 
 // Units a thread (0: any number) and threads for rows of so many units.
